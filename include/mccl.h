@@ -573,6 +573,86 @@ int mccl_moe_combine(const void* const* x, const size_t* x_rows, int n, const in
                      const int64_t* src_row, const float* weights, size_t tokens, int topk,
                      size_t hidden_elems, int dtype, void* y, void* stream);
 
+/*
+ * Operators that compute around the exchange (no counterpart in the reference's sources; its users
+ * write them in torch).  Device pointers, the caller's stream, no allocation, no synchronisation, as
+ * everywhere in this header; workspaces are the caller's, 16-byte aligned, hold nothing from one call
+ * to the next and must not be shared by calls that may overlap.
+ *
+ * mccl_embedding: out[i] = scale * table[ids[i] - first_row] for i < n, rounded once, where that row
+ * lies in [0, rows); a row of zeros elsewhere.  table: [rows][hidden], ids: int32 or int64 (id_dtype
+ * MCCL_I32 / MCCL_I64), out: [n][hidden]; bf16 / f16 / f32, any row length, element alignment.  With
+ * first_row a rank looks up its shard of a vocabulary and an all_reduce (SUM) adds the ranks' rows;
+ * ids that mean nothing (-1 for padding) give zeros on every rank.
+ */
+int mccl_embedding(const void* table, size_t rows, const void* ids, int id_dtype, size_t n, int64_t first_row,
+                   size_t hidden, float scale, int dtype, void* out, void* stream);
+
+/*
+ * mccl_sort_ids: the tokens by row.  order (n int64) is the stable ascending order of the rows
+ * ids[i] - first_row, ids outside [0, rows) last; offsets (rows + 1 int64): row v's tokens are
+ * order[offsets[v]] .. order[offsets[v + 1] - 1], in ascending i.  For expert ids it is the send order
+ * of a dispatch (row_index = order / topk) with offsets[v + 1] - offsets[v] pairs for expert v.
+ * n and rows at most 2^31 - 1.  workspace: mccl_sort_ids_workspace(n) bytes (0 for few ids).
+ */
+size_t mccl_sort_ids_workspace(size_t n);
+int mccl_sort_ids(const void* ids, int id_dtype, size_t n, int64_t first_row, size_t rows, void* workspace,
+                  size_t workspace_bytes, int64_t* order, int64_t* offsets, void* stream);
+
+/*
+ * mccl_embedding_grad: the gradient of mccl_embedding in its table (and of mccl_gather_rows in its
+ * source), from the order of mccl_sort_ids: out[v] = scale * sum of grad[order[j]] over
+ * offsets[v] <= j < offsets[v + 1], fp32 sums in an order that only depends on the offsets (the
+ * same bits every time), one rounding.  Rows without a token become zero; with accumulate != 0 the sum
+ * is added to what out holds instead, and rows without a token are not touched.  grad: [n][hidden] in
+ * bf16 / f16 / f32, out: [rows][hidden] in the same type or f32, n at most 2^28.  order must hold indices below n (others
+ * are skipped).  workspace: mccl_embedding_grad_workspace(n, hidden) bytes (0 for few tokens).
+ */
+size_t mccl_embedding_grad_workspace(size_t n, size_t hidden);
+int mccl_embedding_grad(const void* grad, const int64_t* order, const int64_t* offsets, size_t n, size_t rows,
+                        size_t hidden, float scale, int dtype, void* out, int out_dtype, int accumulate,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * mccl_moe_route: per token p = softmax(logits[t]) over the experts, the topk experts with the largest
+ * logits in descending order (ties to the lowest index; -0 equals +0) and their weights: p, or with
+ * normalize != 0 p divided by the sum of the chosen p.  expert_ids (int32) and weights (fp32), both
+ * [tokens][topk], are what mccl_route_counts, mccl_moe_combine and mccl_moe_layer take.  An expert
+ * whose logit is -inf (or NaN) is never chosen; where fewer than topk can be, the rest is id -1 with
+ * weight 0, which those calls skip.  The weights of a row that holds a NaN or +inf are NaN.  logits:
+ * [tokens][experts] in bf16 / f16 / f32, softmax in fp32; experts <= 4096, topk <= 64.
+ *
+ * mccl_moe_route_grad: the gradient in the logits of sum grad_weights * weights for the chosen experts:
+ * with s = sum_k grad_weights[k] * weights[k], p_e * ([e chosen] g_e - s), or with normalize the same
+ * over the chosen experts alone (zero elsewhere).  Ids outside [0, experts) are skipped.  Written in
+ * the logits' type.
+ */
+int mccl_moe_route(const void* logits, size_t tokens, size_t experts, int topk, int normalize, int dtype,
+                   int32_t* expert_ids, float* weights, void* stream);
+int mccl_moe_route_grad(const float* grad_weights, const void* logits, const int32_t* expert_ids, size_t tokens,
+                        size_t experts, int topk, int normalize, int dtype, void* grad_logits, void* stream);
+
+/*
+ * mccl_moe_layer: a whole mixture-of-experts layer for a few tokens, without an exchange:
+ *   out[t] = sum_k weights[t][k] * w_out[e] . (act(w_in[e][0:inter] . x[t]) * (w_in[e][inter:2*inter] . x[t])),
+ * e = expert_ids[t][k] - first_expert, over the k whose e lies in [0, experts), ascending k in fp32, one
+ * rounding; a token without any gets zeros.  x, out: [tokens][hidden]; w_in: [experts][2 * inter][hidden];
+ * w_out: [experts][hidden][inter]; bf16 or f16, hidden and inter multiples of 8, 16-byte aligned.
+ * Every rank that holds `experts` experts from first_expert on calls it with all tokens, and an
+ * all_reduce (SUM) adds the ranks' outputs.  At most 256 tokens, topk <= 64 and 4096 pairs: each
+ * expert's weights are read once for all of its tokens.  The same bits every time.
+ * workspace: mccl_moe_layer_workspace(...) bytes.
+ */
+typedef enum {
+  MCCL_ACT_SILU = 0, /* v * sigmoid(v) */
+  MCCL_ACT_GELU = 1  /* v * (1 + erf(v / sqrt(2))) / 2 */
+} mccl_activation_t;
+size_t mccl_moe_layer_workspace(size_t tokens, int topk, size_t hidden, size_t inter);
+int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int32_t* expert_ids,
+                   const float* weights, size_t tokens, int topk, size_t experts, int64_t first_expert,
+                   size_t hidden, size_t inter, int activation, int dtype, void* out, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
 /* Launch geometry the library would use for mccl_reduce_n (for reports): returns the grid
  * size in workgroups (negative = mccl_status_t) and writes the workgroup size and the
  * dynamic-LDS reservation; count in elements. */

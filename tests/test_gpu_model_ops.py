@@ -1,0 +1,597 @@
+"""The operators that compute around the collectives, against plain implementations in 64 bits:
+embedding and its gradient by sorted tokens, the router and its gradient, the mixture-of-experts layer
+for a few tokens, and runs of them together with the collectives' own calls.
+
+Tolerances count roundings: u = 2^-24 per fp32 operation, eps / 2 for the one rounding to the output's
+type, times the sums of absolute values that the roundings act on."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+FLOATS = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def gen(*key):
+    return torch.Generator().manual_seed(hash(tuple(int(k) for k in key)) % (1 << 31))
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def within(got, want, tol, what=""):
+    got, want = got.detach().cpu().double(), want.double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    bad = ~((got - want).abs() <= tol)
+    if bad.any():
+        i = tuple(int(v) for v in torch.nonzero(bad)[0])
+        raise AssertionError("%s: %d of %d off; first at %s: got %r want %r tolerance %r" % (
+            what, int(bad.sum()), bad.numel(), i, float(got[i]), float(want[i]), float(torch.as_tensor(tol).expand_as(want)[i])))
+
+
+def keys_of(ids, first, rows):
+    r = ids.long() - first
+    return torch.where((r >= 0) & (r < rows), r, torch.full_like(r, rows))
+
+
+# ---------------------------------------------------------------------------------------------
+# embedding
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", FLOATS, ids=str)
+@pytest.mark.parametrize("n,rows,hidden,first", [(1, 1, 1, 0), (3, 7, 5, 0), (8, 100, 64, 40), (257, 50, 521, -3), (1000, 333, 4096, 5),
+                                                 (33, 10, 7168, 0), (5, 3, 8 * 64 * 4 + 7, 1)])
+@pytest.mark.parametrize("id_dtype", [torch.int32, torch.int64], ids=str)
+def test_embedding_is_the_scaled_row_or_zero(mccl, dtype, id_dtype, n, rows, hidden, first):
+    """Bit for bit: one fp32 product, one rounding.  Ids below, above and far outside the shard give zeros."""
+    g = gen(n, rows, hidden, first)
+    table = torch.randn(rows, hidden, generator=g).to(dtype)
+    ids = torch.randint(first - 2, first + rows + 2, (n,), generator=g)
+    info = torch.iinfo(id_dtype)
+    for i, v in enumerate((info.min, info.max, -1)):
+        if i + 1 < n:
+            ids[i + 1] = v
+    scale = 1.0 / 3.0
+    out = mccl.embedding(table.to(DEV), ids.to(id_dtype).to(DEV), scale=scale, first_row=first)
+    key = torch.tensor([int(v) - first if 0 <= int(v) - first < rows else rows for v in ids])
+    padded = torch.cat([table, torch.zeros(1, hidden, dtype=dtype)])
+    want = (padded[key].float() * torch.tensor(scale, dtype=torch.float32)).to(dtype)
+    assert out.dtype == dtype and torch.equal(out.cpu(), want)
+
+
+@pytest.mark.parametrize("src_off,dst_off", [(1, 0), (0, 3), (5, 1)])
+@pytest.mark.parametrize("hidden", [8, 24, 33, 1024])
+def test_embedding_at_any_alignment_leaves_the_neighbours_alone(mccl, src_off, dst_off, hidden):
+    g = gen(src_off, dst_off, hidden)
+    rows, n, dtype = 19, 40, torch.bfloat16
+    table = torch.randn(src_off + rows * hidden, generator=g).to(dtype).to(DEV)
+    buf = torch.full((dst_off + n * hidden + 40,), 7.0, dtype=dtype, device=DEV)
+    t, o = table[src_off:].view(rows, hidden), buf[dst_off:dst_off + n * hidden].view(n, hidden)
+    ids = torch.randint(0, rows, (n,), generator=g).to(DEV)
+    mccl.embedding(t, ids, out=o)
+    assert torch.equal(o, t[ids])
+    assert bool((buf[:dst_off] == 7).all()) and bool((buf[dst_off + n * hidden:] == 7).all())
+
+
+def test_embedding_shapes_empty_lists_and_an_empty_shard(mccl):
+    table = torch.randn(6, 16, generator=gen(1)).to(DEV)
+    ids = torch.tensor([[0, 5], [9, -1]], device=DEV)
+    out = mccl.embedding(table, ids)
+    assert out.shape == (2, 2, 16) and torch.equal(out[0], table[[0, 5]]) and not out[1].any()
+    assert mccl.embedding(table, ids[:0]).shape == (0, 2, 16)
+    assert not mccl.embedding(table[:0], ids).any()
+
+
+def test_embedding_of_values_that_are_not_finite(mccl):
+    table = torch.tensor([[float("inf"), float("-inf"), float("nan"), 3e38]] * 2, device=DEV)
+    out = mccl.embedding(table, torch.tensor([1, 7], device=DEV), scale=2.0).cpu()
+    assert out[0, 0] == float("inf") and out[0, 1] == float("-inf") and out[0, 2].isnan() and out[0, 3] == float("inf")
+    assert not out[1].any()
+
+
+def test_embedding_rows_past_4_gib(mccl):
+    """Offsets that need more than 32 bits, in the table and in the output."""
+    hidden = 8192
+    rows = (5 << 30) // (2 * hidden)
+    table = torch.zeros(rows, hidden, dtype=torch.bfloat16, device=DEV)
+    marks = torch.arange(1, 9, device=DEV, dtype=torch.bfloat16)
+    at = torch.tensor([0, 1, rows // 2, rows - 3, rows - 2, rows - 1, rows // 3, 5], device=DEV)
+    table[at] = marks[:, None].expand(8, hidden)
+    n = rows + 11
+    ids = torch.full((n,), 2, device=DEV)
+    ids[torch.arange(0, 8, device=DEV) * ((n - 1) // 7)] = at
+    out = mccl.embedding(table, ids)
+    assert torch.equal(out[torch.arange(0, 8, device=DEV) * ((n - 1) // 7), -1], marks)
+    assert int((out[:, 0] != 0).sum()) == 8
+
+
+# ---------------------------------------------------------------------------------------------
+# sort
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n", [0, 1, 2, 64, 255, 256, 257, 2047, 2048, 2049, 4096, 5000, 65537, 1_000_003])
+@pytest.mark.parametrize("rows,first", [(1, 0), (8, -2), (255, 0), (256, 1), (50_000, 10), (3_000_000, 0)])
+def test_sort_ids_is_the_stable_order(mccl, n, rows, first):
+    g = gen(n, rows)
+    ids = torch.randint(first - 1 - rows // 8, first + rows + 2 + rows // 8, (n,), generator=g)
+    if n > 100:
+        ids[torch.rand(n, generator=g) < 0.3] = first + rows // 2
+    order, offsets = mccl.sort_ids(ids.to(torch.int32).to(DEV) if n % 2 else ids.to(DEV), rows, first_row=first)
+    key = keys_of(ids, first, rows)
+    in_order, want = torch.sort(key, stable=True)
+    assert torch.equal(order.cpu(), want)
+    assert torch.equal(offsets.cpu(), torch.searchsorted(in_order, torch.arange(rows + 1)))
+
+
+def test_sort_ids_without_rows_and_with_far_ids(mccl):
+    info = torch.iinfo(torch.int64)
+    ids = torch.tensor([info.max, 5, info.min, 4, 5, -1], device=DEV)
+    order, offsets = mccl.sort_ids(ids, 0)
+    assert order.tolist() == [0, 1, 2, 3, 4, 5] and offsets.tolist() == [0]
+    order, offsets = mccl.sort_ids(ids, 2, first_row=4)
+    assert order.tolist() == [3, 1, 4, 0, 2, 5] and offsets.tolist() == [0, 1, 3]
+    order, offsets = mccl.sort_ids(ids, 4, first_row=info.min)  # a range at the very end of the type
+    assert order.tolist() == [2, 0, 1, 3, 4, 5] and offsets.tolist() == [0, 1, 1, 1, 1]
+
+
+# ---------------------------------------------------------------------------------------------
+# embedding gradient
+# ---------------------------------------------------------------------------------------------
+def grad_reference(grad, ids, first, rows, scale):
+    """(sum, tolerance of the fp32 sum): m terms, at most m roundings of partial sums of the absolute
+    values, one of the scaling."""
+    key = keys_of(ids, first, rows)
+    inside = key < rows
+    total = torch.zeros(rows, grad.shape[1], dtype=torch.float64)
+    size, count = torch.zeros_like(total), torch.zeros(rows, 1, dtype=torch.float64)
+    total.index_add_(0, key[inside], grad[inside].double())
+    size.index_add_(0, key[inside], grad[inside].double().abs())
+    count.index_add_(0, key[inside], torch.ones(int(inside.sum()), 1, dtype=torch.float64))
+    s = float(torch.tensor(scale, dtype=torch.float32))
+    return total * s, (count + 1) * U * size * abs(s)
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16),
+                                             (torch.float16, torch.float32), (torch.float32, torch.float32)], ids=str)
+@pytest.mark.parametrize("n,rows,hidden,hot", [(0, 5, 16, 0.0), (1, 1, 1, 0.0), (64, 3, 40, 1.0), (65, 3, 40, 1.0), (128, 2, 7, 0.5),
+                                               (1000, 40, 521, 0.6), (3000, 500, 264, 0.2), (700, 20, 2056, 0.3), (9000, 7, 130, 0.0)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_embedding_grad(mccl, dtype, out_dtype, n, rows, hidden, hot, accumulate):
+    """Rows without a token, with one, with more than one piece of the sorted tokens holds, and rows that
+    begin and end inside a piece; added into a gradient or written over one that holds NaN."""
+    g = gen(n, rows, hidden, int(accumulate))
+    grad = torch.randn(n, hidden, generator=g).to(dtype)
+    first, scale = 3, 1.5 if n % 2 else 1.0 / 3.0
+    ids = torch.randint(first - 1, first + rows + 1, (n,), generator=g)
+    ids[torch.rand(n, generator=g) < hot] = first + rows // 2
+    old = torch.randn(rows, hidden, generator=g).to(out_dtype) if accumulate else torch.full((rows, hidden), float("nan"), dtype=out_dtype)
+    plan = mccl.sort_ids(ids.to(DEV), rows, first_row=first)
+    out = old.to(DEV)
+    mccl.embedding_grad(grad.to(DEV), plan, scale=scale, out=out, accumulate=accumulate)
+    want, tol = grad_reference(grad, ids, first, rows, scale)
+    if accumulate:
+        touched = torch.zeros(rows + 1, dtype=torch.bool)
+        touched[keys_of(ids, first, rows)] = True
+        assert torch.equal(out.cpu()[~touched[:-1]], old[~touched[:-1]]), "rows without a token"
+        want = want + old.double()
+        tol = tol + U * want.abs()
+    within(out, want, tol + half_step(out_dtype) * (want.abs() + tol) + torch.finfo(out_dtype).smallest_normal * half_step(out_dtype), "grad")
+
+
+def test_embedding_grad_gives_the_same_bits_every_time_and_for_any_split(mccl):
+    g = gen(5)
+    n, rows, hidden = 20000, 300, 200
+    grad = torch.randn(n, hidden, generator=g).to(DEV)
+    ids = torch.randint(0, rows, (n,), generator=g)
+    ids[torch.rand(n, generator=g) < 0.4] = 17
+    plan = mccl.sort_ids(ids.to(DEV), rows)
+    one = mccl.embedding_grad(grad, plan)
+    for _ in range(3):
+        assert torch.equal(one, mccl.embedding_grad(grad, plan))
+
+
+def test_embedding_grad_is_the_derivative(mccl):
+    """Against central differences of a loss through the lookup itself (fp32 table, linear in it: exact
+    but for roundings of the loss, 2^-24 of the sum of its terms' sizes over the step)."""
+    g = gen(8)
+    rows, hidden, n, scale = 9, 24, 50, 0.75
+    table = torch.randn(rows, hidden, generator=g).to(DEV)
+    ids = torch.randint(-1, rows + 1, (n,), generator=g).to(DEV)
+    up = torch.randn(n, hidden, generator=g).to(DEV)
+    grad = mccl.embedding_grad(up, mccl.sort_ids(ids, rows), scale=scale)
+    step = 0.5
+    for v in range(rows):
+        delta = torch.randn(hidden, generator=g).to(DEV)
+        sides = []
+        for sign in (1, -1):
+            moved = table.clone()
+            moved[v] += sign * step * delta
+            sides.append((mccl.embedding(moved, ids, scale=scale).double() * up.double()).sum())
+        slope = float((sides[0] - sides[1]) / (2 * step))
+        size = float((up.double().abs().sum(dim=1) * (ids == v)).sum() * 4 * 4) + 1.0
+        assert abs(slope - float((grad[v].double() * delta.double()).sum())) <= 100 * U * size, v
+
+
+def test_embedding_grad_skips_what_a_foreign_plan_points_past(mccl):
+    """Indices and offsets outside the gradient are not followed."""
+    grad = torch.ones(4, 8, device=DEV)
+    order = torch.tensor([0, 99, -5, 3], device=DEV)
+    offsets = torch.tensor([0, 2, 1 << 40], device=DEV)
+    out = mccl.embedding_grad(grad, (order, offsets))
+    assert out[:, 0].tolist() == [1.0, 1.0]
+
+
+# ---------------------------------------------------------------------------------------------
+# router
+# ---------------------------------------------------------------------------------------------
+def route_reference(logits, topk, normalize):
+    l = logits.double()
+    ids = torch.argsort(torch.where(l.isnan(), torch.full_like(l, float("-inf")), -(-l)).neg(), dim=1, stable=True)[:, :topk]
+    value = l.gather(1, ids)
+    closed = (value == float("-inf")) | value.isnan()
+    p = torch.softmax(l, dim=1)
+    w = p.gather(1, ids)
+    w = torch.where(closed, torch.zeros_like(w), w)
+    if normalize:
+        w = w / w.sum(dim=1, keepdim=True)
+    w = torch.where(closed, torch.zeros_like(w), w)
+    return torch.where(closed, torch.full_like(ids, -1), ids).int(), w
+
+
+ROUTES = [(1, 1, 1), (7, 5, 5), (16, 64, 6), (33, 65, 3), (50, 100, 8), (200, 256, 8), (9, 257, 8), (40, 512, 4), (5, 1000, 64), (3, 4096, 10)]
+
+
+@pytest.mark.parametrize("dtype", FLOATS, ids=str)
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("tokens,experts,topk", ROUTES)
+def test_route_and_its_gradient(mccl, dtype, normalize, tokens, experts, topk):
+    """Choices equal, weights within: the difference to the largest logit, exp (2 u), a sum over the
+    lane's share and six steps, a division.  Every third token has closed experts; ties are frequent in
+    the 16-bit types."""
+    g = gen(tokens, experts, topk, int(normalize))
+    logits = (3.0 * torch.randn(tokens, experts, generator=g)).to(dtype)
+    closed = torch.rand(tokens, experts, generator=g) < 0.4
+    closed[torch.arange(tokens) % 3 != 1] = False
+    closed[:, 0] = False
+    logits[closed] = float("-inf")
+    ids, weights = mccl.moe_route(logits.to(DEV), topk, normalize=normalize)
+    want_ids, want = route_reference(logits, topk, normalize)
+    assert torch.equal(ids.cpu(), want_ids)
+    per_lane = max(1, 1 << max(0, math.ceil(math.log2(experts / 64))))
+    span = 30.0 + per_lane + topk
+    within(weights, want, (span + 20) * U * want, "weights")
+
+    up = torch.randn(tokens, topk, generator=g)
+    d = mccl.moe_route_grad(up.to(DEV), logits.to(DEV), ids, normalize=normalize)
+    at = logits.double().clone().requires_grad_(True)
+    # normalised: p / sum of the chosen p is the softmax of the chosen alone, whose derivative elsewhere is 0 exactly
+    q = torch.softmax(at.gather(1, want_ids.long().clamp(min=0)).masked_fill(want_ids < 0, float("-inf")), dim=1) if normalize \
+        else torch.softmax(at, dim=1).gather(1, want_ids.long().clamp(min=0))
+    q = torch.where(want_ids >= 0, q, torch.zeros_like(q))
+    (q * up.double()).sum().backward()
+    chosen = torch.where(want_ids >= 0, want, torch.zeros_like(want))
+    mean_size = (chosen * up.double().abs()).sum(dim=1, keepdim=True)
+    own = torch.zeros(tokens, experts, dtype=torch.float64).scatter_add(1, want_ids.long().clamp(min=0), torch.where(want_ids >= 0, up.double().abs(), torch.zeros_like(want)))
+    p = torch.softmax(logits.double(), dim=1) if not normalize else torch.zeros(tokens, experts, dtype=torch.float64).scatter_add(1, want_ids.long().clamp(min=0), chosen)
+    tol = 2 * (span + 20) * U * p * (own + mean_size)
+    within(d, at.grad, tol + half_step(dtype) * (at.grad.abs() + tol) + torch.finfo(dtype).smallest_normal * half_step(dtype), "grad")
+
+
+@pytest.mark.parametrize("normalize", [True, False])
+def test_route_gradient_against_differences(mccl, normalize):
+    """fp32 weights of logits moved by 2^-6 either way: the third derivative's part is below
+    step^2 * sum |g|, the roundings' below 40 u * sum |g| / step."""
+    g = gen(77)
+    tokens, experts, topk, step = 6, 40, 4, 2.0 ** -6
+    logits = torch.randn(tokens, experts, generator=g)
+    top = torch.argsort(logits, dim=1, descending=True)
+    logits.scatter_add_(1, top[:, :topk], torch.full((tokens, topk), 0.5))  # no choice changes within the step
+    up = torch.randn(tokens, topk, generator=g)
+    ids, _ = mccl.moe_route(logits.to(DEV), topk, normalize=normalize)
+    d = mccl.moe_route_grad(up.to(DEV), logits.to(DEV), ids, normalize=normalize).cpu().double()
+    for trial in range(4):
+        way = torch.randn(tokens, experts, generator=g).clamp(-2, 2)
+        sides = []
+        for sign in (1, -1):
+            i2, w2 = mccl.moe_route((logits + sign * step * way).to(DEV), topk, normalize=normalize)
+            # the same experts, perhaps in another order: the weight of each choice of ids
+            at = torch.zeros(tokens, experts, dtype=torch.float64).scatter(1, i2.cpu().long(), w2.cpu().double())
+            assert torch.equal(torch.sort(i2.cpu(), dim=1).values, torch.sort(ids.cpu(), dim=1).values)
+            sides.append((at.gather(1, ids.cpu().long()) * up.double()).sum(dim=1))
+        slope = (sides[0] - sides[1]) / (2 * step)
+        size = up.double().abs().sum(dim=1)
+        within(slope, (d * way.double()).sum(dim=1), 8 * step * step * size + 60 * U * size / step, "differences")
+
+
+def test_route_ties_masks_and_values_that_are_not_finite(mccl):
+    inf, nan = float("inf"), float("nan")
+    low = torch.finfo(torch.float32).min
+    rows = [
+        [1.0, 1.0, 1.0, 1.0, 1.0],          # all equal: lowest indices
+        [-0.0, 0.0, -0.0, -1.0, 0.0],       # -0 equals +0
+        [-inf] * 5,                         # nothing open
+        [-inf, -inf, 2.0, -inf, -inf],      # one open
+        [low, low, low, low, low],          # the type's lowest value is a logit like any other
+        [nan, 1.0, 2.0, 0.0, 0.0],          # NaN: not chosen, weights NaN
+        [inf, 1.0, 2.0, 0.0, 0.0],          # +inf: chosen, weights NaN
+        [low, 5.0, low, low, -inf],
+    ]
+    logits = torch.tensor(rows, device=DEV)
+    for normalize in (True, False):
+        ids, w = mccl.moe_route(logits, 3, normalize=normalize)
+        assert ids.tolist() == [[0, 1, 2], [0, 1, 2], [-1] * 3, [2, -1, -1], [0, 1, 2], [2, 1, 3], [0, 2, 1], [1, 0, 2]]
+        w = w.cpu()
+        even = 1.0 / 3.0 if normalize else 0.2
+        within(w[0], torch.full((3,), even), 4 * U, "even")
+        within(w[4], torch.full((3,), even), 4 * U, "lowest")
+        assert w[2].tolist() == [0, 0, 0] and w[3].tolist() == [1, 0, 0] and w[7].tolist() == [1, 0, 0]
+        assert w[5].isnan().all() and w[6].isnan().all()
+        d = mccl.moe_route_grad(torch.ones(8, 3, device=DEV), logits, ids, normalize=normalize).cpu()
+        assert not d[2].any() and not d[3].any(), "no gradient where nothing, or only one expert, was open"
+        assert torch.isfinite(d[4]).all()
+
+
+def test_route_gradient_of_repeated_and_foreign_ids(mccl):
+    """The same expert twice gets both gradients; ids outside are skipped."""
+    logits = torch.tensor([[0.0, 1.0, 2.0, 0.5]], device=DEV)
+    g = torch.tensor([[1.0, 3.0, 100.0, 50.0]], device=DEV)
+    ids = torch.tensor([[2, 2, 4, -7]], dtype=torch.int32, device=DEV)
+    d = mccl.moe_route_grad(g, logits, ids, normalize=False).cpu().double()[0]
+    p = torch.softmax(logits.cpu().double()[0], dim=0)
+    want = -p * (4 * p[2])
+    want[2] += 4 * p[2]
+    within(d, want, 40 * U * 4 * torch.ones(4), "repeated")
+
+
+# ---------------------------------------------------------------------------------------------
+# mixture-of-experts layer
+# ---------------------------------------------------------------------------------------------
+def act64(v, name):
+    return v / (1 + torch.exp(-v)) if name == "silu" else 0.5 * v * torch.erfc(-v / math.sqrt(2.0))
+
+
+def layer_reference(x, w_in, w_out, ids, weights, first, activation, dtype):
+    """(out, tolerance) in 64 bits.  gate and up: hidden roundings of the fp32 sum of |w x| (the slope of
+    either activation is below 1.2); h is rounded once to the layer's type; the second product has inter
+    roundings, the weighted sum topk + 1, the output one half step."""
+    T, H = x.shape
+    E, I = w_out.shape[0], w_out.shape[2]
+    out, tol = torch.zeros(T, H, dtype=torch.float64), torch.zeros(T, H, dtype=torch.float64)
+    size = torch.zeros_like(out)
+    tiny = torch.finfo(dtype).smallest_normal * half_step(dtype)
+    for t in range(T):
+        for k in range(ids.shape[1]):
+            e = int(ids[t, k]) - first
+            if not 0 <= e < E:
+                continue
+            a, b, xt, w = w_in[e].double(), w_out[e].double(), x[t].double(), float(weights[t, k])
+            s, ds = a @ xt, (H + 1) * U * (a.abs() @ xt.abs())
+            act = act64(s[:I], activation)
+            h = act * s[I:]
+            dh = (1.2 * ds[:I] + 8 * U * act.abs()) * (s[I:].abs() + ds[I:]) + act.abs() * ds[I:]
+            dh = dh + half_step(dtype) * (h.abs() + dh) + tiny
+            y, dy = b @ h, b.abs() @ dh + (I + 1) * U * (b.abs() @ (h.abs() + dh))
+            out[t] += w * y
+            size[t] += abs(w) * (y.abs() + dy)
+            tol[t] += abs(w) * dy
+    tol = tol + (ids.shape[1] + 1) * U * size
+    return out, tol + half_step(dtype) * (out.abs() + tol) + tiny
+
+
+def layer_inputs(g, T, k, E, local, H, I, dtype):
+    x = torch.randn(T, H, generator=g).to(dtype)
+    w_in = (torch.randn(local, 2 * I, H, generator=g) / math.sqrt(H)).to(dtype)
+    w_out = (torch.randn(local, H, I, generator=g) / math.sqrt(I)).to(dtype)
+    ids = torch.argsort(torch.rand(T, E, generator=g), dim=1)[:, :k].to(torch.int32).contiguous()
+    weights = torch.softmax(torch.randn(T, k, generator=g), dim=1).contiguous()
+    return x, w_in, w_out, ids, weights
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("T,k,E,local,first,H,I", [
+    (1, 1, 1, 1, 0, 8, 8), (1, 8, 64, 64, 0, 256, 64), (2, 2, 4, 4, 0, 40, 24), (5, 3, 34, 34, 0, 520, 200), (16, 2, 3, 3, 0, 64, 128),
+    (17, 1, 1, 1, 0, 72, 16), (31, 4, 16, 4, 8, 136, 88), (64, 2, 2, 2, 0, 32, 40), (3, 64, 70, 70, 0, 48, 16), (100, 6, 12, 5, 3, 264, 72),
+    (256, 2, 4, 4, 0, 96, 56), (7, 2, 40, 10, 20, 1032, 328), (33, 1, 2, 1, 1, 1024, 512), (2, 1, 300, 300, 0, 16, 2056)])
+def test_moe_layer(mccl, dtype, activation, T, k, E, local, first, H, I):
+    g = gen(T, k, E, H, I)
+    x, w_in, w_out, ids, weights = layer_inputs(g, T, k, E, local, H, I, dtype)
+    if T > 2:
+        ids[1] = -1                      # padding
+        ids[2] = ids[2, 0]               # the same expert topk times
+        x[1] = float("nan")              # what padding holds does not matter
+        weights[1] = float("nan")
+    out = torch.full((T, H), float("nan"), dtype=dtype, device=DEV)
+    mccl.moe_layer(x.to(DEV), w_in.to(DEV), w_out.to(DEV), ids.to(DEV), weights.to(DEV), first_expert=first, activation=activation, out=out)
+    want, tol = layer_reference(x, w_in, w_out, ids, weights, first, activation, dtype)
+    within(out, want, tol, "layer")
+
+
+def test_moe_layer_without_any_pair_is_zero_and_no_tokens_are_no_work(mccl):
+    g = gen(3)
+    x, w_in, w_out, ids, weights = [t.to(DEV) for t in layer_inputs(g, 4, 2, 6, 2, 64, 32, torch.bfloat16)]
+    assert not mccl.moe_layer(x, w_in, w_out, torch.full_like(ids, -1), weights).any()
+    assert not mccl.moe_layer(x, w_in, w_out, ids, weights, first_expert=1 << 40).any()
+    assert not mccl.moe_layer(x, w_in, w_out, ids, weights, first_expert=-(1 << 62)).any()
+    assert mccl.moe_layer(x[:0], w_in, w_out, ids[:0], weights[:0]).shape == (0, 64)
+
+
+def test_moe_layer_keeps_other_tokens_apart_from_one_that_is_not_finite(mccl):
+    """A token with infinities or NaN changes its own output alone, also where it shares an expert."""
+    g = gen(4)
+    x, w_in, w_out, ids, weights = layer_inputs(g, 20, 2, 3, 3, 128, 64, torch.bfloat16)
+    args = [w_in.to(DEV), w_out.to(DEV), ids.to(DEV), weights.to(DEV)]
+    clean = mccl.moe_layer(x.to(DEV), *args)
+    x[7, 5], x[12] = float("inf"), float("nan")
+    out = mccl.moe_layer(x.to(DEV), *args)
+    keep = [t for t in range(20) if t not in (7, 12)]
+    assert torch.equal(out[keep], clean[keep]) and not torch.isfinite(out[12].float()).any()
+
+
+def test_moe_layer_weights_past_4_gib(mccl):
+    """Experts behind the first 4 GiB of weights."""
+    H, I, E, T = 4096, 4096, 70, 3
+    w_in = torch.zeros(E, 2 * I, H, dtype=torch.bfloat16, device=DEV)
+    w_out = torch.zeros(E, H, I, dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    last = E - 1
+    w_in[last].normal_(0, 1 / math.sqrt(H), generator=g)
+    w_out[last].normal_(0, 1 / math.sqrt(I), generator=g)
+    x = torch.randn(T, H, generator=gen(10)).to(torch.bfloat16)
+    ids = torch.tensor([[last], [0], [last]], dtype=torch.int32)
+    weights = torch.ones(T, 1)
+    out = mccl.moe_layer(x.to(DEV), w_in, w_out, ids.to(DEV), weights.to(DEV))
+    want, tol = layer_reference(x, w_in[last:].cpu(), w_out[last:].cpu(), ids, weights, last, "silu", torch.bfloat16)
+    within(out, want, tol, "layer")
+
+
+def test_moe_layer_gives_the_same_bits_every_time(mccl):
+    g = gen(11)
+    args = [t.to(DEV) for t in layer_inputs(g, 40, 4, 8, 8, 512, 256, torch.bfloat16)]
+    one = mccl.moe_layer(*args)
+    for _ in range(5):
+        assert torch.equal(one, mccl.moe_layer(*args))
+
+
+# ---------------------------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------------------------
+def test_route_then_layer_equals_dispatch_experts_combine(mccl):
+    """One decode step both ways: moe_layer, and sort_ids + gather_rows + the experts in torch +
+    moe_combine.  Both are within their tolerance of the definition."""
+    g = gen(21)
+    T, k, E, H, I, dtype = 24, 4, 16, 256, 96, torch.bfloat16
+    x, w_in, w_out, _, _ = layer_inputs(g, T, k, E, E, H, I, dtype)
+    logits = torch.randn(T, E, generator=g)
+    ids, weights = mccl.moe_route(logits.to(DEV), k)
+    out = mccl.moe_layer(x.to(DEV), w_in.to(DEV), w_out.to(DEV), ids, weights)
+    want, tol = layer_reference(x, w_in, w_out, ids.cpu(), weights.cpu(), 0, "silu", dtype)
+    within(out, want, tol, "layer")
+
+    order, offsets = mccl.sort_ids(ids.reshape(-1), E)
+    assert torch.equal(offsets.diff(), mccl.route_counts(ids.reshape(-1), E))
+    sent = mccl.gather_rows(x.to(DEV), torch.div(order, k, rounding_mode="floor"))
+    back = torch.empty_like(sent)
+    at = offsets.tolist()
+    for e in range(E):
+        s = sent[at[e]:at[e + 1]].float() @ w_in[e].to(DEV).float().t().contiguous()
+        h = (torch.nn.functional.silu(s[:, :I]) * s[:, I:]).to(dtype).float()
+        back[at[e]:at[e + 1]] = (h @ w_out[e].to(DEV).float().t().contiguous()).to(dtype)
+    row = torch.empty_like(order)
+    row[order] = torch.arange(T * k, device=DEV)
+    y = mccl.moe_combine([back], torch.zeros(T, k, dtype=torch.int32, device=DEV), row.view(T, k).contiguous(), weights)
+    # the exchanged rows are rounded once more, to the layer's type
+    within(y, want, tol + half_step(dtype) * 2 * (want.abs() + 4 * tol) + half_step(dtype) * 8, "combine")
+
+
+def test_expert_parallel_ranks_add_up_to_the_layer(mccl):
+    """Four ranks with a quarter of the experts each, their outputs added by reduce_n as the all_reduce
+    of the group adds them: within one half step per rank of the definition."""
+    g = gen(22)
+    T, k, E, H, I, W, dtype = 12, 4, 16, 264, 72, 4, torch.float16
+    x, w_in, w_out, ids, weights = layer_inputs(g, T, k, E, E, H, I, dtype)
+    per = E // W
+    parts = [mccl.moe_layer(x.to(DEV), w_in[r * per:(r + 1) * per].contiguous().to(DEV), w_out[r * per:(r + 1) * per].contiguous().to(DEV),
+                            ids.to(DEV), weights.to(DEV), first_expert=r * per) for r in range(W)]
+    total = mccl.reduce_n(parts)
+    want, tol = layer_reference(x, w_in, w_out, ids, weights, 0, "silu", dtype)
+    sizes = sum(p.cpu().double().abs() for p in parts)
+    within(total, want, tol + half_step(dtype) * 2 * sizes, "sum of the ranks")
+
+
+def test_vocabulary_shards_add_up_to_the_lookup_and_its_gradient(mccl):
+    """Every id is in exactly one shard: the sum over the ranks is the lookup bit for bit (0 + x), and
+    each rank's gradient is its rows of the whole table's."""
+    g = gen(23)
+    W, per, hidden, n, dtype = 4, 50, 136, 300, torch.bfloat16
+    table = torch.randn(W * per, hidden, generator=g).to(dtype).to(DEV)
+    ids = torch.randint(0, W * per, (n,), generator=g).to(DEV)
+    shards = [table[r * per:(r + 1) * per].contiguous() for r in range(W)]
+    parts = [mccl.embedding(s, ids, scale=0.5, first_row=r * per) for r, s in enumerate(shards)]
+    assert torch.equal(mccl.reduce_n(parts), mccl.embedding(table, ids, scale=0.5))
+    up = torch.randn(n, hidden, generator=g).to(dtype).to(DEV)
+    whole = mccl.embedding_grad(up, mccl.sort_ids(ids, W * per), scale=0.5)
+    for r in range(W):
+        part = mccl.embedding_grad(up, mccl.sort_ids(ids, per, first_row=r * per), scale=0.5)
+        within(part, whole[r * per:(r + 1) * per].cpu(), 4 * half_step(dtype) * (whole[r * per:(r + 1) * per].cpu().double().abs() + 1), "rank %d" % r)
+
+
+def test_gradient_of_the_token_permute(mccl):
+    """gather_rows' gradient: what autograd gives for the indexing itself, in 64 bits."""
+    g = gen(24)
+    T, k, hidden = 60, 4, 200
+    src = torch.randn(T, hidden, generator=g, dtype=torch.float64, requires_grad=True)
+    index = torch.randperm(T * k, generator=g) % T
+    up = torch.randn(T * k, hidden, generator=g)
+    (src[index] * up.double()).sum().backward()
+    rows = mccl.gather_rows(src.detach().float().to(DEV), index.to(DEV))
+    assert torch.equal(rows.cpu(), src.detach().float()[index])
+    d = mccl.embedding_grad(up.to(DEV), mccl.sort_ids(index.to(DEV), T))
+    size = torch.zeros(T, hidden, dtype=torch.float64).index_add_(0, index, up.double().abs())
+    within(d, src.grad, (k + 1) * U * size, "permute")
+
+
+def test_replayed_from_a_graph_on_a_stream_of_their_own(mccl):
+    """A router, layer, lookup and gradient step recorded once and replayed with new inputs, with eager
+    work in between: every replay equals the eager result bit for bit."""
+    g = gen(31)
+    T, k, E, H, I, V, dtype = 6, 2, 8, 128, 64, 40, torch.bfloat16
+    _, w_in, w_out, _, _ = [t.to(DEV) for t in layer_inputs(g, T, k, E, E, H, I, dtype)]
+    table = torch.randn(V, H, generator=g).to(dtype).to(DEV)
+    ids = torch.zeros(5000, dtype=torch.int64, device=DEV)
+    up = torch.zeros(5000, H, dtype=dtype, device=DEV)
+    logits = torch.zeros(T, E, device=DEV)
+
+    def step():
+        x = mccl.embedding(table, ids[:T], scale=2.0)
+        chosen, w = mccl.moe_route(logits, k)
+        y = mccl.moe_layer(x, w_in, w_out, chosen, w)
+        d = mccl.embedding_grad(up, mccl.sort_ids(ids, V), scale=2.0)
+        dl = mccl.moe_route_grad(w, logits, chosen)
+        return x, chosen, w, y, d, dl
+
+    def fill(seed):
+        gs = gen(seed)
+        ids.copy_(torch.randint(-1, V + 1, (5000,), generator=gs))
+        up.copy_(torch.randn(5000, H, generator=gs))
+        logits.copy_(torch.randn(T, E, generator=gs))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        fill(1)
+        step()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = step()
+        for seed in (2, 3, 4):
+            fill(seed)
+            graph.replay()
+            side.synchronize()
+            got = [t.clone() for t in held]
+            for a, b in zip(got, step()):
+                assert torch.equal(a, b)
+            graph.replay()
+            side.synchronize()
+            for a, b in zip(held, got):
+                assert torch.equal(a, b)
+
+
+def test_workspaces_of_the_caller_are_used_and_may_be_dirty(mccl):
+    from torch_ccl_amd import capi
+    g = gen(41)
+    x, w_in, w_out, ids, weights = [t.to(DEV) for t in layer_inputs(g, 9, 3, 8, 8, 64, 40, torch.bfloat16)]
+    need = capi.lib().mccl_moe_layer_workspace(9, 3, 64, 40)
+    ws = torch.full((need,), 0xFF, dtype=torch.uint8, device=DEV)
+    assert torch.equal(mccl.moe_layer(x, w_in, w_out, ids, weights, workspace=ws), mccl.moe_layer(x, w_in, w_out, ids, weights))
+    tokens = torch.randint(0, 30, (4000,), generator=g).to(DEV)
+    ws = torch.full((capi.lib().mccl_sort_ids_workspace(4000),), 0xFF, dtype=torch.uint8, device=DEV)
+    a, b = mccl.sort_ids(tokens, 30, workspace=ws), mccl.sort_ids(tokens, 30)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    up = torch.randn(4000, 72, generator=g).to(DEV)
+    ws = torch.full((capi.lib().mccl_embedding_grad_workspace(4000, 72),), 0xFF, dtype=torch.uint8, device=DEV)
+    assert torch.equal(mccl.embedding_grad(up, a, workspace=ws), mccl.embedding_grad(up, b))

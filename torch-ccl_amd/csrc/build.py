@@ -21,12 +21,14 @@ LIB_DIR = os.path.join(os.path.dirname(HERE), "torch_ccl_amd", "lib")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 KERNEL_SRC = os.path.join(HERE, "mccl_kernels.hip")          # planning, C ABI, copy and MoE kernels
+MODEL_SRC = os.path.join(HERE, "mccl_model.hip")             # embedding, router, mixture-of-experts layer
 REDUCE_SRC = os.path.join(HERE, "mccl_reduce_dtype.hip")     # reduction kernels, one object per dtype
 REDUCE_DTYPES = range(9)                                      # mccl_dtype_t codes
 KERNEL_LIB = os.path.join(LIB_DIR, "libmi355ccl.so")
 KERNEL_HDRS = [os.path.join(INCLUDE, "mccl.h")] + [
     os.path.join(HERE, h) for h in ("kernels_common.hpp", "kernels_reduce.hpp", "kernels_copy.hpp",
-                                    "kernels_moe.hpp", "kernels_sync.hpp", "kernels_fused.hpp", "kernels_xrank.hpp", "reduce_launch.hpp")]
+                                    "kernels_moe.hpp", "kernels_sync.hpp", "kernels_fused.hpp", "kernels_xrank.hpp", "reduce_launch.hpp",
+                                    "host_checks.hpp", "kernels_embedding.hpp", "kernels_router.hpp", "kernels_layer.hpp")]
 
 # -ffp-contract=off / no fast-math: the reduction chain must round add by add.
 # packed-fp32 ops are switched off for all device code.
@@ -48,7 +50,7 @@ def _stale(out, srcs):
 
 def kernel_units():
     """(source, extra flags, tag) of every translation unit of libmi355ccl.so."""
-    units = [(KERNEL_SRC, [], "main")]
+    units = [(KERNEL_SRC, [], "main"), (MODEL_SRC, [], "model")]
     units += [(REDUCE_SRC, ["-DMCCL_REDUCE_DT=%d" % dt], "dt%d" % dt) for dt in REDUCE_DTYPES]
     return units
 
@@ -69,7 +71,7 @@ def _run_parallel(cmds, jobs=8):
 
 def build_kernels(force=False, extra_flags=(), out=KERNEL_LIB):
     os.makedirs(os.path.dirname(out), exist_ok=True)
-    if not (force or _stale(out, [KERNEL_SRC, REDUCE_SRC] + KERNEL_HDRS)):
+    if not (force or _stale(out, [KERNEL_SRC, MODEL_SRC, REDUCE_SRC] + KERNEL_HDRS)):
         return out
     obj_dir = out + ".objs"
     os.makedirs(obj_dir, exist_ok=True)
@@ -163,7 +165,7 @@ def build_all(force=False):
 
 def stale_outputs():
     """Built libraries that are older than one of their sources."""
-    checks = [(KERNEL_LIB, [KERNEL_SRC, REDUCE_SRC] + KERNEL_HDRS),
+    checks = [(KERNEL_LIB, [KERNEL_SRC, MODEL_SRC, REDUCE_SRC] + KERNEL_HDRS),
               (BENCH_LIB, [BENCH_SRC, os.path.join(BENCH_DIR, "mccl_bench.h")]),
               (backend_lib_path(), BACKEND_SRCS + BACKEND_HDRS)]
     return [out for out, srcs in checks if os.path.exists(out) and _stale(out, srcs)]

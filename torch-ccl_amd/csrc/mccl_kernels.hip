@@ -55,6 +55,7 @@
 
 #include "mccl.h"
 
+#include "host_checks.hpp"
 #include "kernels_common.hpp"
 #include "kernels_copy.hpp"
 #include "kernels_moe.hpp"
@@ -75,6 +76,18 @@ int fail(int code, const char* fmt, ...) {
   va_end(ap);
   return code;
 }
+
+}  // namespace
+
+int mccl_report_error(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+namespace {
 
 #define HIP_TRY(expr)                                                                   \
   do {                                                                                  \
@@ -574,7 +587,7 @@ int launch_gather(const GatherSpec* specs, int nspec, size_t row_bytes, hipStrea
 // ------------------------------------------------------------------------------------------
 extern "C" {
 
-int mccl_version(void) { return 150; }
+int mccl_version(void) { return 160; }
 
 const char* mccl_last_error(void) { return g_err; }
 

@@ -1,0 +1,384 @@
+// The C ABI of the operators around the collectives that compute: embedding lookup and gradient, the
+// router, and the mixture-of-experts layer for a few tokens.  Device code: kernels_embedding.hpp,
+// kernels_router.hpp, kernels_layer.hpp.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "mccl.h"
+
+#include "host_checks.hpp"
+#include "kernels_embedding.hpp"
+#include "kernels_layer.hpp"
+#include "kernels_router.hpp"
+
+namespace {
+
+constexpr size_t kMaxHidden = 1u << 23;       // grids of at most 65535 column chunks
+constexpr size_t kMaxGradTokens = 1u << 28;   // and of at most 2^32 threads along their first axis
+constexpr uint32_t kMaxGroups = 1u << 23;     // rows and tokens beyond that walk the grid
+
+size_t float_size(int dtype) {
+  return dtype == MCCL_F32 ? 4 : (dtype == MCCL_BF16 || dtype == MCCL_F16) ? 2 : 0;
+}
+
+int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return mccl_report_error(MCCL_ERR_HIP, "%s launch failed: %s", what, hipGetErrorString(e));
+  return MCCL_OK;
+}
+
+int check_ids(const void* ids, int id_dtype) {
+  if (id_dtype != MCCL_I32 && id_dtype != MCCL_I64) return mccl_report_error(MCCL_ERR_UNSUPPORTED, "ids are int32 or int64");
+  if (!ids) return mccl_report_error(MCCL_ERR_INVALID_ARG, "id pointer is null");
+  if (misaligned(ids, id_dtype == MCCL_I32 ? 4 : 8)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "ids not aligned to their element size");
+  return MCCL_OK;
+}
+
+size_t up16(size_t b) { return (b + 15) & ~(size_t)15; }
+
+int sort_passes(uint64_t rows) {
+  int passes = 1;
+  while (passes < 4 && (rows >> (kSortBits * passes))) ++passes;
+  return passes;
+}
+
+// Workspace of the sort: two sets of keys and positions, the digit counts per tile, and their totals.
+struct SortPlan {
+  size_t tiles, keys, counts, bytes;
+};
+
+SortPlan plan_sort(size_t n) {
+  SortPlan p{};
+  if (n <= (size_t)kSortSmall) return p;
+  p.tiles = (n + kSortTile - 1) / kSortTile;
+  p.keys = up16(n * 4);
+  p.counts = up16(p.tiles * kSortDigits * 4);
+  p.bytes = 4 * p.keys + p.counts + kSortDigits * 4;
+  return p;
+}
+
+template <typename ID>
+int launch_sort(const ID* ids, size_t n, int64_t first_row, size_t rows, char* ws, int64_t* order, int64_t* offsets, hipStream_t s) {
+  const unsigned offset_groups = (unsigned)((rows + 1 + kSortBlock - 1) / kSortBlock);
+  if (n <= (size_t)kSortSmall) {
+    const unsigned rank_groups = (unsigned)((n + kSortBlock - 1) / kSortBlock);
+    hipLaunchKernelGGL(sort_small_kernel<ID>, dim3(rank_groups + offset_groups), dim3(kSortBlock), 0, s, ids, (uint32_t)n, first_row,
+                       (uint32_t)rows, rank_groups, order, offsets);
+    return launched("sort");
+  }
+  const SortPlan p = plan_sort(n);
+  uint32_t* key[2] = {(uint32_t*)ws, (uint32_t*)(ws + p.keys)};
+  uint32_t* pos[2] = {(uint32_t*)(ws + 2 * p.keys), (uint32_t*)(ws + 3 * p.keys)};
+  SortArgs a{};
+  a.ids = ids;
+  a.order = order;
+  a.counts = (uint32_t*)(ws + 4 * p.keys);
+  a.totals = (uint32_t*)(ws + 4 * p.keys + p.counts);
+  a.n = (uint32_t)n;
+  a.tiles = (uint32_t)p.tiles;
+  a.first_row = first_row;
+  a.rows = (uint32_t)rows;
+  const int passes = sort_passes(rows);
+  const dim3 tiles((unsigned)p.tiles), block(kSortBlock);
+  for (int pass = 0; pass < passes; ++pass) {
+    const bool first = pass == 0, last = pass == passes - 1;
+    a.shift = pass * kSortBits;
+    a.key_in = key[(pass + 1) & 1];
+    a.pos_in = pos[(pass + 1) & 1];
+    a.key_out = key[pass & 1];
+    a.pos_out = pos[pass & 1];
+    if (first) hipLaunchKernelGGL((sort_count_kernel<ID, true>), tiles, block, 0, s, a);
+    else hipLaunchKernelGGL((sort_count_kernel<ID, false>), tiles, block, 0, s, a);
+    hipLaunchKernelGGL(sort_scan_kernel, dim3(kSortDigits), block, 0, s, a.counts, a.tiles, a.totals);
+    if (first && last) hipLaunchKernelGGL((sort_scatter_kernel<ID, true, true>), tiles, block, 0, s, a);
+    else if (first) hipLaunchKernelGGL((sort_scatter_kernel<ID, true, false>), tiles, block, 0, s, a);
+    else if (last) hipLaunchKernelGGL((sort_scatter_kernel<ID, false, true>), tiles, block, 0, s, a);
+    else hipLaunchKernelGGL((sort_scatter_kernel<ID, false, false>), tiles, block, 0, s, a);
+  }
+  hipLaunchKernelGGL(sort_offsets_kernel, dim3(offset_groups), block, 0, s, a.key_out, a.n, a.rows, offsets);
+  return launched("sort");
+}
+
+template <int DT>
+void launch_embedding(const EmbeddingArgs& a, int id_dtype, hipStream_t s) {
+  const dim3 grid((unsigned)((a.vecs + 4ull * kWave * kLookupVecs - 1) / (4 * kWave * kLookupVecs))), block(256);
+  if (id_dtype == MCCL_I32) hipLaunchKernelGGL((embedding_kernel<DT, int32_t>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((embedding_kernel<DT, int64_t>), grid, block, 0, s, a);
+}
+
+size_t grad_pieces(size_t n) { return n > (size_t)kGradPiece ? (n + kGradPiece - 1) / kGradPiece : 0; }
+
+template <int DT, int OUT>
+void launch_embedding_grad(EmbeddingGradArgs a, hipStream_t s) {
+  const uint32_t chunks = (uint32_t)(((uint64_t)a.hidden + kWave * vec_elems<DT>() - 1) / (kWave * vec_elems<DT>()));
+  a.chunk_waves_log2 = chunks >= 4 ? 2 : chunks >= 2 ? 1 : 0;
+  const uint32_t per_group = kGradWaves >> a.chunk_waves_log2;
+  const uint32_t pieces = (uint32_t)grad_pieces(a.n);
+  a.piece_groups = (pieces + per_group - 1) / per_group;
+  const uint32_t row_groups = std::min(kMaxGroups, (a.rows + per_group - 1) / per_group);
+  hipLaunchKernelGGL((embedding_grad_kernel<DT, OUT>), dim3(a.piece_groups + row_groups), dim3(kGradWaves * kWave), 0, s, a);
+  if (pieces) hipLaunchKernelGGL((embedding_grad_join_kernel<DT, OUT>), dim3(pieces, chunks), dim3(kJoinWaves * kWave), 0, s, a);
+}
+
+template <int DT, bool GRAD>
+void launch_router(const RouterArgs& a, hipStream_t s) {
+  const dim3 grid(std::min(kMaxGroups, (a.tokens + kRouterWaves - 1) / kRouterWaves)), block(kRouterWaves * kWave);
+#define MCCL_LAUNCH_ROUTER(PER)                                                                   \
+  if constexpr (GRAD) hipLaunchKernelGGL((router_grad_kernel<DT, PER>), grid, block, 0, s, a);   \
+  else hipLaunchKernelGGL((router_kernel<DT, PER>), grid, block, 0, s, a)
+  if (a.experts <= 64) { MCCL_LAUNCH_ROUTER(1); }
+  else if (a.experts <= 128) { MCCL_LAUNCH_ROUTER(2); }
+  else if (a.experts <= 256) { MCCL_LAUNCH_ROUTER(4); }
+  else if (a.experts <= 512) { MCCL_LAUNCH_ROUTER(8); }
+  else if (a.experts <= 1024) { MCCL_LAUNCH_ROUTER(16); }
+  else { MCCL_LAUNCH_ROUTER(64); }
+#undef MCCL_LAUNCH_ROUTER
+}
+
+int check_router(size_t tokens, size_t experts, int topk, int dtype) {
+  if (!float_size(dtype)) return mccl_report_error(MCCL_ERR_UNSUPPORTED, "the router is defined for bf16, f16 and f32 logits");
+  if (experts < 1 || experts > (size_t)kRouterMaxExperts)
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "expert count %zu outside [1, %d]", experts, kRouterMaxExperts);
+  if (topk < 1 || topk > kRouterMaxTopk || (size_t)topk > experts)
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "topk %d outside [1, %d] or above the expert count %zu", topk, kRouterMaxTopk, experts);
+  if (tokens > 0x7fffffffull) return mccl_report_error(MCCL_ERR_INVALID_ARG, "too many tokens");
+  return MCCL_OK;
+}
+
+template <int DT>
+void launch_layer(const LayerArgs& a, hipStream_t s) {
+  const unsigned slots = a.by_pair ? a.pairs : a.experts;
+  const unsigned per_group = kLayerWaves * kLayerRows;
+  hipLaunchKernelGGL(layer_in_kernel<DT>, dim3((a.inter + per_group - 1) / per_group, slots), dim3(kLayerBlock), 0, s, a);
+  hipLaunchKernelGGL(layer_out_kernel<DT>, dim3((a.hidden + per_group - 1) / per_group, slots), dim3(kLayerBlock), 0, s, a);
+  hipLaunchKernelGGL(layer_join_kernel<DT>, dim3((a.hidden + 255) / 256, a.tokens), dim3(256), 0, s, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mccl_embedding(const void* table, size_t rows, const void* ids, int id_dtype, size_t n, int64_t first_row, size_t hidden,
+                   float scale, int dtype, void* out, void* stream) {
+  const size_t es = float_size(dtype);
+  if (!es) return mccl_report_error(MCCL_ERR_UNSUPPORTED, "embedding is defined for bf16, f16 and f32");
+  if (n == 0 || hidden == 0) return MCCL_OK;
+  int rc = check_ids(ids, id_dtype);
+  if (rc != MCCL_OK) return rc;
+  if (!out || (rows && !table)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "null pointer");
+  if (misaligned(table, es) || misaligned(out, es)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "table or output not aligned to its element size");
+  if (hidden > kMaxHidden || n > 0x7fffffffull) return mccl_report_error(MCCL_ERR_INVALID_ARG, "row or id list too long");
+  const size_t id_bytes = n * (id_dtype == MCCL_I32 ? 4 : 8);
+  if (ranges_overlap(out, n * hidden * es, table, rows * hidden * es) || ranges_overlap(out, n * hidden * es, ids, id_bytes))
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "output overlaps the table or the ids");
+  EmbeddingArgs a{};
+  a.table = (const char*)table;
+  a.first_row = first_row;
+  a.rows = rows;
+  a.hidden = (uint32_t)hidden;
+  a.vecs_per_row = (uint32_t)((hidden * es + 15) / 16);
+  a.scale = scale;
+  // vectors are counted in 32 bits on the device: a longer list is looked up in parts
+  const size_t most = 0x80000000ull / a.vecs_per_row;
+  for (size_t i = 0; i < n; i += most) {
+    const size_t part = std::min(most, n - i);
+    a.ids = (const char*)ids + i * (id_dtype == MCCL_I32 ? 4 : 8);
+    a.out = (char*)out + i * hidden * es;
+    a.vecs = (uint32_t)(part * a.vecs_per_row);
+    switch (dtype) {
+      case MCCL_BF16: launch_embedding<MCCL_BF16>(a, id_dtype, (hipStream_t)stream); break;
+      case MCCL_F16: launch_embedding<MCCL_F16>(a, id_dtype, (hipStream_t)stream); break;
+      default: launch_embedding<MCCL_F32>(a, id_dtype, (hipStream_t)stream); break;
+    }
+  }
+  return launched("embedding");
+}
+
+size_t mccl_sort_ids_workspace(size_t n) { return plan_sort(n).bytes; }
+
+int mccl_sort_ids(const void* ids, int id_dtype, size_t n, int64_t first_row, size_t rows, void* workspace, size_t workspace_bytes,
+                  int64_t* order, int64_t* offsets, void* stream) {
+  if (id_dtype != MCCL_I32 && id_dtype != MCCL_I64) return mccl_report_error(MCCL_ERR_UNSUPPORTED, "ids are int32 or int64");
+  if (n > 0x7fffffffull) return mccl_report_error(MCCL_ERR_INVALID_ARG, "too many ids");
+  if (rows > 0x7fffffffull) return mccl_report_error(MCCL_ERR_INVALID_ARG, "too many rows");
+  if (!offsets || misaligned(offsets, 8)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "offsets pointer is null or misaligned");
+  if (n) {
+    int rc = check_ids(ids, id_dtype);
+    if (rc != MCCL_OK) return rc;
+    if (!order || misaligned(order, 8)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "order pointer is null or misaligned");
+  }
+  const size_t id_bytes = n * (id_dtype == MCCL_I32 ? 4 : 8), need = plan_sort(n).bytes;
+  if (need && (!workspace || misaligned(workspace, 16) || workspace_bytes < need))
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "workspace is null, not 16-byte aligned or smaller than %zu bytes", need);
+  const void* part[] = {ids, order, offsets, workspace};
+  const size_t bytes[] = {id_bytes, n * 8, (rows + 1) * 8, need};
+  for (int i = 0; i < 4; ++i)
+    for (int j = i + 1; j < 4; ++j)
+      if (ranges_overlap(part[i], bytes[i], part[j], bytes[j]))
+        return mccl_report_error(MCCL_ERR_INVALID_ARG, "ids, order, offsets and workspace must not overlap");
+  hipStream_t s = (hipStream_t)stream;
+  if (id_dtype == MCCL_I32) return launch_sort((const int32_t*)ids, n, first_row, rows, (char*)workspace, order, offsets, s);
+  return launch_sort((const int64_t*)ids, n, first_row, rows, (char*)workspace, order, offsets, s);
+}
+
+size_t mccl_embedding_grad_workspace(size_t n, size_t hidden) { return grad_pieces(n) * 2 * hidden * sizeof(float); }
+
+int mccl_embedding_grad(const void* grad, const int64_t* order, const int64_t* offsets, size_t n, size_t rows, size_t hidden,
+                        float scale, int dtype, void* out, int out_dtype, int accumulate, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  const size_t es = float_size(dtype), os = float_size(out_dtype);
+  if (!es || !os || (out_dtype != dtype && out_dtype != MCCL_F32))
+    return mccl_report_error(MCCL_ERR_UNSUPPORTED, "embedding_grad takes bf16, f16 or f32 and writes the same type or f32");
+  if (rows == 0 || hidden == 0) return MCCL_OK;
+  if (hidden > kMaxHidden || n > kMaxGradTokens || rows > 0x7fffffffull)
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "row, id list or table too long");
+  if (!offsets || !out || (n && (!grad || !order))) return mccl_report_error(MCCL_ERR_INVALID_ARG, "null pointer");
+  if (misaligned(grad, es) || misaligned(out, os)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "gradient or output not aligned to its element size");
+  if (misaligned(order, 8) || misaligned(offsets, 8)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "order or offsets misaligned");
+  const size_t need = mccl_embedding_grad_workspace(n, hidden);
+  if (need && (!workspace || misaligned(workspace, 16) || workspace_bytes < need))
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "workspace is null, not 16-byte aligned or smaller than %zu bytes", need);
+  const size_t out_bytes = rows * hidden * os;
+  const void* part[] = {grad, order, offsets};
+  const size_t bytes[] = {n * hidden * es, n * 8, (rows + 1) * 8};
+  for (int i = 0; i < 3; ++i)
+    if (ranges_overlap(out, out_bytes, part[i], bytes[i]) || ranges_overlap(workspace, need, part[i], bytes[i]))
+      return mccl_report_error(MCCL_ERR_INVALID_ARG, "output or workspace overlaps an input");
+  if (ranges_overlap(out, out_bytes, workspace, need)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "output overlaps the workspace");
+  EmbeddingGradArgs a{};
+  a.grad = (const char*)grad;
+  a.order = order;
+  a.offsets = offsets;
+  a.out = (char*)out;
+  a.partial = (float*)workspace;
+  a.rows = (uint32_t)rows;
+  a.n = (uint32_t)n;
+  a.hidden = (uint32_t)hidden;
+  a.scale = scale;
+  a.accumulate = accumulate ? 1 : 0;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == MCCL_F32) launch_embedding_grad<MCCL_F32, MCCL_F32>(a, s);
+  else if (dtype == MCCL_BF16 && out_dtype == MCCL_BF16) launch_embedding_grad<MCCL_BF16, MCCL_BF16>(a, s);
+  else if (dtype == MCCL_BF16) launch_embedding_grad<MCCL_BF16, MCCL_F32>(a, s);
+  else if (out_dtype == MCCL_F16) launch_embedding_grad<MCCL_F16, MCCL_F16>(a, s);
+  else launch_embedding_grad<MCCL_F16, MCCL_F32>(a, s);
+  return launched("embedding gradient");
+}
+
+int mccl_moe_route(const void* logits, size_t tokens, size_t experts, int topk, int normalize, int dtype, int32_t* expert_ids,
+                   float* weights, void* stream) {
+  int rc = check_router(tokens, experts, topk, dtype);
+  if (rc != MCCL_OK || tokens == 0) return rc;
+  const size_t es = float_size(dtype), pairs = tokens * (size_t)topk;
+  if (!logits || !expert_ids || !weights) return mccl_report_error(MCCL_ERR_INVALID_ARG, "null pointer");
+  if (misaligned(logits, es) || misaligned(expert_ids, 4) || misaligned(weights, 4))
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "logits, ids or weights not aligned to their element size");
+  if (ranges_overlap(expert_ids, pairs * 4, logits, tokens * experts * es) || ranges_overlap(weights, pairs * 4, logits, tokens * experts * es) ||
+      ranges_overlap(expert_ids, pairs * 4, weights, pairs * 4))
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "ids, weights and logits must not overlap");
+  RouterArgs a{};
+  a.logits = (const char*)logits;
+  a.ids = expert_ids;
+  a.weights = weights;
+  a.tokens = (uint32_t)tokens;
+  a.experts = (uint32_t)experts;
+  a.topk = (uint32_t)topk;
+  a.normalize = normalize ? 1 : 0;
+  hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+    case MCCL_BF16: launch_router<MCCL_BF16, false>(a, s); break;
+    case MCCL_F16: launch_router<MCCL_F16, false>(a, s); break;
+    default: launch_router<MCCL_F32, false>(a, s); break;
+  }
+  return launched("router");
+}
+
+int mccl_moe_route_grad(const float* grad_weights, const void* logits, const int32_t* expert_ids, size_t tokens, size_t experts, int topk,
+                        int normalize, int dtype, void* grad_logits, void* stream) {
+  int rc = check_router(tokens, experts, topk, dtype);
+  if (rc != MCCL_OK || tokens == 0) return rc;
+  const size_t es = float_size(dtype), pairs = tokens * (size_t)topk, bytes = tokens * experts * es;
+  if (!logits || !expert_ids || !grad_weights || !grad_logits) return mccl_report_error(MCCL_ERR_INVALID_ARG, "null pointer");
+  if (misaligned(logits, es) || misaligned(grad_logits, es) || misaligned(expert_ids, 4) || misaligned(grad_weights, 4))
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "logits, ids or gradients not aligned to their element size");
+  if (ranges_overlap(grad_logits, bytes, logits, bytes) || ranges_overlap(grad_logits, bytes, expert_ids, pairs * 4) ||
+      ranges_overlap(grad_logits, bytes, grad_weights, pairs * 4))
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "the gradient overlaps an input");
+  RouterArgs a{};
+  a.logits = (const char*)logits;
+  a.chosen = expert_ids;
+  a.grad_weights = grad_weights;
+  a.grad_logits = (char*)grad_logits;
+  a.tokens = (uint32_t)tokens;
+  a.experts = (uint32_t)experts;
+  a.topk = (uint32_t)topk;
+  a.normalize = normalize ? 1 : 0;
+  hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+    case MCCL_BF16: launch_router<MCCL_BF16, true>(a, s); break;
+    case MCCL_F16: launch_router<MCCL_F16, true>(a, s); break;
+    default: launch_router<MCCL_F32, true>(a, s); break;
+  }
+  return launched("router gradient");
+}
+
+size_t mccl_moe_layer_workspace(size_t tokens, int topk, size_t hidden, size_t inter) {
+  if (topk < 1) return 0;
+  const size_t pairs = tokens * (size_t)topk;
+  return up16(pairs * inter * 2) + pairs * hidden * sizeof(float);
+}
+
+int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int32_t* expert_ids, const float* weights, size_t tokens,
+                   int topk, size_t experts, int64_t first_expert, size_t hidden, size_t inter, int activation, int dtype, void* out,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype != MCCL_BF16 && dtype != MCCL_F16) return mccl_report_error(MCCL_ERR_UNSUPPORTED, "moe_layer is defined for bf16 and f16");
+  if (activation != MCCL_ACT_SILU && activation != MCCL_ACT_GELU) return mccl_report_error(MCCL_ERR_INVALID_ARG, "unknown activation %d", activation);
+  if (tokens > (size_t)kLayerMaxTokens)
+    return mccl_report_error(MCCL_ERR_UNSUPPORTED, "%zu tokens: moe_layer is for at most %d; dispatch larger batches", tokens, kLayerMaxTokens);
+  if (topk < 1 || topk > kRouterMaxTopk || tokens * (size_t)topk > (size_t)kLayerMaxPairs)
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "topk %d outside [1, %d], or more than %d (token, expert) pairs", topk, kRouterMaxTopk, kLayerMaxPairs);
+  if (experts < 1 || experts > (size_t)kRouterMaxExperts)
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "expert count %zu outside [1, %d]", experts, kRouterMaxExperts);
+  if (tokens == 0 || hidden == 0) return MCCL_OK;
+  if (hidden % 8 || inter % 8 || inter == 0) return mccl_report_error(MCCL_ERR_UNSUPPORTED, "moe_layer needs hidden and inter that are multiples of 8");
+  if (hidden > (1u << 24) || inter > (1u << 24)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "hidden or inter too large");
+  if (!x || !w_in || !w_out || !expert_ids || !weights || !out) return mccl_report_error(MCCL_ERR_INVALID_ARG, "null pointer");
+  if (misaligned(x, 16) || misaligned(w_in, 16) || misaligned(w_out, 16) || misaligned(out, 16))
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "x, the weights or the output are not 16-byte aligned");
+  if (misaligned(expert_ids, 4) || misaligned(weights, 4)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "expert ids or weights misaligned");
+  const size_t pairs = tokens * (size_t)topk, need = mccl_moe_layer_workspace(tokens, topk, hidden, inter), row = tokens * hidden * 2;
+  if (!workspace || misaligned(workspace, 16) || workspace_bytes < need)
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "workspace is null, not 16-byte aligned or smaller than %zu bytes", need);
+  const void* part[] = {x, w_in, w_out, expert_ids, weights};
+  const size_t bytes[] = {row, experts * 2 * inter * hidden * 2, experts * hidden * inter * 2, pairs * 4, pairs * 4};
+  for (int i = 0; i < 5; ++i)
+    if (ranges_overlap(out, row, part[i], bytes[i]) || ranges_overlap(workspace, need, part[i], bytes[i]))
+      return mccl_report_error(MCCL_ERR_INVALID_ARG, "output or workspace overlaps an input");
+  if (ranges_overlap(out, row, workspace, need)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "output overlaps the workspace");
+  LayerArgs a{};
+  a.x = (const char*)x;
+  a.w_in = (const char*)w_in;
+  a.w_out = (const char*)w_out;
+  a.ids = expert_ids;
+  a.weights = weights;
+  a.h = (char*)workspace;
+  a.y = (float*)((char*)workspace + up16(pairs * inter * 2));
+  a.out = (char*)out;
+  a.tokens = (uint32_t)tokens;
+  a.topk = (uint32_t)topk;
+  a.pairs = (uint32_t)pairs;
+  a.experts = (uint32_t)experts;
+  a.hidden = (uint32_t)hidden;
+  a.inter = (uint32_t)inter;
+  a.first_expert = first_expert;
+  a.by_pair = pairs < experts ? 1 : 0;
+  a.activation = activation;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == MCCL_BF16) launch_layer<MCCL_BF16>(a, s);
+  else launch_layer<MCCL_F16>(a, s);
+  return launched("moe layer");
+}
+
+}  // extern "C"

@@ -26,6 +26,7 @@ VARIANT_AUTO, VARIANT_SMALL, VARIANT_PERSISTENT, VARIANT_STREAM = 0, 1, 2, 3
 COPY_SHARED_SOURCES = 1  # flag of mccl_copy_segments_sync
 FUSED_WORK_ONLY, FUSED_SYNC_ONLY = 1, 2  # flags of mccl_allreduce_fused_replayable
 FUSED_STATE_BYTES = 128
+ACT_SILU, ACT_GELU = 0, 1  # mccl_activation_t
 MAX_RANKS = 64
 
 TORCH_DTYPE = {
@@ -44,6 +45,8 @@ EXPORTS = (
     "mccl_reduce_sync_resolved", "mccl_reduce_sync_offers", "mccl_fanout_sync_resolved", "mccl_fanout_sync_offers", "mccl_allreduce_fused", "mccl_allreduce_fused_replayable", "mccl_fanout_sync",
     "mccl_copy_segments_sync", "mccl_copy_segments_sync_resolved", "mccl_alltoall_sync_offers", "mccl_reduce_sync", "mccl_allreduce_sync_shard", "mccl_allreduce_sync",
     "mccl_route_counts", "mccl_route_counts_noalloc", "mccl_placement_check",
+    "mccl_embedding", "mccl_sort_ids", "mccl_sort_ids_workspace", "mccl_embedding_grad", "mccl_embedding_grad_workspace",
+    "mccl_moe_route", "mccl_moe_route_grad", "mccl_moe_layer", "mccl_moe_layer_workspace",
 )
 
 
@@ -134,6 +137,19 @@ def lib():
     L.mccl_placement_check.argtypes = [vp, i32, sz]
     L.mccl_route_counts.argtypes = [vp, sz, i32, vp, vp, vp]
     L.mccl_route_counts_noalloc.argtypes = [vp, sz, i32, vp, vp]
+    i64, f32 = ctypes.c_int64, ctypes.c_float
+    L.mccl_embedding.argtypes = [vp, sz, vp, i32, sz, i64, sz, f32, i32, vp, vp]
+    L.mccl_sort_ids_workspace.argtypes = [sz]
+    L.mccl_sort_ids_workspace.restype = sz
+    L.mccl_sort_ids.argtypes = [vp, i32, sz, i64, sz, vp, sz, vp, vp, vp]
+    L.mccl_embedding_grad_workspace.argtypes = [sz, sz]
+    L.mccl_embedding_grad_workspace.restype = sz
+    L.mccl_embedding_grad.argtypes = [vp, vp, vp, sz, sz, sz, f32, i32, vp, i32, i32, vp, sz, vp]
+    L.mccl_moe_route.argtypes = [vp, sz, sz, i32, i32, i32, vp, vp, vp]
+    L.mccl_moe_route_grad.argtypes = [vp, vp, vp, sz, sz, i32, i32, i32, vp, vp]
+    L.mccl_moe_layer_workspace.argtypes = [sz, i32, sz, sz]
+    L.mccl_moe_layer_workspace.restype = sz
+    L.mccl_moe_layer.argtypes = [vp, vp, vp, vp, vp, sz, i32, sz, i64, sz, sz, i32, i32, vp, vp, sz, vp]
     L.mccl_query_launch.argtypes = [sz, i32, i32, i32, i32, vp, vp]
     L.mccl_set_tuning.argtypes = [i32, ctypes.c_longlong]
     L.mccl_get_tuning.argtypes = [i32]
