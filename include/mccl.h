@@ -647,7 +647,7 @@ typedef enum {
   MCCL_ACT_SILU = 0, /* v * sigmoid(v) */
   MCCL_ACT_GELU = 1  /* v * (1 + erf(v / sqrt(2))) / 2 */
 } mccl_activation_t;
-size_t mccl_moe_layer_workspace(size_t tokens, int topk, size_t hidden, size_t inter);
+size_t mccl_moe_layer_workspace(size_t tokens, int topk, size_t experts, size_t hidden, size_t inter);
 int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int32_t* expert_ids,
                    const float* weights, size_t tokens, int topk, size_t experts, int64_t first_expert,
                    size_t hidden, size_t inter, int activation, int dtype, void* out, void* workspace,

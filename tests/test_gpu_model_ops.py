@@ -585,7 +585,7 @@ def test_workspaces_of_the_caller_are_used_and_may_be_dirty(mccl):
     from torch_ccl_amd import capi
     g = gen(41)
     x, w_in, w_out, ids, weights = [t.to(DEV) for t in layer_inputs(g, 9, 3, 8, 8, 64, 40, torch.bfloat16)]
-    need = capi.lib().mccl_moe_layer_workspace(9, 3, 64, 40)
+    need = capi.lib().mccl_moe_layer_workspace(9, 3, 8, 64, 40)
     ws = torch.full((need,), 0xFF, dtype=torch.uint8, device=DEV)
     assert torch.equal(mccl.moe_layer(x, w_in, w_out, ids, weights, workspace=ws), mccl.moe_layer(x, w_in, w_out, ids, weights))
     tokens = torch.randint(0, 30, (4000,), generator=g).to(DEV)

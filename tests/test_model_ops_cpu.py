@@ -126,7 +126,7 @@ def test_layer_refusals(abi):
     assert call(x=0x10000008) == -1 and "16-byte aligned" in err()
     assert call(w_out=0x200000002) == -1 and "16-byte aligned" in err()
     assert call(ids=0x20000002) == -1 and "misaligned" in err()
-    need = L.mccl_moe_layer_workspace(4, 2, 64, 32)
+    need = L.mccl_moe_layer_workspace(4, 2, 8, 64, 32)
     assert need > 0 and call(ws=0) == -1 and call(wsb=need - 1) == -1 and call(ws=0x40000008) == -1 and "workspace" in err()
     assert call(out=0x10000000) == -1 and "overlaps an input" in err()
     assert call(ws=0x200000000) == -1 and "overlaps an input" in err()

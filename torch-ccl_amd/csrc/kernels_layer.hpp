@@ -8,16 +8,14 @@ namespace {
 
 constexpr int kLayerMaxTokens = 256;
 constexpr int kLayerMaxPairs = 4096;
-constexpr int kLayerWaves = 4;
-constexpr int kLayerBlock = kLayerWaves * kWave;
-constexpr int kLayerRows = 16;  // weight rows per matrix instruction, and tokens
+constexpr int kLayerMaxExperts = 4096;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// 16 x 16 += (16 weight rows x 32) . (32 x 16 tokens): lane l holds 8 consecutive values of row (token)
-// l % 16 from column 8 * (l / 16) on, and gets rows 4 * (l / 16) .. + 3 of token l % 16.
+// 16 x 16 += (16 x 32) . (32 x 16): lane l holds 8 values of row (column) l % 16, from 8 * (l / 16) on of the
+// 32, and gets rows 4 * (l / 16) .. + 3 of column l % 16.
 template <int DT>
 __device__ __forceinline__ f32x4 mfma_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
   if constexpr (DT == MCCL_BF16)
@@ -33,43 +31,22 @@ struct LayerArgs {
   const int32_t* ids;   // [tokens][topk]
   const float* weights; // [tokens][topk]
   char* h;              // workspace [pairs][inter]
-  float* y;             // workspace [pairs][hidden]
+  float* y;             // workspace [parts][pairs][hidden], where the products of a pair meet in memory
   char* out;
   uint32_t tokens, topk, pairs, experts, hidden, inter;
   int64_t first_expert;
-  int by_pair;          // the grid's second axis counts pairs (fewer than experts) instead of experts
+  int by_pair;          // the slots of layer_in_kernel are pairs (fewer than experts) instead of experts
   int activation;
+  uint32_t parts;       // the second product: parts of inter that are work of their own
 };
 
+// The wavefront's number in its workgroup, as a value that the compiler knows to be the same for all lanes.
+__device__ __forceinline__ uint32_t wave_index() { return (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)); }
+
+// The expert of a pair among this rank's, or -1.
 __device__ __forceinline__ int local_expert(const LayerArgs& a, uint32_t pair) {
   const uint64_t e = (uint64_t)(int64_t)a.ids[pair] - (uint64_t)a.first_expert;
-  return e < a.experts ? (int)e : -1;
-}
-
-// The expert of this workgroup's slot and the pairs routed to it, ascending; returns how many (0: nothing
-// to do).  Where there are fewer pairs than experts a slot is a pair, and only the first pair of an
-// expert works.
-__device__ __forceinline__ uint32_t collect_pairs(const LayerArgs& a, uint32_t slot, uint16_t* list, uint32_t* counts, int* expert) {
-  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int e = a.by_pair ? local_expert(a, slot) : (int)slot;
-  *expert = e;
-  if (e < 0) return 0;
-  uint32_t total = 0;
-  for (uint32_t p0 = 0; p0 < a.pairs; p0 += kLayerBlock) {
-    const uint32_t p = p0 + threadIdx.x;
-    const bool mine = p < a.pairs && local_expert(a, p) == e;
-    const uint64_t m = __ballot(mine);
-    __syncthreads();
-    if (lane == 0) counts[wave] = (uint32_t)__popcll(m);
-    __syncthreads();
-    uint32_t at = total;
-    for (uint32_t w = 0; w < wave; ++w) at += counts[w];
-    if (mine) list[at + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)p;
-    for (uint32_t w = 0; w < kLayerWaves; ++w) total += counts[w];
-  }
-  __syncthreads();
-  if (total == 0 || (a.by_pair && list[0] != slot)) return 0;
-  return total;
+  return e < a.experts ? (int)(uint32_t)e : -1;
 }
 
 __device__ __forceinline__ float activate(float v, int activation) {
@@ -77,100 +54,447 @@ __device__ __forceinline__ float activate(float v, int activation) {
   return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
 }
 
-// h[pair][i] = act(w_in[e][i] . x[t]) * (w_in[e][inter + i] . x[t]).  A wavefront takes 16 gate rows and
-// their 16 up rows over the whole of hidden, 16 tokens at a time.
-template <int DT>
-__global__ __launch_bounds__(kLayerBlock) void layer_in_kernel(const LayerArgs a) {
-  using S = typename Elem<DT>::store_t;
-  __shared__ uint16_t list[kLayerMaxPairs];
-  __shared__ uint32_t counts[kLayerWaves];
-  int e;
-  const uint32_t m = collect_pairs(a, blockIdx.y, list, counts, &e);
-  if (m == 0) return;
-  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const uint32_t r = lane % 16, q = lane / 16;
-  const uint32_t i0 = (blockIdx.x * kLayerWaves + wave) * kLayerRows;
-  if (i0 >= a.inter) return;
-  const uint32_t row = i0 + r < a.inter ? i0 + r : a.inter - 1;
-  const S* gate = (const S*)a.w_in + ((size_t)e * 2 * a.inter + row) * a.hidden;
-  const S* up = gate + (size_t)a.inter * a.hidden;
-  for (uint32_t m0 = 0; m0 < m; m0 += 16) {
-    const uint32_t mine = m0 + r < m ? m0 + r : m - 1;
-    const uint32_t pair = list[mine];
-    const S* x = (const S*)a.x + (size_t)(pair / a.topk) * a.hidden;
-    f32x4 cg = {0.0f, 0.0f, 0.0f, 0.0f}, cu = cg;
-    for (uint32_t k0 = 0; k0 < a.hidden; k0 += 32) {
-      const uint32_t k = k0 + q * 8;
-      u32x4 ag = {0u, 0u, 0u, 0u}, au = ag, b = ag;
-      if (k < a.hidden) {
-        ag = *(const u32x4*)(gate + k);
-        au = *(const u32x4*)(up + k);
-        b = *(const u32x4*)(x + k);
-      }
-      cg = mfma_16x16x32<DT>(ag, b, cg);
-      cu = mfma_16x16x32<DT>(au, b, cu);
-    }
-    if (m0 + r < m) {
-      S* h = (S*)a.h + (size_t)pair * a.inter;
+// ------------------------------------------------------------------------------------------
+// products of 8 weight rows with 8 tokens
+// ------------------------------------------------------------------------------------------
+// The matrix instruction takes 16 rows of 32 columns: given 16 weight rows, a load would read 64 bytes
+// of each, half a cache line.  Here its rows are 8 weight rows twice, rows 8 to 15 for the next 32
+// columns, and its columns 8 tokens twice likewise, so that a load reads whole lines: 128 bytes of each
+// of 8 rows.  Two of the four 8 x 8 quarters of the result are the products of the two halves, the others
+// go unused: twice the matrix instructions, of which this kernel has far too few to matter.
+constexpr int kSetRows = 8;
+constexpr int kStepCols = 64;
+
+// Where in a step's 64 columns the 8 values of this lane lie.
+__device__ __forceinline__ uint32_t lane_column() {
+  const uint32_t lane = threadIdx.x % kWave;
+  return ((lane % 16) / 8 * 4 + lane / 16) * 8;
+}
+
+// acc[w][t] += rows . tokens over the steps [s0, s1): this lane's rows lie w[...] bytes behind `rows` (the
+// same for all lanes), its tokens b[...] behind `tokens`, both at the lane's column.  Columns from `depth`
+// on count as zero.  The loads of STEPS steps are issued before the first product.
+template <int DT, int NW, int NT, int STEPS>
+__device__ __forceinline__ void multiply_sets(const char* rows, const uint32_t (&w)[NW], const char* tokens, const uint32_t (&b)[NT],
+                                              uint32_t s0, uint32_t s1, uint32_t depth, f32x4 (&acc)[NW][NT]) {
+  uint32_t s = s0;
+  for (; s + STEPS <= s1 && (s + STEPS) * kStepCols <= depth; s += STEPS) {
+    u32x4 wv[STEPS][NW], bv[STEPS][NT];
+    const char* rows_s = rows + s * (kStepCols * 2);
+    const char* tokens_s = tokens + s * (kStepCols * 2);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t i = i0 + q * 4 + c;
-        if (i < a.inter) h[i] = Elem<DT>::store(activate(cg[c], a.activation) * cu[c]);
+    for (int u = 0; u < STEPS; ++u) {
+#pragma unroll
+      for (int n = 0; n < NW; ++n) wv[u][n] = __builtin_nontemporal_load((const u32x4*)(rows_s + w[n] + u * (kStepCols * 2)));
+#pragma unroll
+      for (int n = 0; n < NT; ++n) bv[u][n] = *(const u32x4*)(tokens_s + b[n] + u * (kStepCols * 2));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u)
+#pragma unroll
+      for (int n = 0; n < NW; ++n)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[n][t] = mfma_16x16x32<DT>(wv[u][n], bv[u][t], acc[n][t]);
+  }
+  const uint32_t left = depth - lane_column();  // columns are multiples of 8, and so is depth: all 8 or none
+  for (; s < s1; ++s) {
+    const uint32_t k = s * kStepCols;
+    const bool inside = (int32_t)(left - k) > 0;
+    u32x4 wv[NW], bv[NT];
+#pragma unroll
+    for (int n = 0; n < NW; ++n) {
+      wv[n] = (u32x4){0u, 0u, 0u, 0u};
+      if (inside) wv[n] = __builtin_nontemporal_load((const u32x4*)(rows + w[n] + k * 2));
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      bv[n] = (u32x4){0u, 0u, 0u, 0u};
+      if (inside) bv[n] = *(const u32x4*)(tokens + b[n] + k * 2);
+    }
+#pragma unroll
+    for (int n = 0; n < NW; ++n)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[n][t] = mfma_16x16x32<DT>(wv[n], bv[t], acc[n][t]);
+  }
+}
+
+// Adds the two halves: afterwards lanes 0 to 7 and 16 to 23 (holds_result) hold rows 4 * (lane / 16) .. + 3 of
+// token lane % 8.
+__device__ __forceinline__ f32x4 add_halves(f32x4 v) {
+  f32x4 r;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) r[c] = v[c] + __shfl_xor(v[c], 40);
+  return r;
+}
+__device__ __forceinline__ bool holds_result() { return (threadIdx.x % kWave) < 32 && (threadIdx.x % 16) < 8; }
+
+// The next pairs of expert e in ascending order into `list`, from pair `from` on: at least kListPairs of them
+// if there are as many, at most kListSpace; returns how many and leaves in `from` where to go on.  Every
+// wavefront lists for itself (several that share the space write the same values).  `expert_of(p)` is the
+// expert of pair p.
+constexpr uint32_t kListPairs = 64;
+constexpr uint32_t kListSpace = kListPairs + kWave;
+
+template <typename F>
+__device__ __forceinline__ uint32_t list_pairs(uint32_t pairs, int e, uint32_t& from, uint16_t* list, F expert_of) {
+  const uint32_t lane = threadIdx.x % kWave;
+  uint32_t m = 0;
+  for (; from < pairs && m < kListPairs; from += kWave) {
+    const bool mine = from + lane < pairs && expert_of(from + lane) == e;
+    const uint64_t set = __ballot(mine);
+    if (mine) list[m + __popcll(set & ((1ull << lane) - 1))] = (uint16_t)(from + lane);
+    m += (uint32_t)__popcll(set);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  return m;
+}
+
+// ------------------------------------------------------------------------------------------
+// h[pair][i] = act(w_in[e][i] . x[t]) * (w_in[e][inter + i] . x[t])
+// ------------------------------------------------------------------------------------------
+// A workgroup takes 16 gate rows and their 16 up rows of one expert; its wavefronts share the columns.
+constexpr int kInWaves = 4;
+constexpr int kInRows = 2 * kSetRows;
+
+template <int DT, int NT, int STEPS>
+__device__ __forceinline__ void layer_in_tokens(const LayerArgs& a, int e, uint32_t i0, const uint16_t* list, uint32_t m0, uint32_t m,
+                                                float (*sums)[4][NT][8][8]) {
+  using S = typename Elem<DT>::store_t;
+  const uint32_t lane = threadIdx.x % kWave, wave = wave_index();
+  const uint32_t r = lane % 8, col = lane_column();
+  uint32_t w[4], b[NT];
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const uint32_t i = i0 + (n % 2) * kSetRows + r;
+    w[n] = (((i < a.inter ? i : a.inter - 1) + (n / 2) * a.inter) * a.hidden + col) * 2;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const uint32_t mine = m0 + t * 8 + r;
+    b[t] = ((list[mine < m ? mine : m - 1] / a.topk) * a.hidden + col) * 2;
+  }
+  f32x4 acc[4][NT];
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[n][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  const uint32_t steps = (a.hidden + kStepCols - 1) / kStepCols, per = (steps + kInWaves - 1) / kInWaves;
+  const uint32_t s0 = wave * per, s1 = s0 + per < steps ? s0 + per : steps;
+  multiply_sets<DT, 4, NT, STEPS>(a.w_in + (size_t)e * 2 * a.inter * a.hidden * 2, w, a.x, b, s0, s1, a.hidden, acc);
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const f32x4 v = add_halves(acc[n][t]);
+      if (holds_result()) *(f32x4*)&sums[wave][n][t][r][lane / 16 * 4] = v;
+    }
+  __syncthreads();
+  for (uint32_t o = threadIdx.x; o < NT * 8 * kInRows; o += kInWaves * kWave) {
+    const uint32_t row = o % kInRows, token = o / kInRows;
+    if (m0 + token >= m || i0 + row >= a.inter) continue;
+    float g = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kInWaves; ++p) {
+      g += sums[p][row / 8][token / 8][token % 8][row % 8];
+      u += sums[p][2 + row / 8][token / 8][token % 8][row % 8];
+    }
+    ((S*)a.h)[(size_t)list[m0 + token] * a.inter + i0 + row] = Elem<DT>::store(activate(g, a.activation) * u);
+  }
+  __syncthreads();
+}
+
+// TOKENS bounds how many tokens one reading of the weights serves (and with it the registers).
+template <int DT, int TOKENS>
+__global__ __launch_bounds__(kInWaves * kWave) void layer_in_kernel(const LayerArgs a) {
+  __shared__ uint16_t list[kListSpace];
+  __shared__ float sums[kInWaves * 4 * (TOKENS / 8) * 64];
+  const int e = a.by_pair ? __builtin_amdgcn_readfirstlane(local_expert(a, blockIdx.y)) : (int)blockIdx.y;
+  if (e < 0) return;
+  const uint32_t i0 = blockIdx.x * kInRows;
+  for (uint32_t from = 0; from < a.pairs;) {
+    const bool begins = from == 0;
+    const uint32_t m = list_pairs(a.pairs, e, from, list, [&](uint32_t p) { return local_expert(a, p); });
+    if (begins && a.by_pair && (m == 0 || list[0] != blockIdx.y)) return;  // of the pairs of an expert the first one works
+    uint32_t m0 = 0;
+    if constexpr (TOKENS >= 32)
+      for (; m0 < m && m - m0 > 16; m0 += 32) layer_in_tokens<DT, 4, 1>(a, e, i0, list, m0, m, (float (*)[4][4][8][8])sums);
+    if constexpr (TOKENS >= 16)
+      for (; m0 < m && m - m0 > 8; m0 += 16) layer_in_tokens<DT, 2, 2>(a, e, i0, list, m0, m, (float (*)[4][2][8][8])sums);
+    for (; m0 < m; m0 += 8) layer_in_tokens<DT, 1, 4>(a, e, i0, list, m0, m, (float (*)[4][1][8][8])sums);
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// out[t][c] = sum_k weights[t][k] * (w_out[e][c] . h[t * topk + k])
+// ------------------------------------------------------------------------------------------
+// A workgroup takes kSetRows * NW rows of w_out of every expert that was chosen and keeps the products of
+// all pairs in LDS, so that the weighted sum needs no other workgroup: work of a wavefront is an expert
+// and one of a.parts parts of inter.
+constexpr uint32_t kOutMaxPairs = 2048;
+
+struct LayerOutLds {
+  uint32_t first, active, lists, y, bytes;
+};
+__host__ __device__ inline LayerOutLds layer_out_lds(uint32_t pairs, uint32_t experts, uint32_t parts, uint32_t rows, uint32_t waves) {
+  LayerOutLds l;
+  const uint32_t p8 = (pairs + 7) / 8 * 8;
+  l.first = p8 * 2;                             // the experts of the pairs come first, int16
+  l.active = l.first + (experts + 3) / 4 * 16;  // first pair of every expert, uint32
+  l.lists = l.active + p8 * 2;                  // first pairs of the chosen experts, uint16
+  l.y = l.lists + waves * kListSpace * 2;       // a list per wavefront, uint16
+  l.bytes = l.y + pairs * parts * rows * 4;
+  return l;
+}
+
+template <int DT, int NW, int NT, int STEPS>
+__device__ __forceinline__ void layer_out_tokens(const LayerArgs& a, int e, uint32_t c0, uint32_t part, const uint16_t* list, uint32_t m0,
+                                                 uint32_t m, float* y) {
+  const uint32_t lane = threadIdx.x % kWave;
+  const uint32_t r = lane % 8, col = lane_column();
+  uint32_t w[NW], b[NT];
+#pragma unroll
+  for (int n = 0; n < NW; ++n) {
+    const uint32_t row = c0 + n * kSetRows + r;
+    w[n] = ((row < a.hidden ? row : a.hidden - 1) * a.inter + col) * 2;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const uint32_t mine = m0 + t * 8 + r;
+    b[t] = (list[mine < m ? mine : m - 1] * a.inter + col) * 2;
+  }
+  f32x4 acc[NW][NT];
+#pragma unroll
+  for (int n = 0; n < NW; ++n)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[n][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  const uint32_t steps = (a.inter + kStepCols - 1) / kStepCols, per = (steps + a.parts - 1) / a.parts;
+  const uint32_t s0 = part * per, s1 = s0 + per < steps ? s0 + per : steps;
+  multiply_sets<DT, NW, NT, STEPS>(a.w_out + (size_t)e * a.hidden * a.inter * 2, w, a.h, b, s0, s1, a.inter, acc);
+#pragma unroll
+  for (int n = 0; n < NW; ++n)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const f32x4 v = add_halves(acc[n][t]);
+      if (holds_result() && m0 + t * 8 + r < m)
+        *(f32x4*)(y + (((size_t)list[m0 + t * 8 + r] * a.parts + part) * NW + n) * kSetRows + lane / 16 * 4) = v;
+    }
+}
+
+template <int DT, int NW>
+__device__ __forceinline__ void layer_out_expert(const LayerArgs& a, int e, uint32_t c0, uint32_t part, const uint16_t* list, uint32_t m, float* y) {
+  uint32_t m0 = 0;
+  for (; m0 < m && m - m0 > 16; m0 += 32) layer_out_tokens<DT, NW, 4, 2>(a, e, c0, part, list, m0, m, y);
+  for (; m0 < m && m - m0 > 8; m0 += 16) layer_out_tokens<DT, NW, 2, 4>(a, e, c0, part, list, m0, m, y);
+  for (; m0 < m; m0 += 8) layer_out_tokens<DT, NW, 1, 8 / NW>(a, e, c0, part, list, m0, m, y);
+}
+
+template <int DT, int NW, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArgs a) {
+  using S = typename Elem<DT>::store_t;
+  constexpr uint32_t kRows = NW * kSetRows;
+  extern __shared__ char lds[];
+  const LayerOutLds l = layer_out_lds(a.pairs, a.experts, a.parts, kRows, WAVES);
+  int16_t* expert = (int16_t*)lds;
+  uint32_t* first = (uint32_t*)(lds + l.first);
+  uint16_t* active = (uint16_t*)(lds + l.active);
+  float* y = (float*)(lds + l.y);
+  const uint32_t lane = threadIdx.x % kWave, wave = wave_index();
+  uint16_t* list = (uint16_t*)(lds + l.lists) + wave * kListSpace;
+  for (uint32_t p = threadIdx.x; p < a.pairs; p += WAVES * kWave) expert[p] = (int16_t)local_expert(a, p);
+  for (uint32_t e = threadIdx.x; e < a.experts; e += WAVES * kWave) first[e] = ~0u;
+  __syncthreads();
+  for (uint32_t p = threadIdx.x; p < a.pairs; p += WAVES * kWave)
+    if (expert[p] >= 0) atomicMin(&first[expert[p]], p);
+  __syncthreads();
+  uint32_t chosen = 0;  // every wavefront lists the first pairs, all with the same result
+  for (uint32_t p0 = 0; p0 < a.pairs; p0 += kWave) {
+    const uint32_t p = p0 + lane;
+    const bool leads = p < a.pairs && expert[p] >= 0 && first[expert[p]] == p;
+    const uint64_t set = __ballot(leads);
+    if (leads) active[chosen + __popcll(set & ((1ull << lane) - 1))] = (uint16_t)p;
+    chosen += (uint32_t)__popcll(set);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const uint32_t c0 = blockIdx.x * kRows, work = chosen * a.parts;
+  for (uint32_t i = wave; i < work; i += WAVES) {
+    const uint32_t part = i % a.parts;
+    uint32_t from = __builtin_amdgcn_readfirstlane(active[i / a.parts]);
+    const int e = __builtin_amdgcn_readfirstlane(expert[from]);
+    from = from / kWave * kWave;
+    while (from < a.pairs) {
+      const uint32_t m = list_pairs(a.pairs, e, from, list, [&](uint32_t p) { return (int)expert[p]; });
+      uint32_t m0 = 0;
+      for (; m0 < m && m - m0 > 16; m0 += 32) layer_out_tokens<DT, NW, 4, 2>(a, e, c0, part, list, m0, m, y);
+      for (; m0 < m && m - m0 > 8; m0 += 16) layer_out_tokens<DT, NW, 2, 4>(a, e, c0, part, list, m0, m, y);
+      for (; m0 < m; m0 += 8) layer_out_tokens<DT, NW, 1, 8 / NW>(a, e, c0, part, list, m0, m, y);
+    }
+  }
+  __syncthreads();
+  for (uint32_t o = threadIdx.x; o < a.tokens * kRows; o += WAVES * kWave) {
+    const uint32_t t = o / kRows, c = o % kRows;
+    if (c0 + c >= a.hidden) continue;
+    float sum = 0.0f;
+    for (uint32_t k = 0; k < a.topk; ++k) {
+      const uint32_t p = t * a.topk + k;
+      if (expert[p] < 0) continue;
+      float v = 0.0f;
+      for (uint32_t q = 0; q < a.parts; ++q) v += y[(p * a.parts + q) * kRows + c];
+      sum += a.weights[p] * v;
+    }
+    ((S*)a.out)[(size_t)t * a.hidden + c0 + c] = Elem<DT>::store(sum);
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// many tokens per expert
+// ------------------------------------------------------------------------------------------
+// The same products where an expert has so many tokens that reading them again for every 16 rows costs
+// more than the weights: a workgroup takes 8 wavefronts x NW sets of rows over all (or a part) of the
+// columns, and the tokens go through LDS, 128 columns of TOKENS of them at a time.  While a chunk is
+// multiplied, the rows and tokens of the next one are on their way into registers.
+constexpr int kDenseWaves = 8;
+constexpr int kDenseCols = 2 * kStepCols;
+
+// acc = rows . tokens over the columns of the chunks [c0, c1); tokens: row offsets of this thread's share of
+// the staging, one per 32 tokens.  `space` holds two chunks of TOKENS x kDenseCols values; the 16-byte pieces
+// of a token's 128 bytes are stored in an order turned by the token, so that the 8 tokens which a load from
+// LDS takes at the same columns lie in different banks.
+template <int DT, int NW, int TOKENS>
+__device__ __forceinline__ void multiply_dense(const char* rows, const uint32_t (&w)[NW], const char* tokens, const uint32_t (&from)[TOKENS / 32],
+                                               uint32_t used, uint32_t c0, uint32_t c1, uint32_t depth, char* space,
+                                               f32x4 (&acc)[NW][TOKENS / 8]) {
+  constexpr int kShare = TOKENS / 32;
+  constexpr uint32_t kRowBytes = kDenseCols * 2;
+  const uint32_t lane = threadIdx.x % kWave;
+  const uint32_t piece = threadIdx.x % 16, token = threadIdx.x / 16;       // staging: 16 pieces a token
+  const uint32_t put = token * kRowBytes + (piece / 8) * 128 + ((piece ^ token) % 8) * 16;
+  const uint32_t r = lane % 8, q8 = (lane % 16) / 8 * 4 + lane / 16;       // products: token in its set, piece of its 128 bytes
+  const uint32_t get = r * kRowBytes + ((q8 ^ r) % 8) * 16;
+  u32x4 wv[2][NW], tv[kShare];
+  const auto load = [&](uint32_t c) {
+    const uint32_t k = c * kDenseCols;
+    const bool whole = k + kDenseCols <= depth;
+#pragma unroll
+    for (int i = 0; i < kShare; ++i) {
+      tv[i] = (u32x4){0u, 0u, 0u, 0u};
+      if (i * 32u < used && (whole || k + piece * 8 < depth)) tv[i] = *(const u32x4*)(tokens + (size_t)k * 2 + from[i]);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int n = 0; n < NW; ++n) {
+        wv[u][n] = (u32x4){0u, 0u, 0u, 0u};
+        if (whole || k + u * kStepCols + q8 * 8 < depth)
+          wv[u][n] = __builtin_nontemporal_load((const u32x4*)(rows + (size_t)(k + u * kStepCols) * 2 + w[n]));
+      }
+  };
+  load(c0);
+  for (uint32_t c = c0; c < c1; ++c) {
+    char* buf = space + (c & 1) * (TOKENS * kRowBytes);
+    u32x4 now[2][NW];
+#pragma unroll
+    for (int i = 0; i < kShare; ++i)
+      if (i * 32u < used) *(u32x4*)(buf + put + i * 32 * kRowBytes) = tv[i];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int n = 0; n < NW; ++n) now[u][n] = wv[u][n];
+    __syncthreads();
+    if (c + 1 < c1) load(c + 1);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int t = 0; t < TOKENS / 8; ++t) {
+        if (t * 8u >= used) continue;
+        const u32x4 b = *(const u32x4*)(buf + get + t * 8 * kRowBytes + u * 128);
+#pragma unroll
+        for (int n = 0; n < NW; ++n) acc[n][t] = mfma_16x16x32<DT>(now[u][n], b, acc[n][t]);
+      }
+  }
+  __syncthreads();  // the space may be filled for the next tokens
+}
+
+// Pairs of the workgroup's expert, TOKENS at a time, in the order of `list` (which holds them all).
+template <int DT, int TOKENS, bool IN>
+__global__ __launch_bounds__(kDenseWaves * kWave) void layer_dense_kernel(const LayerArgs a) {
+  using S = typename Elem<DT>::store_t;
+  __shared__ __align__(16) char space[2 * TOKENS * kDenseCols * 2];
+  __shared__ uint16_t list[kLayerMaxPairs + kWave];
+  const int e = (int)blockIdx.y;
+  uint32_t m = 0;
+  for (uint32_t from = 0; from < a.pairs;) m += list_pairs(a.pairs, e, from, list + m, [&](uint32_t p) { return local_expert(a, p); });
+  if (m == 0) return;
+  const uint32_t lane = threadIdx.x % kWave, wave = wave_index();
+  const uint32_t r = lane % 8, col = lane_column(), part = blockIdx.z;
+  const uint32_t depth = IN ? a.hidden : a.inter, nrows = IN ? a.inter : a.hidden;
+  const uint32_t chunks = (depth + kDenseCols - 1) / kDenseCols, per = IN ? chunks : (chunks + a.parts - 1) / a.parts;
+  const uint32_t c0 = part * per, c1 = c0 + per < chunks ? c0 + per : chunks;
+  const uint32_t row0 = IN ? (blockIdx.x * kDenseWaves + wave) * kSetRows : (blockIdx.x * kDenseWaves + wave) * 2 * kSetRows;
+  uint32_t w[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const uint32_t row = row0 + (IN ? 0 : n * kSetRows) + r;
+    w[n] = (((row < nrows ? row : nrows - 1) + (IN ? n * a.inter : 0)) * depth + col) * 2;
+  }
+  const char* rows = (IN ? a.w_in + (size_t)e * 2 * a.inter * a.hidden * 2 : a.w_out + (size_t)e * a.hidden * a.inter * 2);
+  for (uint32_t m0 = 0; m0 < m; m0 += TOKENS) {
+    const uint32_t used = m - m0 < TOKENS ? m - m0 : TOKENS;
+    uint32_t from[TOKENS / 32];
+#pragma unroll
+    for (int i = 0; i < TOKENS / 32; ++i) {
+      const uint32_t t = i * 32 + threadIdx.x / 16;
+      const uint32_t pair = list[m0 + (t < used ? t : used - 1)];
+      from[i] = ((IN ? pair / a.topk : pair) * depth + threadIdx.x % 16 * 8) * 2;
+    }
+    f32x4 acc[2][TOKENS / 8];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int t = 0; t < TOKENS / 8; ++t) acc[n][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    multiply_dense<DT, 2, TOKENS>(rows, w, IN ? a.x : a.h, from, used, c0, c1, depth, space, acc);
+#pragma unroll
+    for (int t = 0; t < TOKENS / 8; ++t) {
+      if (t * 8u >= used) continue;
+      const f32x4 v0 = add_halves(acc[0][t]), v1 = add_halves(acc[1][t]);
+      if (!holds_result() || t * 8 + r >= used) continue;
+      const uint32_t pair = list[m0 + t * 8 + r], row = row0 + lane / 16 * 4;
+      if constexpr (IN) {
+        if (row < a.inter) {  // inter is a multiple of 8: all four rows or none
+          union { S e[4]; uint2 v; } h;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) h.e[c] = Elem<DT>::store(activate(v0[c], a.activation) * v1[c]);
+          *(uint2*)((S*)a.h + (size_t)pair * a.inter + row) = h.v;
+        }
+      } else {
+        float* y = a.y + ((size_t)part * a.pairs + pair) * a.hidden + row;
+        if (row < a.hidden) *(f32x4*)y = v0;
+        if (row + kSetRows < a.hidden) *(f32x4*)(y + kSetRows) = v1;
       }
     }
   }
 }
 
-// y[pair][c] = w_out[e][c] . h[pair]
-template <int DT>
-__global__ __launch_bounds__(kLayerBlock) void layer_out_kernel(const LayerArgs a) {
-  using S = typename Elem<DT>::store_t;
-  __shared__ uint16_t list[kLayerMaxPairs];
-  __shared__ uint32_t counts[kLayerWaves];
-  int e;
-  const uint32_t m = collect_pairs(a, blockIdx.y, list, counts, &e);
-  if (m == 0) return;
-  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const uint32_t r = lane % 16, q = lane / 16;
-  const uint32_t c0 = (blockIdx.x * kLayerWaves + wave) * kLayerRows;
-  if (c0 >= a.hidden) return;
-  const uint32_t row = c0 + r < a.hidden ? c0 + r : a.hidden - 1;
-  const S* w = (const S*)a.w_out + ((size_t)e * a.hidden + row) * a.inter;
-  for (uint32_t m0 = 0; m0 < m; m0 += 16) {
-    const uint32_t mine = m0 + r < m ? m0 + r : m - 1;
-    const uint32_t pair = list[mine];
-    const S* h = (const S*)a.h + (size_t)pair * a.inter;
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t k0 = 0; k0 < a.inter; k0 += 32) {
-      const uint32_t k = k0 + q * 8;
-      u32x4 av = {0u, 0u, 0u, 0u}, b = av;
-      if (k < a.inter) {
-        av = *(const u32x4*)(w + k);
-        b = *(const u32x4*)(h + k);
-      }
-      acc = mfma_16x16x32<DT>(av, b, acc);
-    }
-    if (m0 + r < m) {
-      float* y = a.y + (size_t)pair * a.hidden;
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (c0 + q * 4 + c < a.hidden) y[c0 + q * 4 + c] = acc[c];
-    }
-  }
-}
-
-// out[t] = sum_k weights[t][k] * y[t * topk + k], ascending k.
+// out[t] = sum_k weights[t][k] * (sum over the parts of y[t * topk + k]), ascending.
 template <int DT>
 __global__ __launch_bounds__(256) void layer_join_kernel(const LayerArgs a) {
   using S = typename Elem<DT>::store_t;
-  const uint32_t t = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
+  const uint32_t t = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (c >= a.hidden) return;
-  float acc = 0.0f;
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
   for (uint32_t k = 0; k < a.topk; ++k) {
     const uint32_t p = t * a.topk + k;
-    if (local_expert(a, p) >= 0) acc += a.weights[p] * a.y[(size_t)p * a.hidden + c];
+    if (local_expert(a, p) < 0) continue;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t q = 0; q < a.parts; ++q) v += *(const f32x4*)(a.y + ((size_t)q * a.pairs + p) * a.hidden + c);
+    sum += a.weights[p] * v;
   }
-  ((S*)a.out)[(size_t)t * a.hidden + c] = Elem<DT>::store(acc);
+  union { S e[4]; uint2 v; } r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.e[i] = Elem<DT>::store(sum[i]);
+  *(uint2*)((S*)a.out + (size_t)t * a.hidden + c) = r.v;
 }
 
 }  // namespace

@@ -147,13 +147,64 @@ int check_router(size_t tokens, size_t experts, int topk, int dtype) {
   return MCCL_OK;
 }
 
+// How a layer is run, from its sizes alone (the routing is only known on the device).
+struct LayerPlan {
+  bool dense;      // many tokens per expert: layer_dense_kernel
+  uint32_t parts;  // of inter, in the second product
+  size_t h_bytes, bytes;
+};
+
+constexpr size_t kDensePairs = 16;  // per expert
+LayerPlan plan_layer(size_t pairs, size_t experts, size_t hidden, size_t inter) {
+  LayerPlan p{};
+  p.dense = pairs > kDensePairs * experts || pairs > kOutMaxPairs;
+  p.h_bytes = up16(pairs * inter * 2);
+  p.bytes = p.h_bytes;
+  if (p.dense) {
+    const size_t groups = (hidden + kDenseWaves * 2 * kSetRows - 1) / (kDenseWaves * 2 * kSetRows) * experts;
+    const size_t chunks = (inter + kDenseCols - 1) / kDenseCols;
+    p.parts = (uint32_t)std::min<size_t>({chunks, 8, (512 + groups - 1) / groups});
+    p.bytes += p.parts * pairs * hidden * sizeof(float);
+  } else {
+    p.parts = (uint32_t)std::min<size_t>((inter + kStepCols - 1) / kStepCols, (16 + pairs - 1) / pairs);
+  }
+  return p;
+}
+
+template <int DT, int TOKENS>
+void launch_dense(const LayerArgs& a, hipStream_t s) {
+  const uint32_t in_rows = kDenseWaves * kSetRows, out_rows = 2 * in_rows;
+  hipLaunchKernelGGL((layer_dense_kernel<DT, TOKENS, true>), dim3((a.inter + in_rows - 1) / in_rows, a.experts), dim3(kDenseWaves * kWave), 0, s, a);
+  hipLaunchKernelGGL((layer_dense_kernel<DT, TOKENS, false>), dim3((a.hidden + out_rows - 1) / out_rows, a.experts, a.parts),
+                     dim3(kDenseWaves * kWave), 0, s, a);
+  hipLaunchKernelGGL(layer_join_kernel<DT>, dim3((a.hidden / 4 + 255) / 256, a.tokens), dim3(256), 0, s, a);
+}
+
+template <int DT, int NW, int WAVES>
+int launch_layer_out(const LayerArgs& a, hipStream_t s) {
+  const uint32_t rows = NW * kSetRows, bytes = layer_out_lds(a.pairs, a.experts, a.parts, rows, WAVES).bytes;
+  if (bytes > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)layer_out_kernel<DT, NW, WAVES>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != hipSuccess) return mccl_report_error(MCCL_ERR_HIP, "hipFuncSetAttribute failed: %s", hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL((layer_out_kernel<DT, NW, WAVES>), dim3((a.hidden + rows - 1) / rows), dim3(WAVES * kWave), bytes, s, a);
+  return MCCL_OK;
+}
+
 template <int DT>
-void launch_layer(const LayerArgs& a, hipStream_t s) {
-  const unsigned slots = a.by_pair ? a.pairs : a.experts;
-  const unsigned per_group = kLayerWaves * kLayerRows;
-  hipLaunchKernelGGL(layer_in_kernel<DT>, dim3((a.inter + per_group - 1) / per_group, slots), dim3(kLayerBlock), 0, s, a);
-  hipLaunchKernelGGL(layer_out_kernel<DT>, dim3((a.hidden + per_group - 1) / per_group, slots), dim3(kLayerBlock), 0, s, a);
-  hipLaunchKernelGGL(layer_join_kernel<DT>, dim3((a.hidden + 255) / 256, a.tokens), dim3(256), 0, s, a);
+int launch_layer(const LayerArgs& a, bool dense, hipStream_t s) {
+  if (dense) {
+    if (a.tokens <= 32) launch_dense<DT, 32>(a, s);
+    else if (a.tokens <= 64 || a.pairs <= 48 * a.experts) launch_dense<DT, 64>(a, s);
+    else launch_dense<DT, 128>(a, s);
+    return launched("moe layer");
+  }
+  const dim3 in_grid((a.inter + kInRows - 1) / kInRows, a.by_pair ? a.pairs : a.experts), in_block(kInWaves * kWave);
+  if (a.tokens <= 8) hipLaunchKernelGGL((layer_in_kernel<DT, 8>), in_grid, in_block, 0, s, a);
+  else if (a.tokens <= 16) hipLaunchKernelGGL((layer_in_kernel<DT, 16>), in_grid, in_block, 0, s, a);
+  else hipLaunchKernelGGL((layer_in_kernel<DT, 32>), in_grid, in_block, 0, s, a);
+  const int rc = a.hidden >= 4096 && a.pairs <= 1024 ? launch_layer_out<DT, 2, 8>(a, s) : launch_layer_out<DT, 1, 16>(a, s);
+  return rc != MCCL_OK ? rc : launched("moe layer");
 }
 
 }  // namespace
@@ -324,10 +375,9 @@ int mccl_moe_route_grad(const float* grad_weights, const void* logits, const int
   return launched("router gradient");
 }
 
-size_t mccl_moe_layer_workspace(size_t tokens, int topk, size_t hidden, size_t inter) {
-  if (topk < 1) return 0;
-  const size_t pairs = tokens * (size_t)topk;
-  return up16(pairs * inter * 2) + pairs * hidden * sizeof(float);
+size_t mccl_moe_layer_workspace(size_t tokens, int topk, size_t experts, size_t hidden, size_t inter) {
+  if (topk < 1 || tokens == 0 || experts == 0) return 0;
+  return plan_layer(tokens * (size_t)topk, experts, hidden, inter).bytes;
 }
 
 int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int32_t* expert_ids, const float* weights, size_t tokens,
@@ -343,12 +393,15 @@ int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int
     return mccl_report_error(MCCL_ERR_INVALID_ARG, "expert count %zu outside [1, %d]", experts, kRouterMaxExperts);
   if (tokens == 0 || hidden == 0) return MCCL_OK;
   if (hidden % 8 || inter % 8 || inter == 0) return mccl_report_error(MCCL_ERR_UNSUPPORTED, "moe_layer needs hidden and inter that are multiples of 8");
-  if (hidden > (1u << 24) || inter > (1u << 24)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "hidden or inter too large");
+  if (hidden > (1u << 18) || inter > (1u << 18) || 4 * inter * hidden > 0x7fffffffull)
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "hidden or inter too large: an expert's w_in has to be below 2 GiB");
   if (!x || !w_in || !w_out || !expert_ids || !weights || !out) return mccl_report_error(MCCL_ERR_INVALID_ARG, "null pointer");
   if (misaligned(x, 16) || misaligned(w_in, 16) || misaligned(w_out, 16) || misaligned(out, 16))
     return mccl_report_error(MCCL_ERR_INVALID_ARG, "x, the weights or the output are not 16-byte aligned");
   if (misaligned(expert_ids, 4) || misaligned(weights, 4)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "expert ids or weights misaligned");
-  const size_t pairs = tokens * (size_t)topk, need = mccl_moe_layer_workspace(tokens, topk, hidden, inter), row = tokens * hidden * 2;
+  const size_t pairs = tokens * (size_t)topk, row = tokens * hidden * 2;
+  const LayerPlan plan = plan_layer(pairs, experts, hidden, inter);
+  const size_t need = plan.bytes;
   if (!workspace || misaligned(workspace, 16) || workspace_bytes < need)
     return mccl_report_error(MCCL_ERR_INVALID_ARG, "workspace is null, not 16-byte aligned or smaller than %zu bytes", need);
   const void* part[] = {x, w_in, w_out, expert_ids, weights};
@@ -364,8 +417,9 @@ int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int
   a.ids = expert_ids;
   a.weights = weights;
   a.h = (char*)workspace;
-  a.y = (float*)((char*)workspace + up16(pairs * inter * 2));
+  a.y = (float*)((char*)workspace + plan.h_bytes);
   a.out = (char*)out;
+  a.parts = plan.parts;
   a.tokens = (uint32_t)tokens;
   a.topk = (uint32_t)topk;
   a.pairs = (uint32_t)pairs;
@@ -376,9 +430,7 @@ int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int
   a.by_pair = pairs < experts ? 1 : 0;
   a.activation = activation;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == MCCL_BF16) launch_layer<MCCL_BF16>(a, s);
-  else launch_layer<MCCL_F16>(a, s);
-  return launched("moe layer");
+  return dtype == MCCL_BF16 ? launch_layer<MCCL_BF16>(a, plan.dense, s) : launch_layer<MCCL_F16>(a, plan.dense, s);
 }
 
 }  // extern "C"

@@ -147,7 +147,7 @@ def lib():
     L.mccl_embedding_grad.argtypes = [vp, vp, vp, sz, sz, sz, f32, i32, vp, i32, i32, vp, sz, vp]
     L.mccl_moe_route.argtypes = [vp, sz, sz, i32, i32, i32, vp, vp, vp]
     L.mccl_moe_route_grad.argtypes = [vp, vp, vp, sz, sz, i32, i32, i32, vp, vp]
-    L.mccl_moe_layer_workspace.argtypes = [sz, i32, sz, sz]
+    L.mccl_moe_layer_workspace.argtypes = [sz, i32, sz, sz, sz]
     L.mccl_moe_layer_workspace.restype = sz
     L.mccl_moe_layer.argtypes = [vp, vp, vp, vp, vp, sz, i32, sz, i64, sz, sz, i32, i32, vp, vp, sz, vp]
     L.mccl_query_launch.argtypes = [sz, i32, i32, i32, i32, vp, vp]

@@ -454,7 +454,7 @@ def moe_layer(x, w_in, w_out, expert_ids, weights, first_expert=0, activation="s
     _check_shape("moe_layer", "weights", weights, (tokens, topk), torch.float32)
     _check_shape("moe_layer", "out", out, x.shape, x.dtype)
     device = _check_gpu("moe_layer", x=x, w_in=w_in, w_out=w_out, expert_ids=expert_ids, weights=weights, out=out)
-    ws = _workspace("moe_layer", workspace, capi.lib().mccl_moe_layer_workspace(tokens, topk, hidden, inter), device)
+    ws = _workspace("moe_layer", workspace, capi.lib().mccl_moe_layer_workspace(tokens, topk, experts, hidden, inter), device)
     with torch.cuda.device(device):
         capi.check(capi.lib().mccl_moe_layer(x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), expert_ids.data_ptr(), weights.data_ptr(),
                                              tokens, topk, experts, int(first_expert), hidden, inter, _ACTIVATIONS[activation],
