@@ -58,36 +58,55 @@ __device__ __forceinline__ float activate(float v, int activation) {
 // products of 8 weight rows with 8 tokens
 // ------------------------------------------------------------------------------------------
 // The matrix instruction takes 16 rows of 32 columns: given 16 weight rows, a load would read 64 bytes
-// of each, half a cache line.  Here its rows are 8 weight rows twice, rows 8 to 15 for the next 32
-// columns, and its columns 8 tokens twice likewise, so that a load reads whole lines: 128 bytes of each
-// of 8 rows.  Two of the four 8 x 8 quarters of the result are the products of the two halves, the others
-// go unused: twice the matrix instructions, of which this kernel has far too few to matter.
+// of each, half a cache line, with every lane in another row than its neighbours.  Here its rows are 8
+// weight rows twice, the odd ones for other columns than the even ones, and its columns 8 tokens twice
+// likewise: a load reads 128 bytes of each of 8 rows, two lanes next to each other at a time.  Of each
+// 2 x 2 block of the result the diagonal is used, the products of the two halves, and the rest is not:
+// twice the matrix instructions, of which these kernels have far too few to matter.
 constexpr int kSetRows = 8;
 constexpr int kStepCols = 64;
 
-// Where in a step's 64 columns the 8 values of this lane lie.
-__device__ __forceinline__ uint32_t lane_column() {
-  const uint32_t lane = threadIdx.x % kWave;
-  return ((lane % 16) / 8 * 4 + lane / 16) * 8;
+// This lane's weight row, and token, of a set of 8, and where in a step's 64 columns its 8 values lie.
+__device__ __forceinline__ uint32_t lane_member() { return (threadIdx.x % 16) / 2; }
+__device__ __forceinline__ uint32_t lane_column() { return (threadIdx.x % 2 + (threadIdx.x % kWave) / 16 * 2) * 8; }
+
+// Where the sums are, once add_halves has been called: rows lane_row() and lane_row() + 1 of token
+// lane_member(), in even lanes.
+__device__ __forceinline__ uint32_t lane_row() { return (threadIdx.x % kWave) / 16 * 2; }
+__device__ __forceinline__ bool lane_holds() { return threadIdx.x % 2 == 0; }
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float from_neighbour(float v) {
+  return bits_to_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_to_bits(v), 0xb1, 0xf, 0xf, true));  // lanes 1 0 3 2
+}
+__device__ __forceinline__ f32x2 add_halves(f32x4 v) { return (f32x2){v[0] + from_neighbour(v[1]), v[2] + from_neighbour(v[3])}; }
+
+// Rows and tokens are read through buffer descriptors: the base is the same for all lanes, a lane has a
+// 32-bit offset, and an offset of kOutside reads zeros without touching memory, which is how columns that do
+// not exist are left out without a branch.
+constexpr uint32_t kOutside = 0x80000000u;
+constexpr int kStreamed = 2;  // non-temporal: weights are read once
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t matrix_at(const char* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, (int)bytes, 0x00020000);
 }
 
-// acc[w][t] += rows . tokens over the steps [s0, s1): this lane's rows lie w[...] bytes behind `rows` (the
-// same for all lanes), its tokens b[...] behind `tokens`, both at the lane's column.  Columns from `depth`
-// on count as zero.  The loads of STEPS steps are issued before the first product.
+// acc[w][t] += rows . tokens over the steps [s0, s1) below column `depth`: this lane's rows lie w[...] bytes into
+// `rows`, its tokens b[...] into `tokens`, both at the lane's column.  The loads of STEPS steps are issued
+// before the first product.
 template <int DT, int NW, int NT, int STEPS>
-__device__ __forceinline__ void multiply_sets(const char* rows, const uint32_t (&w)[NW], const char* tokens, const uint32_t (&b)[NT],
-                                              uint32_t s0, uint32_t s1, uint32_t depth, f32x4 (&acc)[NW][NT]) {
-  uint32_t s = s0;
-  for (; s + STEPS <= s1 && (s + STEPS) * kStepCols <= depth; s += STEPS) {
+__device__ __forceinline__ void multiply_sets(__amdgpu_buffer_rsrc_t rows, const uint32_t (&w)[NW], __amdgpu_buffer_rsrc_t tokens,
+                                              const uint32_t (&b)[NT], uint32_t s0, uint32_t s1, uint32_t depth, f32x4 (&acc)[NW][NT]) {
+  const uint32_t end = s1 * kStepCols < depth ? s1 * kStepCols : depth, col = lane_column();
+  for (uint32_t s = s0; s < s1; s += STEPS) {
     u32x4 wv[STEPS][NW], bv[STEPS][NT];
-    const char* rows_s = rows + s * (kStepCols * 2);
-    const char* tokens_s = tokens + s * (kStepCols * 2);
 #pragma unroll
     for (int u = 0; u < STEPS; ++u) {
+      const uint32_t k = (s + u) * kStepCols;
+      const uint32_t out = k + col < end ? 0 : kOutside;  // columns, depth: multiples of 8, so all 8 or none
 #pragma unroll
-      for (int n = 0; n < NW; ++n) wv[u][n] = __builtin_nontemporal_load((const u32x4*)(rows_s + w[n] + u * (kStepCols * 2)));
+      for (int n = 0; n < NT; ++n) bv[u][n] = __builtin_amdgcn_raw_buffer_load_b128(tokens, b[n] | out, k * 2, 0);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) bv[u][n] = *(const u32x4*)(tokens_s + b[n] + u * (kStepCols * 2));
+      for (int n = 0; n < NW; ++n) wv[u][n] = __builtin_amdgcn_raw_buffer_load_b128(rows, w[n] | out, k * 2, kStreamed);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -97,37 +116,16 @@ __device__ __forceinline__ void multiply_sets(const char* rows, const uint32_t (
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[n][t] = mfma_16x16x32<DT>(wv[u][n], bv[u][t], acc[n][t]);
   }
-  const uint32_t left = depth - lane_column();  // columns are multiples of 8, and so is depth: all 8 or none
-  for (; s < s1; ++s) {
-    const uint32_t k = s * kStepCols;
-    const bool inside = (int32_t)(left - k) > 0;
-    u32x4 wv[NW], bv[NT];
-#pragma unroll
-    for (int n = 0; n < NW; ++n) {
-      wv[n] = (u32x4){0u, 0u, 0u, 0u};
-      if (inside) wv[n] = __builtin_nontemporal_load((const u32x4*)(rows + w[n] + k * 2));
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      bv[n] = (u32x4){0u, 0u, 0u, 0u};
-      if (inside) bv[n] = *(const u32x4*)(tokens + b[n] + k * 2);
-    }
-#pragma unroll
-    for (int n = 0; n < NW; ++n)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) acc[n][t] = mfma_16x16x32<DT>(wv[n], bv[t], acc[n][t]);
-  }
 }
 
-// Adds the two halves: afterwards lanes 0 to 7 and 16 to 23 (holds_result) hold rows 4 * (lane / 16) .. + 3 of
-// token lane % 8.
-__device__ __forceinline__ f32x4 add_halves(f32x4 v) {
-  f32x4 r;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) r[c] = v[c] + __shfl_xor(v[c], 40);
-  return r;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t w_in_of(const LayerArgs& a, int e) {
+  const uint32_t bytes = 4 * a.inter * a.hidden;  // below 2 GiB
+  return matrix_at(a.w_in + (size_t)e * bytes, bytes);
 }
-__device__ __forceinline__ bool holds_result() { return (threadIdx.x % kWave) < 32 && (threadIdx.x % 16) < 8; }
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t w_out_of(const LayerArgs& a, int e) {
+  const uint32_t bytes = 2 * a.inter * a.hidden;
+  return matrix_at(a.w_out + (size_t)e * bytes, bytes);
+}
 
 // The next pairs of expert e in ascending order into `list`, from pair `from` on: at least kListPairs of them
 // if there are as many, at most kListSpace; returns how many and leaves in `from` where to go on.  Every
@@ -162,8 +160,8 @@ template <int DT, int NT, int STEPS>
 __device__ __forceinline__ void layer_in_tokens(const LayerArgs& a, int e, uint32_t i0, const uint16_t* list, uint32_t m0, uint32_t m,
                                                 float (*sums)[4][NT][8][8]) {
   using S = typename Elem<DT>::store_t;
-  const uint32_t lane = threadIdx.x % kWave, wave = wave_index();
-  const uint32_t r = lane % 8, col = lane_column();
+  const uint32_t wave = wave_index();
+  const uint32_t r = lane_member(), col = lane_column();
   uint32_t w[4], b[NT];
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
@@ -182,13 +180,13 @@ __device__ __forceinline__ void layer_in_tokens(const LayerArgs& a, int e, uint3
     for (int t = 0; t < NT; ++t) acc[n][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   const uint32_t steps = (a.hidden + kStepCols - 1) / kStepCols, per = (steps + kInWaves - 1) / kInWaves;
   const uint32_t s0 = wave * per, s1 = s0 + per < steps ? s0 + per : steps;
-  multiply_sets<DT, 4, NT, STEPS>(a.w_in + (size_t)e * 2 * a.inter * a.hidden * 2, w, a.x, b, s0, s1, a.hidden, acc);
+  multiply_sets<DT, 4, NT, STEPS>(w_in_of(a, e), w, matrix_at(a.x, a.tokens * a.hidden * 2), b, s0, s1, a.hidden, acc);
 #pragma unroll
   for (int n = 0; n < 4; ++n)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const f32x4 v = add_halves(acc[n][t]);
-      if (holds_result()) *(f32x4*)&sums[wave][n][t][r][lane / 16 * 4] = v;
+      const f32x2 v = add_halves(acc[n][t]);
+      if (lane_holds()) *(f32x2*)&sums[wave][n][t][r][lane_row()] = v;
     }
   __syncthreads();
   for (uint32_t o = threadIdx.x; o < NT * 8 * kInRows; o += kInWaves * kWave) {
@@ -251,8 +249,7 @@ __host__ __device__ inline LayerOutLds layer_out_lds(uint32_t pairs, uint32_t ex
 template <int DT, int NW, int NT, int STEPS>
 __device__ __forceinline__ void layer_out_tokens(const LayerArgs& a, int e, uint32_t c0, uint32_t part, const uint16_t* list, uint32_t m0,
                                                  uint32_t m, float* y) {
-  const uint32_t lane = threadIdx.x % kWave;
-  const uint32_t r = lane % 8, col = lane_column();
+  const uint32_t r = lane_member(), col = lane_column();
   uint32_t w[NW], b[NT];
 #pragma unroll
   for (int n = 0; n < NW; ++n) {
@@ -271,14 +268,14 @@ __device__ __forceinline__ void layer_out_tokens(const LayerArgs& a, int e, uint
     for (int t = 0; t < NT; ++t) acc[n][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   const uint32_t steps = (a.inter + kStepCols - 1) / kStepCols, per = (steps + a.parts - 1) / a.parts;
   const uint32_t s0 = part * per, s1 = s0 + per < steps ? s0 + per : steps;
-  multiply_sets<DT, NW, NT, STEPS>(a.w_out + (size_t)e * a.hidden * a.inter * 2, w, a.h, b, s0, s1, a.inter, acc);
+  multiply_sets<DT, NW, NT, STEPS>(w_out_of(a, e), w, matrix_at(a.h, a.pairs * a.inter * 2), b, s0, s1, a.inter, acc);
 #pragma unroll
   for (int n = 0; n < NW; ++n)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const f32x4 v = add_halves(acc[n][t]);
-      if (holds_result() && m0 + t * 8 + r < m)
-        *(f32x4*)(y + (((size_t)list[m0 + t * 8 + r] * a.parts + part) * NW + n) * kSetRows + lane / 16 * 4) = v;
+      const f32x2 v = add_halves(acc[n][t]);
+      if (lane_holds() && m0 + t * 8 + r < m)
+        *(f32x2*)(y + (((size_t)list[m0 + t * 8 + r] * a.parts + part) * NW + n) * kSetRows + lane_row()) = v;
     }
 }
 
@@ -353,84 +350,85 @@ __global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArg
 // ------------------------------------------------------------------------------------------
 // The same products where an expert has so many tokens that reading them again for every 16 rows costs
 // more than the weights: a workgroup takes 8 wavefronts x NW sets of rows over all (or a part) of the
-// columns, and the tokens go through LDS, 128 columns of TOKENS of them at a time.  While a chunk is
+// columns, and the tokens go through LDS, a chunk of columns of TOKENS of them at a time.  While a chunk is
 // multiplied, the rows and tokens of the next one are on their way into registers.
 constexpr int kDenseWaves = 8;
-constexpr int kDenseCols = 2 * kStepCols;
+// Steps of columns in a chunk: as many as the registers have room for beside the sums of TOKENS tokens.
+constexpr int dense_steps(int tokens) { return tokens > 64 ? 2 : 4; }
+constexpr uint32_t kDenseMinCols = 2 * kStepCols;
 
-// acc = rows . tokens over the columns of the chunks [c0, c1); tokens: row offsets of this thread's share of
-// the staging, one per 32 tokens.  `space` holds two chunks of TOKENS x kDenseCols values; the 16-byte pieces
-// of a token's 128 bytes are stored in an order turned by the token, so that the 8 tokens which a load from
-// LDS takes at the same columns lie in different banks.
+// Tokens that one thread stages a 16-byte piece of.
+constexpr int dense_share(int tokens) { return tokens * dense_steps(tokens) * 8 / (kDenseWaves * kWave); }
+
+// acc = rows . tokens over the columns of the chunks [c0, c1); from: where this thread's pieces of the tokens
+// begin.  `space` holds two chunks of TOKENS tokens; the
+// 16-byte pieces of a token's 128 bytes are stored in an order turned by the token, so that the 8 tokens
+// which a load from LDS takes at the same columns lie in different banks.
 template <int DT, int NW, int TOKENS>
-__device__ __forceinline__ void multiply_dense(const char* rows, const uint32_t (&w)[NW], const char* tokens, const uint32_t (&from)[TOKENS / 32],
-                                               uint32_t used, uint32_t c0, uint32_t c1, uint32_t depth, char* space,
-                                               f32x4 (&acc)[NW][TOKENS / 8]) {
-  constexpr int kShare = TOKENS / 32;
-  constexpr uint32_t kRowBytes = kDenseCols * 2;
-  const uint32_t lane = threadIdx.x % kWave;
-  const uint32_t piece = threadIdx.x % 16, token = threadIdx.x / 16;       // staging: 16 pieces a token
-  const uint32_t put = token * kRowBytes + (piece / 8) * 128 + ((piece ^ token) % 8) * 16;
-  const uint32_t r = lane % 8, q8 = (lane % 16) / 8 * 4 + lane / 16;       // products: token in its set, piece of its 128 bytes
-  const uint32_t get = r * kRowBytes + ((q8 ^ r) % 8) * 16;
-  u32x4 wv[2][NW], tv[kShare];
-  const auto load = [&](uint32_t c) {
-    const uint32_t k = c * kDenseCols;
-    const bool whole = k + kDenseCols <= depth;
+__device__ __forceinline__ void multiply_dense(__amdgpu_buffer_rsrc_t rows, const uint32_t (&w)[NW], __amdgpu_buffer_rsrc_t tokens,
+                                               const uint32_t (&from)[dense_share(TOKENS)], uint32_t used, uint32_t c0, uint32_t c1,
+                                               uint32_t depth, char* space, f32x4 (&acc)[NW][TOKENS / 8]) {
+  constexpr int kSteps = dense_steps(TOKENS), kPieces = kSteps * 8, kShare = dense_share(TOKENS), kStaged = kDenseWaves * kWave / kPieces;
+  constexpr uint32_t kCols = kSteps * kStepCols, kRowBytes = kCols * 2;
+  const uint32_t col = lane_column();
+  const uint32_t piece = threadIdx.x % kPieces, token = threadIdx.x / kPieces;  // staging
+  const uint32_t put = token * kRowBytes + (piece / 8) * 128 + ((piece ^ (token * 2)) % 8) * 16;
+  const uint32_t r = lane_member();
+  const uint32_t get = r * kRowBytes + ((col / 8) ^ (r * 2 % 8)) * 16;
+  const uint32_t end = c1 * kCols < depth ? c1 * kCols : depth;
+  u32x4 wv[2][kSteps][NW], tv[kShare];
+  const auto load = [&](uint32_t c, u32x4(&v)[kSteps][NW]) {
+    const uint32_t k = c * kCols;
+    const uint32_t tokens_out = k + piece * 8 < end ? 0 : kOutside;
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) {
-      tv[i] = (u32x4){0u, 0u, 0u, 0u};
-      if (i * 32u < used && (whole || k + piece * 8 < depth)) tv[i] = *(const u32x4*)(tokens + (size_t)k * 2 + from[i]);
+    for (int i = 0; i < kShare; ++i) tv[i] = __builtin_amdgcn_raw_buffer_load_b128(tokens, from[i] | tokens_out, k * 2, 0);
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) {
+      const uint32_t out = k + u * kStepCols + col < end ? 0 : kOutside;
+#pragma unroll
+      for (int n = 0; n < NW; ++n) v[u][n] = __builtin_amdgcn_raw_buffer_load_b128(rows, w[n] | out, (k + u * kStepCols) * 2, kStreamed);
     }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int n = 0; n < NW; ++n) {
-        wv[u][n] = (u32x4){0u, 0u, 0u, 0u};
-        if (whole || k + u * kStepCols + q8 * 8 < depth)
-          wv[u][n] = __builtin_nontemporal_load((const u32x4*)(rows + (size_t)(k + u * kStepCols) * 2 + w[n]));
-      }
   };
-  load(c0);
-  for (uint32_t c = c0; c < c1; ++c) {
-    char* buf = space + (c & 1) * (TOKENS * kRowBytes);
-    u32x4 now[2][NW];
+  const auto turn = [&](uint32_t c, u32x4(&now)[kSteps][NW], u32x4(&next)[kSteps][NW], char* buf) {
 #pragma unroll
-    for (int i = 0; i < kShare; ++i)
-      if (i * 32u < used) *(u32x4*)(buf + put + i * 32 * kRowBytes) = tv[i];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int n = 0; n < NW; ++n) now[u][n] = wv[u][n];
+    for (int i = 0; i < kShare; ++i) *(u32x4*)(buf + put + i * kStaged * kRowBytes) = tv[i];
     __syncthreads();
-    if (c + 1 < c1) load(c + 1);
+    load(c + 1, next);  // behind the last chunk: columns outside, nothing is read
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int t = 0; t < TOKENS / 8; ++t) {
+      if (t * 8u >= used) break;
 #pragma unroll
-      for (int t = 0; t < TOKENS / 8; ++t) {
-        if (t * 8u >= used) continue;
+      for (int u = 0; u < kSteps; ++u) {
         const u32x4 b = *(const u32x4*)(buf + get + t * 8 * kRowBytes + u * 128);
 #pragma unroll
         for (int n = 0; n < NW; ++n) acc[n][t] = mfma_16x16x32<DT>(now[u][n], b, acc[n][t]);
       }
+    }
+  };
+  load(c0, wv[0]);
+  for (uint32_t c = c0; c < c1; c += 2) {
+    turn(c, wv[0], wv[1], space);
+    if (c + 1 < c1) turn(c + 1, wv[1], wv[0], space + TOKENS * kRowBytes);
   }
   __syncthreads();  // the space may be filled for the next tokens
 }
 
 // Pairs of the workgroup's expert, TOKENS at a time, in the order of `list` (which holds them all).
 template <int DT, int TOKENS, bool IN>
-__global__ __launch_bounds__(kDenseWaves * kWave) void layer_dense_kernel(const LayerArgs a) {
+__global__ __launch_bounds__(kDenseWaves * kWave, 2) void layer_dense_kernel(const LayerArgs a) {
   using S = typename Elem<DT>::store_t;
-  __shared__ __align__(16) char space[2 * TOKENS * kDenseCols * 2];
+  constexpr uint32_t kPieces = dense_steps(TOKENS) * 8, kCols = kPieces * 8, kStaged = kDenseWaves * kWave / kPieces;
+  __shared__ __align__(16) char space[2 * TOKENS * kCols * 2];
   __shared__ uint16_t list[kLayerMaxPairs + kWave];
   const int e = (int)blockIdx.y;
   uint32_t m = 0;
   for (uint32_t from = 0; from < a.pairs;) m += list_pairs(a.pairs, e, from, list + m, [&](uint32_t p) { return local_expert(a, p); });
   if (m == 0) return;
-  const uint32_t lane = threadIdx.x % kWave, wave = wave_index();
-  const uint32_t r = lane % 8, col = lane_column(), part = blockIdx.z;
+  const uint32_t wave = wave_index();
+  const uint32_t r = lane_member(), col = lane_column(), part = blockIdx.z;
   const uint32_t depth = IN ? a.hidden : a.inter, nrows = IN ? a.inter : a.hidden;
-  const uint32_t chunks = (depth + kDenseCols - 1) / kDenseCols, per = IN ? chunks : (chunks + a.parts - 1) / a.parts;
+  const uint32_t chunks = (depth + kCols - 1) / kCols, per = IN ? chunks : (chunks + a.parts - 1) / a.parts;
   const uint32_t c0 = part * per, c1 = c0 + per < chunks ? c0 + per : chunks;
   const uint32_t row0 = IN ? (blockIdx.x * kDenseWaves + wave) * kSetRows : (blockIdx.x * kDenseWaves + wave) * 2 * kSetRows;
   uint32_t w[2];
@@ -439,39 +437,40 @@ __global__ __launch_bounds__(kDenseWaves * kWave) void layer_dense_kernel(const 
     const uint32_t row = row0 + (IN ? 0 : n * kSetRows) + r;
     w[n] = (((row < nrows ? row : nrows - 1) + (IN ? n * a.inter : 0)) * depth + col) * 2;
   }
-  const char* rows = (IN ? a.w_in + (size_t)e * 2 * a.inter * a.hidden * 2 : a.w_out + (size_t)e * a.hidden * a.inter * 2);
+  const __amdgpu_buffer_rsrc_t rows = IN ? w_in_of(a, e) : w_out_of(a, e);
+  const __amdgpu_buffer_rsrc_t tokens = IN ? matrix_at(a.x, a.tokens * a.hidden * 2) : matrix_at(a.h, a.pairs * a.inter * 2);
   for (uint32_t m0 = 0; m0 < m; m0 += TOKENS) {
     const uint32_t used = m - m0 < TOKENS ? m - m0 : TOKENS;
-    uint32_t from[TOKENS / 32];
+    uint32_t from[dense_share(TOKENS)];
 #pragma unroll
-    for (int i = 0; i < TOKENS / 32; ++i) {
-      const uint32_t t = i * 32 + threadIdx.x / 16;
-      const uint32_t pair = list[m0 + (t < used ? t : used - 1)];
-      from[i] = ((IN ? pair / a.topk : pair) * depth + threadIdx.x % 16 * 8) * 2;
+    for (int i = 0; i < dense_share(TOKENS); ++i) {
+      const uint32_t t = i * kStaged + threadIdx.x / kPieces;
+      const uint32_t pair = list[m0 + (t < used ? t : 0)];
+      from[i] = t < used ? ((IN ? pair / a.topk : pair) * depth + threadIdx.x % kPieces * 8) * 2 : kOutside;
     }
     f32x4 acc[2][TOKENS / 8];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int t = 0; t < TOKENS / 8; ++t) acc[n][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    multiply_dense<DT, 2, TOKENS>(rows, w, IN ? a.x : a.h, from, used, c0, c1, depth, space, acc);
+    multiply_dense<DT, 2, TOKENS>(rows, w, tokens, from, used, c0, c1, depth, space, acc);
 #pragma unroll
     for (int t = 0; t < TOKENS / 8; ++t) {
       if (t * 8u >= used) continue;
-      const f32x4 v0 = add_halves(acc[0][t]), v1 = add_halves(acc[1][t]);
-      if (!holds_result() || t * 8 + r >= used) continue;
-      const uint32_t pair = list[m0 + t * 8 + r], row = row0 + lane / 16 * 4;
+      const f32x2 v0 = add_halves(acc[0][t]), v1 = add_halves(acc[1][t]);
+      if (!lane_holds() || t * 8 + r >= used) continue;
+      const uint32_t pair = list[m0 + t * 8 + r], row = row0 + lane_row();
       if constexpr (IN) {
-        if (row < a.inter) {  // inter is a multiple of 8: all four rows or none
-          union { S e[4]; uint2 v; } h;
+        if (row < a.inter) {  // inter is a multiple of 8: both rows or none
+          union { S e[2]; uint32_t v; } h;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) h.e[c] = Elem<DT>::store(activate(v0[c], a.activation) * v1[c]);
-          *(uint2*)((S*)a.h + (size_t)pair * a.inter + row) = h.v;
+          for (int c = 0; c < 2; ++c) h.e[c] = Elem<DT>::store(activate(v0[c], a.activation) * v1[c]);
+          *(uint32_t*)((S*)a.h + (size_t)pair * a.inter + row) = h.v;
         }
       } else {
         float* y = a.y + ((size_t)part * a.pairs + pair) * a.hidden + row;
-        if (row < a.hidden) *(f32x4*)y = v0;
-        if (row + kSetRows < a.hidden) *(f32x4*)(y + kSetRows) = v1;
+        if (row < a.hidden) *(f32x2*)y = v0;
+        if (row + kSetRows < a.hidden) *(f32x2*)(y + kSetRows) = v1;
       }
     }
   }

@@ -162,7 +162,7 @@ LayerPlan plan_layer(size_t pairs, size_t experts, size_t hidden, size_t inter) 
   p.bytes = p.h_bytes;
   if (p.dense) {
     const size_t groups = (hidden + kDenseWaves * 2 * kSetRows - 1) / (kDenseWaves * 2 * kSetRows) * experts;
-    const size_t chunks = (inter + kDenseCols - 1) / kDenseCols;
+    const size_t chunks = (inter + kDenseMinCols - 1) / kDenseMinCols;
     p.parts = (uint32_t)std::min<size_t>({chunks, 8, (512 + groups - 1) / groups});
     p.bytes += p.parts * pairs * hidden * sizeof(float);
   } else {
