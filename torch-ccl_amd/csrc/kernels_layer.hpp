@@ -8,6 +8,7 @@ namespace {
 
 constexpr int kLayerMaxTokens = 256;
 constexpr int kLayerMaxPairs = 4096;
+constexpr uint32_t kFewMaxPairs = 2048;  // of layer_in_kernel and layer_out_kernel
 constexpr int kLayerMaxExperts = 4096;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -127,19 +128,24 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t w_out_of(const LayerArgs& a, i
   return matrix_at(a.w_out + (size_t)e * bytes, bytes);
 }
 
+// The experts of all pairs into LDS: the lists are made from there, at an LDS round trip for every 64 pairs
+// instead of one to memory.  Ends with a barrier.
+__device__ __forceinline__ void stage_experts(const LayerArgs& a, int16_t* expert) {
+  for (uint32_t p = threadIdx.x; p < a.pairs; p += blockDim.x) expert[p] = (int16_t)local_expert(a, p);
+  __syncthreads();
+}
+
 // The next pairs of expert e in ascending order into `list`, from pair `from` on: at least kListPairs of them
 // if there are as many, at most kListSpace; returns how many and leaves in `from` where to go on.  Every
-// wavefront lists for itself (several that share the space write the same values).  `expert_of(p)` is the
-// expert of pair p.
+// wavefront lists for itself (several that share the space write the same values).
 constexpr uint32_t kListPairs = 64;
 constexpr uint32_t kListSpace = kListPairs + kWave;
 
-template <typename F>
-__device__ __forceinline__ uint32_t list_pairs(uint32_t pairs, int e, uint32_t& from, uint16_t* list, F expert_of) {
+__device__ __forceinline__ uint32_t list_pairs(const int16_t* expert, uint32_t pairs, int e, uint32_t& from, uint16_t* list) {
   const uint32_t lane = threadIdx.x % kWave;
   uint32_t m = 0;
   for (; from < pairs && m < kListPairs; from += kWave) {
-    const bool mine = from + lane < pairs && expert_of(from + lane) == e;
+    const bool mine = from + lane < pairs && expert[from + lane] == e;
     const uint64_t set = __ballot(mine);
     if (mine) list[m + __popcll(set & ((1ull << lane) - 1))] = (uint16_t)(from + lane);
     m += (uint32_t)__popcll(set);
@@ -206,14 +212,16 @@ __device__ __forceinline__ void layer_in_tokens(const LayerArgs& a, int e, uint3
 // TOKENS bounds how many tokens one reading of the weights serves (and with it the registers).
 template <int DT, int TOKENS>
 __global__ __launch_bounds__(kInWaves * kWave) void layer_in_kernel(const LayerArgs a) {
+  __shared__ int16_t expert[kFewMaxPairs];
   __shared__ uint16_t list[kListSpace];
   __shared__ float sums[kInWaves * 4 * (TOKENS / 8) * 64];
-  const int e = a.by_pair ? __builtin_amdgcn_readfirstlane(local_expert(a, blockIdx.y)) : (int)blockIdx.y;
+  stage_experts(a, expert);
+  const int e = a.by_pair ? __builtin_amdgcn_readfirstlane(expert[blockIdx.y]) : (int)blockIdx.y;
   if (e < 0) return;
   const uint32_t i0 = blockIdx.x * kInRows;
   for (uint32_t from = 0; from < a.pairs;) {
     const bool begins = from == 0;
-    const uint32_t m = list_pairs(a.pairs, e, from, list, [&](uint32_t p) { return local_expert(a, p); });
+    const uint32_t m = list_pairs(expert, a.pairs, e, from, list);
     if (begins && a.by_pair && (m == 0 || list[0] != blockIdx.y)) return;  // of the pairs of an expert the first one works
     uint32_t m0 = 0;
     if constexpr (TOKENS >= 32)
@@ -230,8 +238,6 @@ __global__ __launch_bounds__(kInWaves * kWave) void layer_in_kernel(const LayerA
 // A workgroup takes kSetRows * NW rows of w_out of every expert that was chosen and keeps the products of
 // all pairs in LDS, so that the weighted sum needs no other workgroup: work of a wavefront is an expert
 // and one of a.parts parts of inter.
-constexpr uint32_t kOutMaxPairs = 2048;
-
 struct LayerOutLds {
   uint32_t first, active, lists, y, bytes;
 };
@@ -299,9 +305,8 @@ __global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArg
   float* y = (float*)(lds + l.y);
   const uint32_t lane = threadIdx.x % kWave, wave = wave_index();
   uint16_t* list = (uint16_t*)(lds + l.lists) + wave * kListSpace;
-  for (uint32_t p = threadIdx.x; p < a.pairs; p += WAVES * kWave) expert[p] = (int16_t)local_expert(a, p);
   for (uint32_t e = threadIdx.x; e < a.experts; e += WAVES * kWave) first[e] = ~0u;
-  __syncthreads();
+  stage_experts(a, expert);
   for (uint32_t p = threadIdx.x; p < a.pairs; p += WAVES * kWave)
     if (expert[p] >= 0) atomicMin(&first[expert[p]], p);
   __syncthreads();
@@ -322,7 +327,7 @@ __global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArg
     const int e = __builtin_amdgcn_readfirstlane(expert[from]);
     from = from / kWave * kWave;
     while (from < a.pairs) {
-      const uint32_t m = list_pairs(a.pairs, e, from, list, [&](uint32_t p) { return (int)expert[p]; });
+      const uint32_t m = list_pairs(expert, a.pairs, e, from, list);
       uint32_t m0 = 0;
       for (; m0 < m && m - m0 > 16; m0 += 32) layer_out_tokens<DT, NW, 4, 2>(a, e, c0, part, list, m0, m, y);
       for (; m0 < m && m - m0 > 8; m0 += 16) layer_out_tokens<DT, NW, 2, 4>(a, e, c0, part, list, m0, m, y);
@@ -349,117 +354,127 @@ __global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArg
 // many tokens per expert
 // ------------------------------------------------------------------------------------------
 // The same products where an expert has so many tokens that reading them again for every 16 rows costs
-// more than the weights: a workgroup takes 8 wavefronts x NW sets of rows over all (or a part) of the
-// columns, and the tokens go through LDS, a chunk of columns of TOKENS of them at a time.  While a chunk is
-// multiplied, the rows and tokens of the next one are on their way into registers.
+// more than the weights.  A tile is 8 wavefronts x 2 sets of rows of an expert, over all of hidden (first
+// product: 64 gate rows and their up rows) or one part of inter (second product: 128 rows).  Its tokens go
+// through LDS, a chunk of columns of TOKENS of them at a time.  While a chunk is multiplied, the rows and
+// tokens of the next one are on their way into registers.
 constexpr int kDenseWaves = 8;
+constexpr int kDenseBlock = kDenseWaves * kWave;
+constexpr uint32_t kDenseInRows = kDenseWaves * kSetRows, kDenseOutRows = 2 * kDenseInRows;
+
 // Steps of columns in a chunk: as many as the registers have room for beside the sums of TOKENS tokens.
 constexpr int dense_steps(int tokens) { return tokens > 64 ? 2 : 4; }
-constexpr uint32_t kDenseMinCols = 2 * kStepCols;
-
 // Tokens that one thread stages a 16-byte piece of.
-constexpr int dense_share(int tokens) { return tokens * dense_steps(tokens) * 8 / (kDenseWaves * kWave); }
+constexpr int dense_share(int tokens) { return tokens * dense_steps(tokens) * 8 / kDenseBlock; }
 
-// acc = rows . tokens over the columns of the chunks [c0, c1); from: where this thread's pieces of the tokens
-// begin.  `space` holds two chunks of TOKENS tokens; the
-// 16-byte pieces of a token's 128 bytes are stored in an order turned by the token, so that the 8 tokens
-// which a load from LDS takes at the same columns lie in different banks.
-template <int DT, int NW, int TOKENS>
-__device__ __forceinline__ void multiply_dense(__amdgpu_buffer_rsrc_t rows, const uint32_t (&w)[NW], __amdgpu_buffer_rsrc_t tokens,
-                                               const uint32_t (&from)[dense_share(TOKENS)], uint32_t used, uint32_t c0, uint32_t c1,
-                                               uint32_t depth, char* space, f32x4 (&acc)[NW][TOKENS / 8]) {
-  constexpr int kSteps = dense_steps(TOKENS), kPieces = kSteps * 8, kShare = dense_share(TOKENS), kStaged = kDenseWaves * kWave / kPieces;
-  constexpr uint32_t kCols = kSteps * kStepCols, kRowBytes = kCols * 2;
-  const uint32_t col = lane_column();
-  const uint32_t piece = threadIdx.x % kPieces, token = threadIdx.x / kPieces;  // staging
-  const uint32_t put = token * kRowBytes + (piece / 8) * 128 + ((piece ^ (token * 2)) % 8) * 16;
-  const uint32_t r = lane_member();
-  const uint32_t get = r * kRowBytes + ((col / 8) ^ (r * 2 % 8)) * 16;
-  const uint32_t end = c1 * kCols < depth ? c1 * kCols : depth;
-  u32x4 wv[2][kSteps][NW], tv[kShare];
-  const auto load = [&](uint32_t c, u32x4(&v)[kSteps][NW]) {
-    const uint32_t k = c * kCols;
-    const uint32_t tokens_out = k + piece * 8 < end ? 0 : kOutside;
-#pragma unroll
-    for (int i = 0; i < kShare; ++i) tv[i] = __builtin_amdgcn_raw_buffer_load_b128(tokens, from[i] | tokens_out, k * 2, 0);
-#pragma unroll
-    for (int u = 0; u < kSteps; ++u) {
-      const uint32_t out = k + u * kStepCols + col < end ? 0 : kOutside;
-#pragma unroll
-      for (int n = 0; n < NW; ++n) v[u][n] = __builtin_amdgcn_raw_buffer_load_b128(rows, w[n] | out, (k + u * kStepCols) * 2, kStreamed);
-    }
-  };
-  const auto turn = [&](uint32_t c, u32x4(&now)[kSteps][NW], u32x4(&next)[kSteps][NW], char* buf) {
-#pragma unroll
-    for (int i = 0; i < kShare; ++i) *(u32x4*)(buf + put + i * kStaged * kRowBytes) = tv[i];
-    __syncthreads();
-    load(c + 1, next);  // behind the last chunk: columns outside, nothing is read
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int t = 0; t < TOKENS / 8; ++t) {
-      if (t * 8u >= used) break;
-#pragma unroll
-      for (int u = 0; u < kSteps; ++u) {
-        const u32x4 b = *(const u32x4*)(buf + get + t * 8 * kRowBytes + u * 128);
-#pragma unroll
-        for (int n = 0; n < NW; ++n) acc[n][t] = mfma_16x16x32<DT>(now[u][n], b, acc[n][t]);
-      }
-    }
-  };
-  load(c0, wv[0]);
-  for (uint32_t c = c0; c < c1; c += 2) {
-    turn(c, wv[0], wv[1], space);
-    if (c + 1 < c1) turn(c + 1, wv[1], wv[0], space + TOKENS * kRowBytes);
-  }
-  __syncthreads();  // the space may be filled for the next tokens
-}
-
-// Pairs of the workgroup's expert, TOKENS at a time, in the order of `list` (which holds them all).
 template <int DT, int TOKENS, bool IN>
-__global__ __launch_bounds__(kDenseWaves * kWave, 2) void layer_dense_kernel(const LayerArgs a) {
+__global__ __launch_bounds__(kDenseBlock, 2) void layer_dense_kernel(const LayerArgs a) {
   using S = typename Elem<DT>::store_t;
-  constexpr uint32_t kPieces = dense_steps(TOKENS) * 8, kCols = kPieces * 8, kStaged = kDenseWaves * kWave / kPieces;
-  __shared__ __align__(16) char space[2 * TOKENS * kCols * 2];
-  __shared__ uint16_t list[kLayerMaxPairs + kWave];
-  const int e = (int)blockIdx.y;
-  uint32_t m = 0;
-  for (uint32_t from = 0; from < a.pairs;) m += list_pairs(a.pairs, e, from, list + m, [&](uint32_t p) { return local_expert(a, p); });
-  if (m == 0) return;
-  const uint32_t wave = wave_index();
-  const uint32_t r = lane_member(), col = lane_column(), part = blockIdx.z;
+  constexpr int kSteps = dense_steps(TOKENS), kPieces = kSteps * 8, kShare = dense_share(TOKENS), kStaged = kDenseBlock / kPieces;
+  constexpr uint32_t kCols = kSteps * kStepCols, kRowBytes = kCols * 2;
+  __shared__ __align__(16) char space[2 * TOKENS * kRowBytes];  // two chunks of the tokens
+  __shared__ int16_t expert[kLayerMaxPairs];
+  __shared__ uint16_t list[kLayerMaxPairs];
+  const uint32_t wave = wave_index(), r = lane_member(), col = lane_column();
   const uint32_t depth = IN ? a.hidden : a.inter, nrows = IN ? a.inter : a.hidden;
   const uint32_t chunks = (depth + kCols - 1) / kCols, per = IN ? chunks : (chunks + a.parts - 1) / a.parts;
-  const uint32_t c0 = part * per, c1 = c0 + per < chunks ? c0 + per : chunks;
-  const uint32_t row0 = IN ? (blockIdx.x * kDenseWaves + wave) * kSetRows : (blockIdx.x * kDenseWaves + wave) * 2 * kSetRows;
+  const uint32_t row_tiles = (nrows + (IN ? kDenseInRows : kDenseOutRows) - 1) / (IN ? kDenseInRows : kDenseOutRows);
+
+  // The tile: neighbouring workgroups take neighbouring rows of one expert, which share its tokens.
+  const uint32_t rest = blockIdx.x / row_tiles, part = IN ? 0 : rest / a.experts, e = rest - part * a.experts;
+  const uint32_t row0 = (blockIdx.x - rest * row_tiles) * (IN ? kDenseInRows : kDenseOutRows) + wave * (IN ? 1 : 2) * kSetRows;
   uint32_t w[2];
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     const uint32_t row = row0 + (IN ? 0 : n * kSetRows) + r;
     w[n] = (((row < nrows ? row : nrows - 1) + (IN ? n * a.inter : 0)) * depth + col) * 2;
   }
-  const __amdgpu_buffer_rsrc_t rows = IN ? w_in_of(a, e) : w_out_of(a, e);
+  const uint32_t c0 = part * per, c1 = c0 + per < chunks ? c0 + per : chunks;
+  const uint32_t end = c1 * kCols < depth ? c1 * kCols : depth;
+  const __amdgpu_buffer_rsrc_t rows = IN ? w_in_of(a, (int)e) : w_out_of(a, (int)e);
+  // Columns from `end` on (whole chunks too) are outside and not read.
+  const auto load_rows = [&](uint32_t c, u32x4(&v)[kSteps][2]) {
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) {
+      const uint32_t k = c * kCols + u * kStepCols, out = k + col < end ? 0 : kOutside;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) v[u][n] = __builtin_amdgcn_raw_buffer_load_b128(rows, w[n] | out, k * 2, kStreamed);
+    }
+  };
+
+  // Staging: a thread's piece of a token's 128 bytes, which are stored in an order turned by the token so that
+  // the 8 tokens which a load from LDS takes at the same columns lie in different banks.
   const __amdgpu_buffer_rsrc_t tokens = IN ? matrix_at(a.x, a.tokens * a.hidden * 2) : matrix_at(a.h, a.pairs * a.inter * 2);
+  const uint32_t piece = threadIdx.x % kPieces, staged = threadIdx.x / kPieces;
+  const uint32_t put = staged * kRowBytes + (piece / 8) * 128 + ((piece ^ (staged * 2)) % 8) * 16;
+  const uint32_t get = r * kRowBytes + ((col / 8) ^ (r * 2 % 8)) * 16;
+
+  u32x4 wv[2][kSteps][2], tv[kShare];
+  stage_experts(a, expert);
+  uint32_t m = 0, turns = 0;
+  for (uint32_t from = 0; from < a.pairs;) m += list_pairs(expert, a.pairs, (int)e, from, list + m);
   for (uint32_t m0 = 0; m0 < m; m0 += TOKENS) {
     const uint32_t used = m - m0 < TOKENS ? m - m0 : TOKENS;
-    uint32_t from[dense_share(TOKENS)];
+    uint32_t from[kShare];
 #pragma unroll
-    for (int i = 0; i < dense_share(TOKENS); ++i) {
-      const uint32_t t = i * kStaged + threadIdx.x / kPieces;
-      const uint32_t pair = list[m0 + (t < used ? t : 0)];
-      from[i] = t < used ? ((IN ? pair / a.topk : pair) * depth + threadIdx.x % kPieces * 8) * 2 : kOutside;
+    for (int i = 0; i < kShare; ++i) {
+      const uint32_t at = i * kStaged + staged, pair = list[m0 + (at < used ? at : 0)];
+      from[i] = at < used ? ((IN ? pair / a.topk : pair) * depth + piece * 8) * 2 : kOutside;
     }
+    const auto load_tokens = [&](uint32_t c) {
+      const uint32_t k = c * kCols, out = k + piece * 8 < end ? 0 : kOutside;
+#pragma unroll
+      for (int i = 0; i < kShare; ++i) tv[i] = __builtin_amdgcn_raw_buffer_load_b128(tokens, from[i] | out, k * 2, 0);
+    };
     f32x4 acc[2][TOKENS / 8];
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int t = 0; t < TOKENS / 8; ++t) acc[n][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    multiply_dense<DT, 2, TOKENS>(rows, w, tokens, from, used, c0, c1, depth, space, acc);
+      for (int g = 0; g < TOKENS / 8; ++g) acc[n][g] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    const auto stage = [&]() {
+      char* buf = space + (turns & 1) * (TOKENS * kRowBytes);
 #pragma unroll
-    for (int t = 0; t < TOKENS / 8; ++t) {
-      if (t * 8u >= used) continue;
-      const f32x2 v0 = add_halves(acc[0][t]), v1 = add_halves(acc[1][t]);
-      if (!lane_holds() || t * 8 + r >= used) continue;
-      const uint32_t pair = list[m0 + t * 8 + r], row = row0 + lane_row();
+      for (int i = 0; i < kShare; ++i) *(u32x4*)(buf + put + i * kStaged * kRowBytes) = tv[i];
+      __syncthreads();
+    };
+    const auto product = [&](const u32x4(&v)[kSteps][2]) {
+      const char* buf = space + (turns & 1) * (TOKENS * kRowBytes) + get;
+      __builtin_amdgcn_sched_barrier(0);  // the loads go first
+#pragma unroll
+      for (int g = 0; g < TOKENS / 8; g += 2) {  // 16 tokens: as many loads from LDS in flight
+        if (g * 8u >= used) break;
+        u32x4 b[2][kSteps];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int u = 0; u < kSteps; ++u) b[i][u] = *(const u32x4*)(buf + (g + i) * 8 * kRowBytes + u * 128);
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) acc[n][g + i] = mfma_16x16x32<DT>(v[u][n], b[i][u], acc[n][g + i]);
+      }
+      ++turns;
+    };
+    load_tokens(c0);
+    if (m0 == 0) load_rows(c0, wv[0]);
+    for (uint32_t c = c0; c < c1; c += 2) {
+      stage();
+      load_tokens(c + 1);
+      load_rows(c + 1, wv[1]);
+      product(wv[0]);
+      if (c + 1 < c1) stage();
+      load_tokens(c + 2);
+      load_rows(c + 2 < c1 || m0 + TOKENS >= m ? c + 2 : c0, wv[0]);  // behind the last chunk the first, for the next tokens
+      if (c + 1 < c1) product(wv[1]);
+    }
+#pragma unroll
+    for (int g = 0; g < TOKENS / 8; ++g) {
+      if (g * 8u >= used) break;
+      const f32x2 v0 = add_halves(acc[0][g]), v1 = add_halves(acc[1][g]);
+      if (!lane_holds() || g * 8 + r >= used) continue;
+      const uint32_t pair = list[m0 + g * 8 + r], row = row0 + lane_row();
       if constexpr (IN) {
         if (row < a.inter) {  // inter is a multiple of 8: both rows or none
           union { S e[2]; uint32_t v; } h;

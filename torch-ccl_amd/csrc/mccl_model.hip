@@ -149,21 +149,23 @@ int check_router(size_t tokens, size_t experts, int topk, int dtype) {
 
 // How a layer is run, from its sizes alone (the routing is only known on the device).
 struct LayerPlan {
-  bool dense;      // many tokens per expert: layer_dense_kernel
+  int dense;       // tokens of a tile of layer_dense_kernel, 0: few tokens per expert
   uint32_t parts;  // of inter, in the second product
   size_t h_bytes, bytes;
 };
 
 constexpr size_t kDensePairs = 16;  // per expert
-LayerPlan plan_layer(size_t pairs, size_t experts, size_t hidden, size_t inter) {
+LayerPlan plan_layer(size_t tokens, size_t pairs, size_t experts, size_t hidden, size_t inter) {
   LayerPlan p{};
-  p.dense = pairs > kDensePairs * experts || pairs > kOutMaxPairs;
+  if (pairs > kDensePairs * experts || pairs > kFewMaxPairs)
+    p.dense = tokens <= 32 ? 32 : (tokens <= 64 || pairs <= 48 * experts) ? 64 : 128;
   p.h_bytes = up16(pairs * inter * 2);
   p.bytes = p.h_bytes;
   if (p.dense) {
-    const size_t groups = (hidden + kDenseWaves * 2 * kSetRows - 1) / (kDenseWaves * 2 * kSetRows) * experts;
-    const size_t chunks = (inter + kDenseMinCols - 1) / kDenseMinCols;
-    p.parts = (uint32_t)std::min<size_t>({chunks, 8, (512 + groups - 1) / groups});
+    const size_t groups = (hidden + kDenseOutRows - 1) / kDenseOutRows * experts;
+    const size_t cols = dense_steps(p.dense) * kStepCols, chunks = (inter + cols - 1) / cols;
+    const size_t per = (chunks + std::min<size_t>({chunks, 8, (512 + groups - 1) / groups}) - 1) / std::min<size_t>({chunks, 8, (512 + groups - 1) / groups});
+    p.parts = (uint32_t)((chunks + per - 1) / per);
     p.bytes += p.parts * pairs * hidden * sizeof(float);
   } else {
     p.parts = (uint32_t)std::min<size_t>((inter + kStepCols - 1) / kStepCols, (16 + pairs - 1) / pairs);
@@ -172,12 +174,13 @@ LayerPlan plan_layer(size_t pairs, size_t experts, size_t hidden, size_t inter) 
 }
 
 template <int DT, int TOKENS>
-void launch_dense(const LayerArgs& a, hipStream_t s) {
-  const uint32_t in_rows = kDenseWaves * kSetRows, out_rows = 2 * in_rows;
-  hipLaunchKernelGGL((layer_dense_kernel<DT, TOKENS, true>), dim3((a.inter + in_rows - 1) / in_rows, a.experts), dim3(kDenseWaves * kWave), 0, s, a);
-  hipLaunchKernelGGL((layer_dense_kernel<DT, TOKENS, false>), dim3((a.hidden + out_rows - 1) / out_rows, a.experts, a.parts),
-                     dim3(kDenseWaves * kWave), 0, s, a);
+int launch_dense(const LayerArgs& a, hipStream_t s) {
+  const uint32_t in_tiles = (a.inter + kDenseInRows - 1) / kDenseInRows * a.experts;
+  const uint32_t out_tiles = (a.hidden + kDenseOutRows - 1) / kDenseOutRows * a.experts * a.parts;
+  hipLaunchKernelGGL((layer_dense_kernel<DT, TOKENS, true>), dim3(in_tiles), dim3(kDenseBlock), 0, s, a);
+  hipLaunchKernelGGL((layer_dense_kernel<DT, TOKENS, false>), dim3(out_tiles), dim3(kDenseBlock), 0, s, a);
   hipLaunchKernelGGL(layer_join_kernel<DT>, dim3((a.hidden / 4 + 255) / 256, a.tokens), dim3(256), 0, s, a);
+  return launched("moe layer");
 }
 
 template <int DT, int NW, int WAVES>
@@ -192,13 +195,8 @@ int launch_layer_out(const LayerArgs& a, hipStream_t s) {
 }
 
 template <int DT>
-int launch_layer(const LayerArgs& a, bool dense, hipStream_t s) {
-  if (dense) {
-    if (a.tokens <= 32) launch_dense<DT, 32>(a, s);
-    else if (a.tokens <= 64 || a.pairs <= 48 * a.experts) launch_dense<DT, 64>(a, s);
-    else launch_dense<DT, 128>(a, s);
-    return launched("moe layer");
-  }
+int launch_layer(const LayerArgs& a, int dense, hipStream_t s) {
+  if (dense) return dense == 32 ? launch_dense<DT, 32>(a, s) : dense == 64 ? launch_dense<DT, 64>(a, s) : launch_dense<DT, 128>(a, s);
   const dim3 in_grid((a.inter + kInRows - 1) / kInRows, a.by_pair ? a.pairs : a.experts), in_block(kInWaves * kWave);
   if (a.tokens <= 8) hipLaunchKernelGGL((layer_in_kernel<DT, 8>), in_grid, in_block, 0, s, a);
   else if (a.tokens <= 16) hipLaunchKernelGGL((layer_in_kernel<DT, 16>), in_grid, in_block, 0, s, a);
@@ -377,7 +375,7 @@ int mccl_moe_route_grad(const float* grad_weights, const void* logits, const int
 
 size_t mccl_moe_layer_workspace(size_t tokens, int topk, size_t experts, size_t hidden, size_t inter) {
   if (topk < 1 || tokens == 0 || experts == 0) return 0;
-  return plan_layer(tokens * (size_t)topk, experts, hidden, inter).bytes;
+  return plan_layer(tokens, tokens * (size_t)topk, experts, hidden, inter).bytes;
 }
 
 int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int32_t* expert_ids, const float* weights, size_t tokens,
@@ -400,7 +398,7 @@ int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int
     return mccl_report_error(MCCL_ERR_INVALID_ARG, "x, the weights or the output are not 16-byte aligned");
   if (misaligned(expert_ids, 4) || misaligned(weights, 4)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "expert ids or weights misaligned");
   const size_t pairs = tokens * (size_t)topk, row = tokens * hidden * 2;
-  const LayerPlan plan = plan_layer(pairs, experts, hidden, inter);
+  const LayerPlan plan = plan_layer(tokens, pairs, experts, hidden, inter);
   const size_t need = plan.bytes;
   if (!workspace || misaligned(workspace, 16) || workspace_bytes < need)
     return mccl_report_error(MCCL_ERR_INVALID_ARG, "workspace is null, not 16-byte aligned or smaller than %zu bytes", need);

@@ -283,24 +283,35 @@ def route_counts(expert_ids, n_experts, workspace=None, out=None):
     return out
 
 
-def _check_gpu(what, **tensors):
+def _check_gpu(what, names, tensors):
     """Every tensor on the GPU, contiguous, all on one device; returns that device."""
-    device = None
-    for name, t in tensors.items():
+    device = tensors[0].device
+    for i, t in enumerate(tensors):
         if not t.is_cuda:
             raise RuntimeError("%s: tensors must be on the GPU (got %s)" % (what, t.device))
         if not t.is_contiguous():
-            raise RuntimeError("%s: %s has to be contiguous" % (what, name))
-        if device is not None and t.device != device:
+            raise RuntimeError("%s: %s has to be contiguous" % (what, names[i]))
+        if t.device != device:
             raise RuntimeError("%s: tensors must share one device" % what)
-        device = t.device
     return device
 
 
 def _check_shape(what, name, t, shape, *dtypes):
-    if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes:
+    if t.shape != shape or t.dtype not in dtypes:
         raise RuntimeError("%s: %s must be %s of shape %s (got %s %s)" % (
             what, name, " or ".join(str(d).replace("torch.", "") for d in dtypes), list(shape), t.dtype, list(t.shape)))
+
+
+def _launch(device, entry, *args):
+    """Calls `entry` of the C ABI on the current stream of `device`, which is made current if it is not.
+    These calls are short: the device is switched only where it has to be (1.3 us) and the stream's
+    handle is taken without its Python object (0.1 us against 2.7)."""
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        capi.check(entry(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            capi.check(entry(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 _MODEL_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -308,12 +319,15 @@ _ID_TYPES = (torch.int32, torch.int64)
 
 
 def _workspace(what, given, nbytes, device):
-    """The caller's workspace (uint8, large enough) or one from torch's allocator for this call."""
+    """(address, bytes) of the caller's workspace (uint8, large enough) or of one from torch's allocator
+    for this call, and the tensor itself, to be kept until the call has been made."""
     if given is None:
-        return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
-    if given.dtype != torch.uint8 or given.device != device or not given.is_contiguous() or given.numel() < nbytes:
+        if nbytes == 0:
+            return None, 0, None
+        given = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    elif given.dtype != torch.uint8 or given.device != device or not given.is_contiguous() or given.numel() < nbytes:
         raise RuntimeError("%s: workspace must be %d bytes of uint8 on %s" % (what, nbytes, device))
-    return given
+    return given.data_ptr(), given.numel(), given
 
 
 def embedding(table, ids, scale=1.0, first_row=0, out=None):
@@ -328,11 +342,9 @@ def embedding(table, ids, scale=1.0, first_row=0, out=None):
     if out is None:
         out = torch.empty(shape, dtype=table.dtype, device=table.device)
     _check_shape("embedding", "out", out, shape, table.dtype)
-    device = _check_gpu("embedding", table=table, ids=ids, out=out)
-    with torch.cuda.device(device):
-        capi.check(capi.lib().mccl_embedding(table.data_ptr(), table.shape[0], ids.data_ptr(), _dtype_code(ids.dtype), ids.numel(),
-                                             int(first_row), table.shape[1], float(scale), _dtype_code(table.dtype), out.data_ptr(),
-                                             _stream()))
+    device = _check_gpu("embedding", ("table", "ids", "out"), (table, ids, out))
+    _launch(device, capi.lib().mccl_embedding, table.data_ptr(), table.shape[0], ids.data_ptr(), _dtype_code(ids.dtype), ids.numel(),
+            first_row, table.shape[1], scale, _dtype_code(table.dtype), out.data_ptr())
     return out
 
 
@@ -346,15 +358,13 @@ def sort_ids(ids, rows, first_row=0, workspace=None):
     rows = int(rows)
     if rows < 0:
         raise RuntimeError("sort_ids: negative row count")
-    device = _check_gpu("sort_ids", ids=ids)
+    device = _check_gpu("sort_ids", ("ids",), (ids,))
     n = ids.numel()
-    need = capi.lib().mccl_sort_ids_workspace(n)
     order = torch.empty(n, dtype=torch.int64, device=device)
     offsets = torch.empty(rows + 1, dtype=torch.int64, device=device)
-    ws = _workspace("sort_ids", workspace, need, device)
-    with torch.cuda.device(device):
-        capi.check(capi.lib().mccl_sort_ids(ids.data_ptr(), _dtype_code(ids.dtype), n, int(first_row), rows, ws.data_ptr(), ws.numel(),
-                                            order.data_ptr(), offsets.data_ptr(), _stream()))
+    ws, ws_bytes, _held = _workspace("sort_ids", workspace, capi.lib().mccl_sort_ids_workspace(n), device)
+    _launch(device, capi.lib().mccl_sort_ids, ids.data_ptr(), _dtype_code(ids.dtype), n, first_row, rows, ws, ws_bytes,
+            order.data_ptr(), offsets.data_ptr())
     return order, offsets
 
 
@@ -379,12 +389,10 @@ def embedding_grad(grad, sorted_ids, scale=1.0, dtype=None, out=None, accumulate
             raise RuntimeError("embedding_grad: accumulate needs the tensor to add to (out)")
         out = torch.empty((rows, hidden), dtype=dtype or grad.dtype, device=grad.device)
     _check_shape("embedding_grad", "out", out, (rows, hidden), *((dtype,) if dtype else (grad.dtype, torch.float32)))
-    device = _check_gpu("embedding_grad", grad=grad, order=order, offsets=offsets, out=out)
-    ws = _workspace("embedding_grad", workspace, capi.lib().mccl_embedding_grad_workspace(n, hidden), device)
-    with torch.cuda.device(device):
-        capi.check(capi.lib().mccl_embedding_grad(grad.data_ptr(), order.data_ptr(), offsets.data_ptr(), n, rows, hidden, float(scale),
-                                                  _dtype_code(grad.dtype), out.data_ptr(), _dtype_code(out.dtype), int(bool(accumulate)),
-                                                  ws.data_ptr(), ws.numel(), _stream()))
+    device = _check_gpu("embedding_grad", ("grad", "order", "offsets", "out"), (grad, order, offsets, out))
+    ws, ws_bytes, _held = _workspace("embedding_grad", workspace, capi.lib().mccl_embedding_grad_workspace(n, hidden), device)
+    _launch(device, capi.lib().mccl_embedding_grad, grad.data_ptr(), order.data_ptr(), offsets.data_ptr(), n, rows, hidden, scale,
+            _dtype_code(grad.dtype), out.data_ptr(), _dtype_code(out.dtype), bool(accumulate), ws, ws_bytes)
     return out
 
 
@@ -404,10 +412,9 @@ def moe_route(logits, topk, normalize=True, out=None):
     ids, weights = out
     _check_shape("moe_route", "expert_ids", ids, shape, torch.int32)
     _check_shape("moe_route", "weights", weights, shape, torch.float32)
-    device = _check_gpu("moe_route", logits=logits, expert_ids=ids, weights=weights)
-    with torch.cuda.device(device):
-        capi.check(capi.lib().mccl_moe_route(logits.data_ptr(), tokens, experts, shape[1], int(bool(normalize)), _dtype_code(logits.dtype),
-                                             ids.data_ptr(), weights.data_ptr(), _stream()))
+    device = _check_gpu("moe_route", ("logits", "expert_ids", "weights"), (logits, ids, weights))
+    _launch(device, capi.lib().mccl_moe_route, logits.data_ptr(), tokens, experts, shape[1], bool(normalize), _dtype_code(logits.dtype),
+            ids.data_ptr(), weights.data_ptr())
     return ids, weights
 
 
@@ -425,10 +432,9 @@ def moe_route_grad(grad_weights, logits, expert_ids, normalize=True, out=None):
     _check_shape("moe_route_grad", "expert_ids", expert_ids, (tokens, topk), torch.int32)
     _check_shape("moe_route_grad", "grad_weights", grad_weights, (tokens, topk), torch.float32)
     _check_shape("moe_route_grad", "out", out, logits.shape, logits.dtype)
-    device = _check_gpu("moe_route_grad", grad_weights=grad_weights, logits=logits, expert_ids=expert_ids, out=out)
-    with torch.cuda.device(device):
-        capi.check(capi.lib().mccl_moe_route_grad(grad_weights.data_ptr(), logits.data_ptr(), expert_ids.data_ptr(), tokens, experts, topk,
-                                                  int(bool(normalize)), _dtype_code(logits.dtype), out.data_ptr(), _stream()))
+    device = _check_gpu("moe_route_grad", ("grad_weights", "logits", "expert_ids", "out"), (grad_weights, logits, expert_ids, out))
+    _launch(device, capi.lib().mccl_moe_route_grad, grad_weights.data_ptr(), logits.data_ptr(), expert_ids.data_ptr(), tokens, experts,
+            topk, bool(normalize), _dtype_code(logits.dtype), out.data_ptr())
     return out
 
 
@@ -453,12 +459,10 @@ def moe_layer(x, w_in, w_out, expert_ids, weights, first_expert=0, activation="s
     _check_shape("moe_layer", "expert_ids", expert_ids, (tokens, topk), torch.int32)
     _check_shape("moe_layer", "weights", weights, (tokens, topk), torch.float32)
     _check_shape("moe_layer", "out", out, x.shape, x.dtype)
-    device = _check_gpu("moe_layer", x=x, w_in=w_in, w_out=w_out, expert_ids=expert_ids, weights=weights, out=out)
-    ws = _workspace("moe_layer", workspace, capi.lib().mccl_moe_layer_workspace(tokens, topk, experts, hidden, inter), device)
-    with torch.cuda.device(device):
-        capi.check(capi.lib().mccl_moe_layer(x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), expert_ids.data_ptr(), weights.data_ptr(),
-                                             tokens, topk, experts, int(first_expert), hidden, inter, _ACTIVATIONS[activation],
-                                             _dtype_code(x.dtype), out.data_ptr(), ws.data_ptr(), ws.numel(), _stream()))
+    device = _check_gpu("moe_layer", ("x", "w_in", "w_out", "expert_ids", "weights", "out"), (x, w_in, w_out, expert_ids, weights, out))
+    ws, ws_bytes, _held = _workspace("moe_layer", workspace, capi.lib().mccl_moe_layer_workspace(tokens, topk, experts, hidden, inter), device)
+    _launch(device, capi.lib().mccl_moe_layer, x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), expert_ids.data_ptr(), weights.data_ptr(),
+            tokens, topk, experts, first_expert, hidden, inter, _ACTIVATIONS[activation], _dtype_code(x.dtype), out.data_ptr(), ws, ws_bytes)
     return out
 
 
