@@ -76,7 +76,7 @@ def test_embedding_grad_refusals(abi):
     assert call(order=0x20000004) == -1 and "misaligned" in err()
     assert call(n=(1 << 28) + 1) == -1 and "too long" in err()
     need = L.mccl_embedding_grad_workspace(1000, 64)
-    assert need == 16 * 2 * 64 * 4 and L.mccl_embedding_grad_workspace(64, 64) == 0
+    assert need >= 16 * 2 * 64 * 4 and L.mccl_embedding_grad_workspace(64, 64) == 0
     assert call(n=1000) == -1 and "workspace" in err()
     assert call(n=1000, ws=0x40000000, wsb=need - 4) == -1 and "workspace" in err()
     assert call(out=0x10000000 + 8) == -1 and "overlaps an input" in err()

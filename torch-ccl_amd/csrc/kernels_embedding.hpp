@@ -3,9 +3,32 @@
 // activations, and before and after the exchange of routed tokens).
 #pragma once
 
+#include <type_traits>
+
 #include "kernels_common.hpp"
 
 namespace {
+
+// ------------------------------------------------------------------------------------------
+// conversions
+// ------------------------------------------------------------------------------------------
+// Round to nearest even by the hardware's conversion, two elements an instruction (the exchange kernels'
+// Elem::store makes every NaN the canonical one, at five instructions an element; here a NaN stays a NaN).
+typedef float f32pair __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16pair __attribute__((ext_vector_type(2)));
+typedef _Float16 f16pair __attribute__((ext_vector_type(2)));
+
+template <int DT>
+__device__ __forceinline__ uint32_t narrow_pair(float lo, float hi) {
+  if constexpr (DT == MCCL_BF16) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32pair){lo, hi}, bf16pair));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32pair){lo, hi}, f16pair));
+}
+
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::store_t narrow(float f) {
+  if constexpr (DT == MCCL_F32) return f;
+  else return (typename Elem<DT>::store_t)narrow_pair<DT>(f, 0.0f);
+}
 
 // ------------------------------------------------------------------------------------------
 // rows of any length: a row is cut into 16-byte vectors of the storage type, the last one may be short
@@ -28,8 +51,9 @@ __device__ __forceinline__ void load_vec_f32(const typename Elem<DT>::store_t* p
   for (int e = 0; e < VE; ++e) f[e] = Elem<DT>::load(x.e[e]);
 }
 
-// Stores N values as elements of DT (N may be more than one 16-byte vector of it).
-template <int DT, int N>
+// Stores N values as elements of DT (N may be more than one 16-byte vector of it); STREAM: past the caches, for
+// what is too large to be read from them again.
+template <int DT, bool STREAM = false, int N>
 __device__ __forceinline__ void store_vec_f32(typename Elem<DT>::store_t* p, uint32_t left, const float (&f)[N]) {
   constexpr int VE = vec_elems<DT>();
   static_assert(N % VE == 0, "whole vectors");
@@ -37,14 +61,16 @@ __device__ __forceinline__ void store_vec_f32(typename Elem<DT>::store_t* p, uin
 #pragma unroll
     for (int b = 0; b < N; b += VE) {
       VecU<DT> x;
-#pragma unroll
-      for (int e = 0; e < VE; ++e) x.e[e] = Elem<DT>::store(f[b + e]);
-      *(u32x4_unaligned*)(p + b) = x.v;
+      if constexpr (VE == 4) x.v = (u32x4){f32_to_bits(f[b]), f32_to_bits(f[b + 1]), f32_to_bits(f[b + 2]), f32_to_bits(f[b + 3])};
+      else x.v = (u32x4){narrow_pair<DT>(f[b], f[b + 1]), narrow_pair<DT>(f[b + 2], f[b + 3]), narrow_pair<DT>(f[b + 4], f[b + 5]),
+                         narrow_pair<DT>(f[b + 6], f[b + 7])};
+      if constexpr (STREAM) __builtin_nontemporal_store(x.v, (u32x4_unaligned*)(p + b));
+      else *(u32x4_unaligned*)(p + b) = x.v;
     }
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if ((uint32_t)e < left) p[e] = Elem<DT>::store(f[e]);
+      if ((uint32_t)e < left) p[e] = narrow<DT>(f[e]);
   }
 }
 
@@ -64,38 +90,64 @@ struct EmbeddingArgs {
 };
 
 constexpr int kLookupVecs = 4;  // vectors per lane
+constexpr int kLookupWaves = 4;
 
 // The output is one run of n * vecs_per_row vectors, of which a wavefront takes 64 * kLookupVecs in a row
-// whatever the row length; every lane looks up the row of each of its vectors.
-template <int DT, typename ID>
-__global__ __launch_bounds__(256) void embedding_kernel(const EmbeddingArgs a) {
+// whatever the row length; every lane looks up the row of each of its vectors.  All ids are loaded before
+// the first row, all rows before the first store, and nothing in between depends on a branch: a vector
+// behind the list reads the last one, an id outside the table reads row 0, and the last vector of a row
+// that is no whole number of them begins early enough to be whole (its first elements are written twice,
+// with the same values).  Rows shorter than a vector, and a table without rows, take the SHORT form.
+template <int DT, typename ID, bool SHORT>
+__global__ __launch_bounds__(kLookupWaves * kWave) void embedding_kernel(const EmbeddingArgs a) {
   using S = typename Elem<DT>::store_t;
   constexpr int VE = vec_elems<DT>();
   const S* table = (const S*)a.table;
   S* out = (S*)a.out;
   const ID* ids = (const ID*)a.ids;
-  const uint32_t v0 = (blockIdx.x * 4 + threadIdx.x / kWave) * (uint32_t)(kWave * kLookupVecs) + threadIdx.x % kWave;
-  float f[kLookupVecs][VE];
+  const uint32_t v0 = (blockIdx.x * kLookupWaves + threadIdx.x / kWave) * (uint32_t)(kWave * kLookupVecs) + threadIdx.x % kWave;
+  uint32_t i[kLookupVecs], c[kLookupVecs];
+  uint64_t r[kLookupVecs];
 #pragma unroll
   for (int u = 0; u < kLookupVecs; ++u) {
-    const uint32_t v = v0 + (uint32_t)u * kWave;
+    const uint32_t v = v0 + (uint32_t)u * kWave < a.vecs ? v0 + (uint32_t)u * kWave : a.vecs - 1;
+    i[u] = v / a.vecs_per_row;
+    c[u] = (v - i[u] * a.vecs_per_row) * VE;
+    if (!SHORT && c[u] + VE > a.hidden) c[u] = a.hidden - VE;
+    r[u] = (uint64_t)(int64_t)ids[i[u]];
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  bool inside[kLookupVecs];
 #pragma unroll
-    for (int e = 0; e < VE; ++e) f[u][e] = 0.0f;
-    if (v >= a.vecs) continue;
-    const uint32_t i = v / a.vecs_per_row;
-    const uint32_t c = (v - i * a.vecs_per_row) * VE;
-    const uint64_t r = (uint64_t)(int64_t)ids[i] - (uint64_t)a.first_row;  // wraps: below the table is far above it
-    if (r < a.rows) load_vec_f32<DT>(table + r * a.hidden + c, a.hidden - c, f[u]);
+  for (int u = 0; u < kLookupVecs; ++u) {
+    r[u] -= (uint64_t)a.first_row;  // wraps: below the table is far above it
+    inside[u] = r[u] < a.rows;
+    if (!inside[u]) r[u] = 0;
+  }
+  float f[kLookupVecs][VE];
+  if constexpr (SHORT) {
+#pragma unroll
+    for (int u = 0; u < kLookupVecs; ++u) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) f[u][e] = 0.0f;
+      if (inside[u]) load_vec_f32<DT>(table + r[u] * a.hidden + c[u], a.hidden - c[u], f[u]);
+    }
+  } else {
+    VecU<DT> x[kLookupVecs];
+#pragma unroll
+    for (int u = 0; u < kLookupVecs; ++u) x[u].v = *(const u32x4_unaligned*)(table + r[u] * a.hidden + c[u]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < kLookupVecs; ++u)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) f[u][e] = Elem<DT>::load(x[u].e[e]);
   }
 #pragma unroll
   for (int u = 0; u < kLookupVecs; ++u) {
-    const uint32_t v = v0 + (uint32_t)u * kWave;
-    if (v >= a.vecs) break;
-    const uint32_t i = v / a.vecs_per_row;
-    const uint32_t c = (v - i * a.vecs_per_row) * VE;
+    if (v0 + (uint32_t)u * kWave >= a.vecs) break;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) f[u][e] = a.scale * f[u][e];
-    store_vec_f32<DT>(out + (size_t)i * a.hidden + c, a.hidden - c, f[u]);
+    for (int e = 0; e < VE; ++e) f[u][e] = inside[u] ? a.scale * f[u][e] : 0.0f;
+    store_vec_f32<DT, true>(out + (size_t)i[u] * a.hidden + c[u], a.hidden - c[u], f[u]);
   }
 }
 
@@ -288,26 +340,28 @@ __global__ __launch_bounds__(kSortBlock) void sort_offsets_kernel(const uint32_t
 // ------------------------------------------------------------------------------------------
 // gradient: d_table[v] = scale * sum of grad[order[j]], offsets[v] <= j < offsets[v + 1]
 // ------------------------------------------------------------------------------------------
-// A row with at most kGradPiece tokens is summed by one wavefront per column chunk, in ascending
-// order.  A longer one (padding, a frequent word) is cut where the sorted tokens are cut into pieces of
-// kGradPiece: every piece is summed on its own into the workspace and a second launch adds the pieces
-// in ascending order.  A piece touches at most two such rows, the one it begins in (slot 0) and the
-// one that begins inside it (slot 1), and at most one of them can begin in it.
-constexpr int kGradPiece = 64;
+// A row with at most kGradPiece tokens is summed by the wavefronts of its columns, in ascending order.  A
+// longer one (padding, a frequent word) is cut where the sorted tokens are cut into pieces of kGradPiece:
+// every piece is summed on its own into the workspace and a second launch adds the pieces in ascending
+// order.  A piece touches at most two such rows, the one it begins in (slot 0) and the one that begins
+// inside it (slot 1), and at most one of them can begin in it.
+constexpr int kGradPiece = kWave;  // a lane holds the index of each
 constexpr int kGradWaves = 4;
-constexpr int kGradLoads = 4;  // rows in flight per lane
+constexpr int kGradLoads = 8;      // gradient rows in flight
+constexpr uint32_t kNoRow = ~0u;
 
 struct EmbeddingGradArgs {
   const char* grad;
   const int64_t* order;
   const int64_t* offsets;
   char* out;
-  float* partial;       // [pieces][2][hidden]
+  float* partial;        // [pieces][2][hidden]
+  uint32_t* long_row;    // [pieces]: the long row that begins in the piece, kNoRow if none does
   uint32_t rows;
   uint32_t n;
   uint32_t piece_groups; // workgroups that take pieces: the first ones; 0 where no row can be longer than a piece
   uint32_t hidden;
-  uint32_t chunk_waves_log2;  // 1, 2 or 4 wavefronts share a row (a piece), each a chunk of 64 vectors at a time
+  uint32_t sharing_log2; // 1, 2 or 4 wavefronts share a row (a piece)
   float scale;
   int accumulate;
 };
@@ -320,51 +374,119 @@ __device__ __forceinline__ uint32_t offset_at(const EmbeddingGradArgs& a, uint32
   return high || low > a.n ? a.n : low;
 }
 
-// Sum of grad[order[j]] over j0 <= j < j1 in ascending j, one vector of columns per lane.
-template <int DT>
-__device__ __forceinline__ void sum_rows(const EmbeddingGradArgs& a, uint32_t j0, uint32_t j1, uint32_t col, float (&acc)[vec_elems<DT>()]) {
-  constexpr int VE = vec_elems<DT>();
-  const typename Elem<DT>::store_t* grad = (const typename Elem<DT>::store_t*)a.grad;
+// The columns of a lane: VL vectors, 64 vectors apart.  A vector that would end behind the row is read from
+// further ahead, and `skip` of its elements belong to the lane before; `own` is how many are its own.
+template <int DT, int VL, bool SHORT>
+struct GradColumns {
+  static constexpr int VE = vec_elems<DT>();
+  uint32_t col[VL], skip[VL], own[VL];
+  __device__ __forceinline__ GradColumns(uint32_t first, uint32_t hidden) {
 #pragma unroll
-  for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
-  for (uint32_t j = j0; j < j1; j += kGradLoads) {
-    float f[kGradLoads][VE];
-#pragma unroll
-    for (int u = 0; u < kGradLoads; ++u) {
-#pragma unroll
-      for (int e = 0; e < VE; ++e) f[u][e] = 0.0f;
-      if (j + u < j1 && col < a.hidden) {
-        const uint64_t i = (uint64_t)a.order[j + u];
-        if (i < a.n) load_vec_f32<DT>(grad + i * a.hidden + col, a.hidden - col, f[u]);
+    for (int x = 0; x < VL; ++x) {
+      const uint32_t c = first + x * kWave * VE;
+      own[x] = c < hidden ? (hidden - c < VE ? hidden - c : VE) : 0;
+      col[x] = c;
+      skip[x] = 0;
+      if (!SHORT && own[x] < VE) {
+        col[x] = hidden - VE;
+        skip[x] = own[x] ? VE - own[x] : 0;
       }
     }
+  }
+};
+
+// Sums of the gradient rows that lanes [l0, l1) hold the indices of, in ascending order.
+template <int DT, int VL, bool SHORT>
+__device__ __forceinline__ void sum_rows(const EmbeddingGradArgs& a, int index, uint32_t l0, uint32_t l1,
+                                         const GradColumns<DT, VL, SHORT>& c, float (&acc)[VL][vec_elems<DT>()]) {
+  constexpr int VE = vec_elems<DT>();
+  using S = typename Elem<DT>::store_t;
+  const S* grad = (const S*)a.grad;
 #pragma unroll
-    for (int u = 0; u < kGradLoads; ++u)
+  for (int x = 0; x < VL; ++x)
 #pragma unroll
-      for (int e = 0; e < VE; ++e) acc[e] += f[u][e];
+    for (int e = 0; e < VE; ++e) acc[x][e] = 0.0f;
+  uint32_t l = l0;
+  if constexpr (!SHORT) {
+    constexpr int G = kGradLoads / VL;
+    const bool whole = __ballot(threadIdx.x % kWave >= l0 && threadIdx.x % kWave < l1 && index < 0) == 0;
+    for (; whole && l + G <= l1; l += G) {
+      VecU<DT> v[G][VL];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const S* row = grad + (size_t)(uint32_t)__builtin_amdgcn_readlane(index, l + g) * a.hidden;
+#pragma unroll
+        for (int x = 0; x < VL; ++x) v[g][x].v = __builtin_nontemporal_load((const u32x4_unaligned*)(row + c.col[x]));
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int x = 0; x < VL; ++x)
+#pragma unroll
+          for (int e = 0; e < VE; ++e) acc[x][e] += Elem<DT>::load(v[g][x].e[e]);
+    }
+  }
+  for (; l < l1; ++l) {
+    const int i = __builtin_amdgcn_readlane(index, l);
+    if (i < 0) continue;
+    const S* row = grad + (size_t)(uint32_t)i * a.hidden;
+#pragma unroll
+    for (int x = 0; x < VL; ++x) {
+      float f[VE];
+      if constexpr (SHORT) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) f[e] = 0.0f;
+        if (c.own[x]) load_vec_f32<DT>(row + c.col[x], c.own[x], f);
+      } else {
+        load_vec_f32<DT>(row + c.col[x], VE, f);
+      }
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[x][e] += f[e];
+    }
   }
 }
 
-template <int DT, int OUT>
-__device__ __forceinline__ void write_row(const EmbeddingGradArgs& a, uint32_t v, uint32_t col, const float (&acc)[vec_elems<DT>()]) {
-  constexpr int VE = vec_elems<DT>();
-  if (col >= a.hidden) return;
-  typename Elem<OUT>::store_t* out = (typename Elem<OUT>::store_t*)a.out + (size_t)v * a.hidden + col;
-  float r[VE];
+// Stores (or adds) a lane's columns of a row of the result, scaled and rounded once.
+template <int DT, int OUT, int VL, bool SHORT>
+__device__ __forceinline__ void write_row(const EmbeddingGradArgs& a, uint32_t v, const GradColumns<DT, VL, SHORT>& c,
+                                          const float (&acc)[VL][vec_elems<DT>()]) {
+  constexpr int VE = vec_elems<DT>(), OE = vec_elems<OUT>();
+  typename Elem<OUT>::store_t* row = (typename Elem<OUT>::store_t*)a.out + (size_t)v * a.hidden;
 #pragma unroll
-  for (int e = 0; e < VE; ++e) r[e] = a.scale * acc[e];
-  if (a.accumulate) {
-    constexpr int OE = vec_elems<OUT>();
+  for (int x = 0; x < VL; ++x) {
+    float r[VE];
 #pragma unroll
-    for (int b = 0; b < VE; b += OE) {
-      if (col + b >= a.hidden) break;
-      float old[OE];
-      load_vec_f32<OUT>(out + b, a.hidden - col - b, old);
+    for (int e = 0; e < VE; ++e) r[e] = a.scale * acc[x][e];
+    if (c.own[x] == VE) {
+      if (a.accumulate) {
 #pragma unroll
-      for (int e = 0; e < OE; ++e) r[b + e] = old[e] + r[b + e];
+        for (int b = 0; b < VE; b += OE) {
+          float old[OE];
+          load_vec_f32<OUT>(row + c.col[x] + b, OE, old);
+#pragma unroll
+          for (int e = 0; e < OE; ++e) r[b + e] = old[e] + r[b + e];
+        }
+      }
+      store_vec_f32<OUT, true>(row + c.col[x], VE, r);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if ((uint32_t)e >= c.skip[x] && (uint32_t)e < c.skip[x] + c.own[x]) {
+          auto* p = row + c.col[x] + e;
+          *p = narrow<OUT>(a.accumulate ? Elem<OUT>::load(*p) + r[e] : r[e]);
+        }
     }
   }
-  store_vec_f32<OUT>(out, a.hidden - col, r);
+}
+
+template <int DT, int VL, bool SHORT>
+__device__ __forceinline__ void write_partial(float* row, const GradColumns<DT, VL, SHORT>& c, const float (&acc)[VL][vec_elems<DT>()]) {
+  constexpr int VE = vec_elems<DT>();
+#pragma unroll
+  for (int x = 0; x < VL; ++x) {
+    if (!SHORT && c.own[x]) store_vec_f32<MCCL_F32>(row + c.col[x], VE, acc[x]);  // elements of two lanes are the same in both
+    if (SHORT) store_vec_f32<MCCL_F32>(row + c.col[x], c.own[x], acc[x]);
+  }
 }
 
 // The row that holds sorted position j: the largest v with offsets[v] <= j, by a search in which the
@@ -382,85 +504,120 @@ __device__ __forceinline__ uint32_t row_of_position(const EmbeddingGradArgs& a, 
   return lo;
 }
 
-template <int DT, int OUT>
+// The token at sorted position j, or -1 where there is none.
+__device__ __forceinline__ int token_at(const EmbeddingGradArgs& a, uint32_t j, uint32_t end) {
+  if (j >= end) return -1;
+  const uint64_t i = (uint64_t)a.order[j];
+  return i < a.n ? (int)(uint32_t)i : -1;
+}
+
+template <int DT, int OUT, int VL, bool SHORT>
 __global__ __launch_bounds__(kGradWaves * kWave) void embedding_grad_kernel(const EmbeddingGradArgs a) {
   constexpr int VE = vec_elems<DT>();
-  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const uint32_t sharing = 1u << a.chunk_waves_log2;
-  const uint32_t col0 = ((wave & (sharing - 1)) * kWave + lane) * VE, stride = sharing * kWave * VE;
-  const uint32_t per_group_log2 = 2 - a.chunk_waves_log2;
-  float acc[VE];
+  const uint32_t lane = threadIdx.x % kWave, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  const uint32_t sharing = 1u << a.sharing_log2, per_group_log2 = 2 - a.sharing_log2;
+  const uint32_t member = wave >> a.sharing_log2;
+  const uint32_t first_col = (wave & (sharing - 1)) * (kWave * VL * VE), stride = sharing * kWave * VL * VE;
+  float acc[VL][VE];
   if (blockIdx.x >= a.piece_groups) {
     const uint32_t step = (gridDim.x - a.piece_groups) << per_group_log2;
-    for (uint32_t v = ((blockIdx.x - a.piece_groups) << per_group_log2) + (wave >> a.chunk_waves_log2); v < a.rows; v += step) {
+    for (uint32_t v = ((blockIdx.x - a.piece_groups) << per_group_log2) + member; v < a.rows; v += step) {
       const uint32_t j0 = offset_at(a, v), j1 = offset_at(a, v + 1);
-      if ((j1 > j0 && j1 - j0 > kGradPiece) || (a.accumulate && j1 <= j0)) continue;
-      for (uint32_t col = col0; col - lane * VE < a.hidden; col += stride) {
-        sum_rows<DT>(a, j0, j1, col, acc);
-        write_row<DT, OUT>(a, v, col, acc);
+      const uint32_t count = j1 > j0 ? j1 - j0 : 0;
+      if (count > kGradPiece || (a.accumulate && count == 0)) continue;
+      const int index = token_at(a, j0 + lane, j1);
+      for (uint32_t col = first_col; col < a.hidden; col += stride) {
+        const GradColumns<DT, VL, SHORT> c(col + lane * VE, a.hidden);
+        sum_rows<DT, VL, SHORT>(a, index, 0, count, c, acc);
+        write_row<DT, OUT, VL, SHORT>(a, v, c, acc);
       }
     }
   } else {
-    const uint32_t piece = (blockIdx.x << per_group_log2) + (wave >> a.chunk_waves_log2);
+    const uint32_t piece = (blockIdx.x << per_group_log2) + member;
     const uint32_t in_table = offset_at(a, a.rows);
-    if (piece >= (in_table + kGradPiece - 1) / kGradPiece) return;
     const uint32_t p0 = piece * kGradPiece;
-    const uint32_t p1 = p0 + kGradPiece < in_table ? p0 + kGradPiece : in_table;
-    const uint32_t first = row_of_position(a, p0);
-    const uint32_t last = row_of_position(a, p1 - 1);
-    const uint32_t first_end = offset_at(a, first + 1), last_begin = offset_at(a, last);
-    const bool first_long = first_end - offset_at(a, first) > kGradPiece;
-    const bool last_long = last != first && offset_at(a, last + 1) - last_begin > kGradPiece;
-    for (uint32_t col = col0; col - lane * VE < a.hidden; col += stride) {
-      float* slot = a.partial + (size_t)piece * 2 * a.hidden + col;
-      if (first_long) {
-        sum_rows<DT>(a, p0, first_end < p1 ? first_end : p1, col, acc);
-        if (col < a.hidden) store_vec_f32<MCCL_F32>(slot, a.hidden - col, acc);
-      }
-      if (last_long) {
-        sum_rows<DT>(a, last_begin, p1, col, acc);
-        if (col < a.hidden) store_vec_f32<MCCL_F32>(slot + a.hidden, a.hidden - col, acc);
+    if (p0 >= a.n) return;
+    uint32_t begins = kNoRow;
+    if (p0 < in_table) {
+      const uint32_t p1 = p0 + kGradPiece < in_table ? p0 + kGradPiece : in_table;
+      const int index = token_at(a, p0 + lane, p1);
+      const uint32_t first = row_of_position(a, p0), last = row_of_position(a, p1 - 1);
+      const uint32_t first_begin = offset_at(a, first), first_end = offset_at(a, first + 1), last_begin = offset_at(a, last);
+      const bool first_long = first_end - first_begin > kGradPiece;
+      const bool last_long = last != first && offset_at(a, last + 1) - last_begin > kGradPiece;
+      if (last_long) begins = last;
+      else if (first_long && first_begin == p0) begins = first;
+      for (uint32_t col = first_col; col < a.hidden; col += stride) {
+        const GradColumns<DT, VL, SHORT> c(col + lane * VE, a.hidden);
+        float* slot = a.partial + (size_t)piece * 2 * a.hidden;
+        if (first_long) {
+          sum_rows<DT, VL, SHORT>(a, index, 0, (first_end < p1 ? first_end : p1) - p0, c, acc);
+          write_partial<DT, VL, SHORT>(slot, c, acc);
+        }
+        if (last_long) {
+          sum_rows<DT, VL, SHORT>(a, index, last_begin - p0, p1 - p0, c, acc);
+          write_partial<DT, VL, SHORT>(slot + a.hidden, c, acc);
+        }
       }
     }
+    if (lane == 0 && first_col == 0) a.long_row[piece] = begins;
   }
 }
 
 // Adds the pieces of the long row that begins in a workgroup's piece, a chunk of columns per workgroup:
-// kJoinWaves wavefronts take every kJoinWaves-th piece each, and their sums are added in the order of the
-// wavefronts.
+// kJoinWaves wavefronts take every kJoinWaves-th piece each, kJoinLoads of them at a time, and their sums
+// are added in the order of the wavefronts.
 constexpr int kJoinWaves = 8;
+constexpr int kJoinLoads = 4;
 
-template <int DT, int OUT>
+template <int DT, int OUT, bool SHORT>
 __global__ __launch_bounds__(kJoinWaves * kWave) void embedding_grad_join_kernel(const EmbeddingGradArgs a) {
   constexpr int VE = vec_elems<DT>();
-  __shared__ float sum[kJoinWaves][kWave * VE];
-  const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const uint32_t in_table = offset_at(a, a.rows);
-  const uint32_t piece = blockIdx.x, col = (blockIdx.y * kWave + lane) * VE;
-  if (piece >= (in_table + kGradPiece - 1) / kGradPiece) return;
-  const uint32_t p0 = piece * kGradPiece;
-  const uint32_t p1 = p0 + kGradPiece < in_table ? p0 + kGradPiece : in_table;
-  const uint32_t v = row_of_position(a, p1 - 1);  // of the rows of a piece only the last can begin in it and be long
-  const uint32_t j0 = offset_at(a, v), j1 = offset_at(a, v + 1);
-  if (j1 <= j0 || j1 - j0 <= kGradPiece || j0 < p0) return;
-  const uint32_t last = (j1 - 1) / kGradPiece;
-  float acc[VE];
+  __shared__ float sum[kJoinWaves][VE * kWave];
+  const uint32_t lane = threadIdx.x % kWave, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  const uint32_t piece = blockIdx.x;
+  const uint32_t v = a.long_row[piece];
+  if (v == kNoRow) return;
+  const uint32_t j0 = offset_at(a, v), j1 = offset_at(a, v + 1), last = (j1 - 1) / kGradPiece;
+  const GradColumns<DT, 1, SHORT> c((blockIdx.y * kWave + lane) * VE, a.hidden);
+  float acc[1][VE];
 #pragma unroll
-  for (int e = 0; e < VE; ++e) acc[e] = 0.0f;
-  for (uint32_t p = piece + wave; p <= last; p += kJoinWaves) {
-    const float* from = a.partial + ((size_t)p * 2 + (p == piece && j0 != p0 ? 1 : 0)) * a.hidden + col;
+  for (int e = 0; e < VE; ++e) acc[0][e] = 0.0f;
+  const auto slot = [&](uint32_t p) { return a.partial + ((size_t)p * 2 + (p == piece && j0 != p * kGradPiece ? 1 : 0)) * a.hidden + c.col[0]; };
+  const auto add = [&](auto count, uint32_t p) {
+    float f[count][VE];
 #pragma unroll
-    for (int e = 0; e < VE; ++e)
-      if (col + e < a.hidden) acc[e] += from[e];
-  }
+    for (int g = 0; g < count; ++g) {
+      const float* from = slot(p + g * kJoinWaves);
 #pragma unroll
-  for (int e = 0; e < VE; ++e) sum[wave][e * kWave + lane] = acc[e];
+      for (int b = 0; b < VE; b += 4) {
+        if constexpr (SHORT) {
+#pragma unroll
+          for (int e = b; e < b + 4; ++e) f[g][e] = (uint32_t)e < c.own[0] ? from[e] : 0.0f;
+        } else {
+          float four[4];
+          load_vec_f32<MCCL_F32>(from + b, 4, four);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[g][b + e] = four[e];
+        }
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < count; ++g)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[0][e] += f[g][e];
+  };
+  uint32_t p = piece + wave;
+  for (; p + (kJoinLoads - 1) * kJoinWaves <= last; p += kJoinLoads * kJoinWaves) add(std::integral_constant<int, kJoinLoads>{}, p);
+  for (; p <= last; p += kJoinWaves) add(std::integral_constant<int, 1>{}, p);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) sum[wave][e * kWave + lane] = acc[0][e];
   __syncthreads();
   if (wave == 0) {
     for (int w = 1; w < kJoinWaves; ++w)
 #pragma unroll
-      for (int e = 0; e < VE; ++e) acc[e] += sum[w][e * kWave + lane];
-    write_row<DT, OUT>(a, v, col, acc);
+      for (int e = 0; e < VE; ++e) acc[0][e] += sum[w][e * kWave + lane];
+    write_row<DT, OUT, 1, SHORT>(a, v, c, acc);
   }
 }
 

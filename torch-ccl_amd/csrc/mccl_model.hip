@@ -103,23 +103,31 @@ int launch_sort(const ID* ids, size_t n, int64_t first_row, size_t rows, char* w
 
 template <int DT>
 void launch_embedding(const EmbeddingArgs& a, int id_dtype, hipStream_t s) {
-  const dim3 grid((unsigned)((a.vecs + 4ull * kWave * kLookupVecs - 1) / (4 * kWave * kLookupVecs))), block(256);
-  if (id_dtype == MCCL_I32) hipLaunchKernelGGL((embedding_kernel<DT, int32_t>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((embedding_kernel<DT, int64_t>), grid, block, 0, s, a);
+  const unsigned per_group = kLookupWaves * kWave * kLookupVecs;
+  const dim3 grid((a.vecs + per_group - 1) / per_group), block(kLookupWaves * kWave);
+  const bool narrow = a.hidden < (uint32_t)vec_elems<DT>() || a.rows == 0;
+  auto kernel = id_dtype == MCCL_I32 ? (narrow ? embedding_kernel<DT, int32_t, true> : embedding_kernel<DT, int32_t, false>)
+                                     : (narrow ? embedding_kernel<DT, int64_t, true> : embedding_kernel<DT, int64_t, false>);
+  hipLaunchKernelGGL(kernel, grid, block, 0, s, a);
 }
 
 size_t grad_pieces(size_t n) { return n > (size_t)kGradPiece ? (n + kGradPiece - 1) / kGradPiece : 0; }
 
 template <int DT, int OUT>
 void launch_embedding_grad(EmbeddingGradArgs a, hipStream_t s) {
-  const uint32_t chunks = (uint32_t)(((uint64_t)a.hidden + kWave * vec_elems<DT>() - 1) / (kWave * vec_elems<DT>()));
-  a.chunk_waves_log2 = chunks >= 4 ? 2 : chunks >= 2 ? 1 : 0;
-  const uint32_t per_group = kGradWaves >> a.chunk_waves_log2;
+  constexpr uint32_t kChunk = kWave * vec_elems<DT>();
+  const bool narrow = a.hidden < (uint32_t)vec_elems<DT>();
+  const uint32_t chunks = (a.hidden + kChunk - 1) / kChunk;
+  const uint32_t units = chunks > 4 ? (chunks + 1) / 2 : chunks;  // of one wavefront: two chunks where there are many
+  a.sharing_log2 = units >= 4 ? 2 : units >= 2 ? 1 : 0;
+  const uint32_t per_group = kGradWaves >> a.sharing_log2;
   const uint32_t pieces = (uint32_t)grad_pieces(a.n);
   a.piece_groups = (pieces + per_group - 1) / per_group;
   const uint32_t row_groups = std::min(kMaxGroups, (a.rows + per_group - 1) / per_group);
-  hipLaunchKernelGGL((embedding_grad_kernel<DT, OUT>), dim3(a.piece_groups + row_groups), dim3(kGradWaves * kWave), 0, s, a);
-  if (pieces) hipLaunchKernelGGL((embedding_grad_join_kernel<DT, OUT>), dim3(pieces, chunks), dim3(kJoinWaves * kWave), 0, s, a);
+  auto kernel = narrow ? embedding_grad_kernel<DT, OUT, 1, true> : chunks > 4 ? embedding_grad_kernel<DT, OUT, 2, false> : embedding_grad_kernel<DT, OUT, 1, false>;
+  hipLaunchKernelGGL(kernel, dim3(a.piece_groups + row_groups), dim3(kGradWaves * kWave), 0, s, a);
+  auto join = narrow ? embedding_grad_join_kernel<DT, OUT, true> : embedding_grad_join_kernel<DT, OUT, false>;
+  if (pieces) hipLaunchKernelGGL(join, dim3(pieces, chunks), dim3(kJoinWaves * kWave), 0, s, a);
 }
 
 template <int DT, bool GRAD>
@@ -272,7 +280,7 @@ int mccl_sort_ids(const void* ids, int id_dtype, size_t n, int64_t first_row, si
   return launch_sort((const int64_t*)ids, n, first_row, rows, (char*)workspace, order, offsets, s);
 }
 
-size_t mccl_embedding_grad_workspace(size_t n, size_t hidden) { return grad_pieces(n) * 2 * hidden * sizeof(float); }
+size_t mccl_embedding_grad_workspace(size_t n, size_t hidden) { return grad_pieces(n) * (2 * hidden * sizeof(float) + sizeof(uint32_t)); }
 
 int mccl_embedding_grad(const void* grad, const int64_t* order, const int64_t* offsets, size_t n, size_t rows, size_t hidden,
                         float scale, int dtype, void* out, int out_dtype, int accumulate, void* workspace, size_t workspace_bytes,
@@ -302,6 +310,7 @@ int mccl_embedding_grad(const void* grad, const int64_t* order, const int64_t* o
   a.offsets = offsets;
   a.out = (char*)out;
   a.partial = (float*)workspace;
+  a.long_row = (uint32_t*)(a.partial + grad_pieces(n) * 2 * hidden);
   a.rows = (uint32_t)rows;
   a.n = (uint32_t)n;
   a.hidden = (uint32_t)hidden;
