@@ -189,22 +189,28 @@ __global__ __launch_bounds__(kSortBlock) void sort_small_kernel(const ID* ids, u
   }
 }
 
-// More tokens: least-significant-digit radix sort, kSortDigits values a digit, three launches a pass.
+// More tokens: least-significant-digit radix sort, kSortDigits values a digit, two launches a pass: the digits
+// of every tile are counted, then every workgroup adds up the counts of the tiles before its own and of the
+// smaller digits, ranks its keys and writes them where they belong.  Over kSortTilesAdded tiles a third
+// launch in between does the adding up (at 64 tiles a workgroup reads 64 KiB of counts for it, which takes
+// about as long as a launch).  These launches move a few bytes a key: they are bound by their round trips.
 constexpr int kSortBits = 8;
 constexpr int kSortDigits = 1 << kSortBits;
-constexpr int kSortSteps = 8;                                 // keys per lane
-constexpr int kSortWaves = kSortBlock / kWave;
-constexpr int kSortTile = kSortBlock * kSortSteps;            // keys per workgroup
+constexpr int kSortWaves = 8;
+constexpr int kSortThreads = kSortWaves * kWave;
+constexpr int kSortSteps = 4;                                 // keys per lane
+constexpr int kSortTile = kSortThreads * kSortSteps;          // keys per workgroup
+constexpr uint32_t kSortTilesAdded = 64;
 
 struct SortArgs {
   const void* ids;         // first pass: the keys come from here
   const uint32_t* key_in;  // later passes
   const uint32_t* pos_in;
-  uint32_t* key_out;       // null in the last pass but for the sorted keys the offsets are found in
+  uint32_t* key_out;
   uint32_t* pos_out;
   int64_t* order;          // last pass
-  uint32_t* counts;        // [kSortDigits][tiles]; after the scan: keys of the digit in earlier tiles
-  uint32_t* totals;        // [kSortDigits]: keys of the digit in all tiles
+  uint32_t* counts;        // [tiles][kSortDigits]; once added up: keys of the digit in earlier tiles
+  uint32_t* totals;        // [kSortDigits]: keys of the digit in all tiles, where they are added up by a launch
   uint32_t n;
   uint32_t tiles;
   int64_t first_row;
@@ -219,69 +225,93 @@ __device__ __forceinline__ uint32_t sort_key(const SortArgs& a, uint32_t i) {
 }
 
 template <typename ID, bool FIRST>
-__global__ __launch_bounds__(kSortBlock) void sort_count_kernel(const SortArgs a) {
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const SortArgs a) {
   __shared__ uint32_t hist[kSortDigits];
-  for (int d = threadIdx.x; d < kSortDigits; d += kSortBlock) hist[d] = 0;
-  __syncthreads();
-  const uint32_t base = blockIdx.x * (uint32_t)kSortTile;
+  const uint32_t base = blockIdx.x * (uint32_t)kSortTile + threadIdx.x;
+  uint32_t key[kSortSteps];
 #pragma unroll
   for (int s = 0; s < kSortSteps; ++s) {
-    const uint32_t i = base + (uint32_t)s * kSortBlock + threadIdx.x;
-    if (i < a.n) atomicAdd(&hist[(sort_key<ID, FIRST>(a, i) >> a.shift) & (kSortDigits - 1)], 1u);
+    const uint32_t i = base + (uint32_t)s * kSortThreads;
+    key[s] = i < a.n ? sort_key<ID, FIRST>(a, i) : 0;
   }
+  if (threadIdx.x < kSortDigits) hist[threadIdx.x] = 0;
   __syncthreads();
-  for (int d = threadIdx.x; d < kSortDigits; d += kSortBlock) a.counts[(size_t)d * a.tiles + blockIdx.x] = hist[d];
+#pragma unroll
+  for (int s = 0; s < kSortSteps; ++s)
+    if (base + (uint32_t)s * kSortThreads < a.n) atomicAdd(&hist[(key[s] >> a.shift) & (kSortDigits - 1)], 1u);
+  __syncthreads();
+  if (threadIdx.x < kSortDigits) a.counts[(size_t)blockIdx.x * kSortDigits + threadIdx.x] = hist[threadIdx.x];
 }
 
-// One workgroup per digit: exclusive scan of its counts over the tiles, and their total.
-__global__ __launch_bounds__(kSortBlock) void sort_scan_kernel(uint32_t* counts, uint32_t tiles, uint32_t* totals) {
-  __shared__ uint32_t part[kSortBlock];
-  uint32_t* row = counts + (size_t)blockIdx.x * tiles;
-  uint32_t carry = 0;
-  for (uint32_t t0 = 0; t0 < tiles; t0 += kSortBlock) {
-    const uint32_t t = t0 + threadIdx.x;
-    const uint32_t mine = t < tiles ? row[t] : 0;
-    part[threadIdx.x] = mine;
-    __syncthreads();
-    for (int d = 1; d < kSortBlock; d <<= 1) {
-      const uint32_t add = (int)threadIdx.x >= d ? part[threadIdx.x - d] : 0;
-      __syncthreads();
-      part[threadIdx.x] += add;
-      __syncthreads();
-    }
-    if (t < tiles) row[t] = carry + part[threadIdx.x] - mine;
-    carry += part[kSortBlock - 1];
-    __syncthreads();
+// Adds up the counts over the tiles, kAddDigits digits a workgroup, kAddParts parts of the tiles side by side.
+constexpr uint32_t kAddDigits = 16, kAddParts = 64;
+
+__global__ __launch_bounds__(kAddDigits * kAddParts) void sort_add_kernel(uint32_t* counts, uint32_t tiles, uint32_t* totals) {
+  __shared__ uint32_t sum[kAddParts][kAddDigits];
+  const uint32_t digit = threadIdx.x % kAddDigits, part = threadIdx.x / kAddDigits;
+  const uint32_t per = (tiles + kAddParts - 1) / kAddParts;
+  const uint32_t t0 = part * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+  uint32_t* column = counts + blockIdx.x * kAddDigits + digit;
+  uint32_t mine = 0;
+  for (uint32_t t = t0; t < t1; ++t) mine += column[(size_t)t * kSortDigits];
+  sum[part][digit] = mine;
+  __syncthreads();
+  uint32_t before = 0, total = 0;
+  for (uint32_t p = 0; p < kAddParts; ++p) {
+    const uint32_t c = sum[p][digit];
+    total += c;
+    before += p < part ? c : 0;
   }
-  if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+  if (part == 0) totals[blockIdx.x * kAddDigits + digit] = total;
+  for (uint32_t t = t0; t < t1; ++t) {
+    const uint32_t c = column[(size_t)t * kSortDigits];
+    column[(size_t)t * kSortDigits] = before;
+    before += c;
+  }
 }
 
 // A wavefront holds kSortSteps x 64 consecutive keys.  Within one step of 64, a key's rank among the
 // equal digits is the number of lower lanes with the same digit, found by one ballot per bit; the
 // digit's count so far is kept per wavefront in LDS, so equal digits stay in their order.
-template <typename ID, bool FIRST, bool LAST>
-__global__ __launch_bounds__(kSortBlock) void sort_scatter_kernel(const SortArgs a) {
+template <typename ID, bool FIRST, bool LAST, bool ADDED>
+__global__ __launch_bounds__(kSortThreads) void sort_scatter_kernel(const SortArgs a) {
   __shared__ uint32_t seen[kSortWaves][kSortDigits];
-  __shared__ uint32_t start[kSortDigits];
+  __shared__ uint32_t below[kSortDigits / kWave];
   const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  for (int d = threadIdx.x; d < kSortWaves * kSortDigits; d += kSortBlock) (&seen[0][0])[d] = 0;
-  if (threadIdx.x < kSortDigits) start[threadIdx.x] = a.totals[threadIdx.x];
-  __syncthreads();
-  // keys of smaller digits: scan of the totals
-  for (int d = 1; d < kSortDigits; d <<= 1) {
-    const uint32_t add = (int)threadIdx.x >= d && threadIdx.x < kSortDigits ? start[threadIdx.x - d] : 0;
-    __syncthreads();
-    if (threadIdx.x < kSortDigits) start[threadIdx.x] += add;
-    __syncthreads();
-  }
   const uint32_t base = blockIdx.x * (uint32_t)kSortTile + wave * (uint32_t)(kSortSteps * kWave) + lane;
-  uint32_t key[kSortSteps], rank[kSortSteps];
+  uint32_t key[kSortSteps], pos[kSortSteps], rank[kSortSteps];
 #pragma unroll
   for (int s = 0; s < kSortSteps; ++s) {
     const uint32_t i = base + (uint32_t)s * kWave;
     key[s] = i < a.n ? sort_key<ID, FIRST>(a, i) : 0;
+    pos[s] = FIRST ? i : i < a.n ? a.pos_in[i] : 0;
     rank[s] = 0;
   }
+  // Where the digit of this thread begins: the keys of smaller digits, and its own in earlier tiles.
+  uint32_t before = 0, total = 0, smaller = 0;
+  if (threadIdx.x < kSortDigits) {
+    if constexpr (ADDED) {
+      before = a.counts[(size_t)blockIdx.x * kSortDigits + threadIdx.x];
+      total = a.totals[threadIdx.x];
+    } else {
+#pragma unroll 8
+      for (uint32_t t = 0; t < a.tiles; ++t) {
+        const uint32_t c = a.counts[(size_t)t * kSortDigits + threadIdx.x];
+        total += c;
+        before += t < blockIdx.x ? c : 0;
+      }
+    }
+    uint32_t scan = total;  // over the wavefront's 64 digits
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const uint32_t add = __shfl_up(scan, d);
+      scan += (int)lane >= d ? add : 0;
+    }
+    smaller = scan - total;
+    if (lane == kWave - 1) below[wave] = scan;
+  }
+  for (uint32_t d = threadIdx.x; d < kSortWaves * kSortDigits; d += kSortThreads) (&seen[0][0])[d] = 0;
+  __syncthreads();
 #pragma unroll
   for (int s = 0; s < kSortSteps; ++s) {
     const bool live = base + (uint32_t)s * kWave < a.n;
@@ -293,48 +323,61 @@ __global__ __launch_bounds__(kSortBlock) void sort_scatter_kernel(const SortArgs
       same &= ((digit >> b) & 1u) ? set : ~set;
     }
     if (live) {
-      const uint32_t before = __popcll(same & ((1ull << lane) - 1));
-      rank[s] = seen[wave][digit] + before;
+      const uint32_t lower = __popcll(same & ((1ull << lane) - 1));
+      rank[s] = seen[wave][digit] + lower;
       // every lane of the group has read the count (one wavefront, in step); its first lane advances it
-      if (before == 0) seen[wave][digit] += (uint32_t)__popcll(same);
+      if (lower == 0) seen[wave][digit] += (uint32_t)__popcll(same);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
   if (threadIdx.x < kSortDigits) {
-    const uint32_t d = threadIdx.x;
-    uint32_t at = start[d] - a.totals[d] + a.counts[(size_t)d * a.tiles + blockIdx.x];
+    uint32_t at = smaller + before;
+    for (uint32_t w = 0; w < wave; ++w) at += below[w];
 #pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
-      const uint32_t c = seen[w][d];
-      seen[w][d] = at;
+      const uint32_t c = seen[w][threadIdx.x];
+      seen[w][threadIdx.x] = at;
       at += c;
     }
   }
   __syncthreads();
 #pragma unroll
   for (int s = 0; s < kSortSteps; ++s) {
-    const uint32_t i = base + (uint32_t)s * kWave;
-    if (i >= a.n) continue;
+    if (base + (uint32_t)s * kWave >= a.n) continue;
     const uint32_t at = seen[wave][(key[s] >> a.shift) & (kSortDigits - 1)] + rank[s];
-    const uint32_t p = FIRST ? i : a.pos_in[i];
     a.key_out[at] = key[s];
-    if constexpr (LAST) a.order[at] = p;
-    else a.pos_out[at] = p;
+    if constexpr (LAST) a.order[at] = pos[s];
+    else a.pos_out[at] = pos[s];
   }
 }
 
-// offsets[v] = first position in the sorted keys whose key is not below v.
-__global__ __launch_bounds__(kSortBlock) void sort_offsets_kernel(const uint32_t* key, uint32_t n, uint32_t rows, int64_t* offsets) {
-  for (uint64_t v = (uint64_t)blockIdx.x * kSortBlock + threadIdx.x; v <= rows; v += (uint64_t)gridDim.x * kSortBlock) {
-    uint32_t lo = 0, hi = n;
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (key[mid] < (uint32_t)v) lo = mid + 1; else hi = mid;
-    }
-    offsets[v] = lo;
+// offsets[v] = first position in the sorted keys whose key is not below v.  Every `every`-th key (a power of
+// two, so that there are at most kSortSamples) goes into LDS and the search begins there: the round trips
+// to memory that are left are those within `every` keys.
+constexpr uint32_t kSortSamples = 1024;
+
+__global__ __launch_bounds__(kSortBlock) void sort_offsets_kernel(const uint32_t* key, uint32_t n, uint32_t every_log2, uint32_t rows,
+                                                                  int64_t* offsets) {
+  __shared__ uint32_t sample[kSortSamples];
+  const uint32_t samples = ((n - 1) >> every_log2) + 1;
+  for (uint32_t i = threadIdx.x; i < samples; i += kSortBlock) sample[i] = key[i << every_log2];
+  __syncthreads();
+  const uint64_t v = (uint64_t)blockIdx.x * kSortBlock + threadIdx.x;
+  if (v > rows) return;
+  uint32_t lo = 0, hi = samples;  // the first sample that is not below v
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (sample[mid] < (uint32_t)v) lo = mid + 1; else hi = mid;
   }
+  uint32_t end = lo < samples ? lo << every_log2 : n;
+  uint32_t begin = lo ? ((lo - 1) << every_log2) + 1 : 0;
+  while (begin < end) {
+    const uint32_t mid = begin + (end - begin) / 2;
+    if (key[mid] < (uint32_t)v) begin = mid + 1; else end = mid;
+  }
+  offsets[v] = begin;
 }
 
 // ------------------------------------------------------------------------------------------

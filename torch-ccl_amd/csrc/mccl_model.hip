@@ -81,7 +81,8 @@ int launch_sort(const ID* ids, size_t n, int64_t first_row, size_t rows, char* w
   a.first_row = first_row;
   a.rows = (uint32_t)rows;
   const int passes = sort_passes(rows);
-  const dim3 tiles((unsigned)p.tiles), block(kSortBlock);
+  const dim3 tiles((unsigned)p.tiles), threads(kSortThreads);
+  const bool added = p.tiles > kSortTilesAdded;
   for (int pass = 0; pass < passes; ++pass) {
     const bool first = pass == 0, last = pass == passes - 1;
     a.shift = pass * kSortBits;
@@ -89,15 +90,17 @@ int launch_sort(const ID* ids, size_t n, int64_t first_row, size_t rows, char* w
     a.pos_in = pos[(pass + 1) & 1];
     a.key_out = key[pass & 1];
     a.pos_out = pos[pass & 1];
-    if (first) hipLaunchKernelGGL((sort_count_kernel<ID, true>), tiles, block, 0, s, a);
-    else hipLaunchKernelGGL((sort_count_kernel<ID, false>), tiles, block, 0, s, a);
-    hipLaunchKernelGGL(sort_scan_kernel, dim3(kSortDigits), block, 0, s, a.counts, a.tiles, a.totals);
-    if (first && last) hipLaunchKernelGGL((sort_scatter_kernel<ID, true, true>), tiles, block, 0, s, a);
-    else if (first) hipLaunchKernelGGL((sort_scatter_kernel<ID, true, false>), tiles, block, 0, s, a);
-    else if (last) hipLaunchKernelGGL((sort_scatter_kernel<ID, false, true>), tiles, block, 0, s, a);
-    else hipLaunchKernelGGL((sort_scatter_kernel<ID, false, false>), tiles, block, 0, s, a);
+    hipLaunchKernelGGL((first ? sort_count_kernel<ID, true> : sort_count_kernel<ID, false>), tiles, threads, 0, s, a);
+    if (added) hipLaunchKernelGGL(sort_add_kernel, dim3(kSortDigits / kAddDigits), dim3(kAddDigits * kAddParts), 0, s, a.counts, a.tiles, a.totals);
+    auto scatter = added ? (first ? (last ? sort_scatter_kernel<ID, true, true, true> : sort_scatter_kernel<ID, true, false, true>)
+                                  : (last ? sort_scatter_kernel<ID, false, true, true> : sort_scatter_kernel<ID, false, false, true>))
+                         : (first ? (last ? sort_scatter_kernel<ID, true, true, false> : sort_scatter_kernel<ID, true, false, false>)
+                                  : (last ? sort_scatter_kernel<ID, false, true, false> : sort_scatter_kernel<ID, false, false, false>));
+    hipLaunchKernelGGL(scatter, tiles, threads, 0, s, a);
   }
-  hipLaunchKernelGGL(sort_offsets_kernel, dim3(offset_groups), block, 0, s, a.key_out, a.n, a.rows, offsets);
+  uint32_t every_log2 = 0;
+  while (((a.n - 1) >> every_log2) + 1 > kSortSamples) ++every_log2;
+  hipLaunchKernelGGL(sort_offsets_kernel, dim3(offset_groups), dim3(kSortBlock), 0, s, a.key_out, a.n, every_log2, a.rows, offsets);
   return launched("sort");
 }
 
