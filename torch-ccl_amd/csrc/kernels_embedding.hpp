@@ -489,9 +489,25 @@ __device__ __forceinline__ void sum_rows(const EmbeddingGradArgs& a, int index, 
   }
 }
 
+// What a lane's whole vectors of a row of the result hold, for the sums that are added to it: loaded before
+// the sums are made.
+template <int DT, int OUT, int VL, bool SHORT>
+__device__ __forceinline__ void read_row(const EmbeddingGradArgs& a, uint32_t v, const GradColumns<DT, VL, SHORT>& c,
+                                         VecU<OUT> (&old)[VL][vec_elems<DT>() / vec_elems<OUT>()]) {
+  constexpr int VE = vec_elems<DT>(), OE = vec_elems<OUT>();
+  if (!a.accumulate) return;
+  const typename Elem<OUT>::store_t* row = (const typename Elem<OUT>::store_t*)a.out + (size_t)v * a.hidden;
+#pragma unroll
+  for (int x = 0; x < VL; ++x)
+#pragma unroll
+    for (int b = 0; b < VE / OE; ++b)
+      if (c.own[x] == VE) old[x][b].v = __builtin_nontemporal_load((const u32x4_unaligned*)(row + c.col[x] + b * OE));
+}
+
 // Stores (or adds) a lane's columns of a row of the result, scaled and rounded once.
 template <int DT, int OUT, int VL, bool SHORT>
 __device__ __forceinline__ void write_row(const EmbeddingGradArgs& a, uint32_t v, const GradColumns<DT, VL, SHORT>& c,
+                                          const VecU<OUT> (&old)[VL][vec_elems<DT>() / vec_elems<OUT>()],
                                           const float (&acc)[VL][vec_elems<DT>()]) {
   constexpr int VE = vec_elems<DT>(), OE = vec_elems<OUT>();
   typename Elem<OUT>::store_t* row = (typename Elem<OUT>::store_t*)a.out + (size_t)v * a.hidden;
@@ -503,12 +519,7 @@ __device__ __forceinline__ void write_row(const EmbeddingGradArgs& a, uint32_t v
     if (c.own[x] == VE) {
       if (a.accumulate) {
 #pragma unroll
-        for (int b = 0; b < VE; b += OE) {
-          float old[OE];
-          load_vec_f32<OUT>(row + c.col[x] + b, OE, old);
-#pragma unroll
-          for (int e = 0; e < OE; ++e) r[b + e] = old[e] + r[b + e];
-        }
+        for (int e = 0; e < VE; ++e) r[e] = Elem<OUT>::load(old[x][e / OE].e[e % OE]) + r[e];
       }
       store_vec_f32<OUT, true>(row + c.col[x], VE, r);
     } else {
@@ -571,8 +582,10 @@ __global__ __launch_bounds__(kGradWaves * kWave) void embedding_grad_kernel(cons
       const int index = token_at(a, j0 + lane, j1);
       for (uint32_t col = first_col; col < a.hidden; col += stride) {
         const GradColumns<DT, VL, SHORT> c(col + lane * VE, a.hidden);
+        VecU<OUT> old[VL][VE / vec_elems<OUT>()];
+        read_row<DT, OUT, VL, SHORT>(a, v, c, old);
         sum_rows<DT, VL, SHORT>(a, index, 0, count, c, acc);
-        write_row<DT, OUT, VL, SHORT>(a, v, c, acc);
+        write_row<DT, OUT, VL, SHORT>(a, v, c, old, acc);
       }
     }
   } else {
@@ -660,7 +673,9 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void embedding_grad_join_kernel
     for (int w = 1; w < kJoinWaves; ++w)
 #pragma unroll
       for (int e = 0; e < VE; ++e) acc[0][e] += sum[w][e * kWave + lane];
-    write_row<DT, OUT, 1, SHORT>(a, v, c, acc);
+    VecU<OUT> old[1][VE / vec_elems<OUT>()];
+    read_row<DT, OUT, 1, SHORT>(a, v, c, old);
+    write_row<DT, OUT, 1, SHORT>(a, v, c, old, acc);
   }
 }
 
