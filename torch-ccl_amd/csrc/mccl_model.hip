@@ -133,19 +133,36 @@ void launch_embedding_grad(EmbeddingGradArgs a, hipStream_t s) {
   if (pieces) hipLaunchKernelGGL(join, dim3(pieces, chunks), dim3(kJoinWaves * kWave), 0, s, a);
 }
 
-template <int DT, bool GRAD>
+template <int DT, int LANES, int PER>
+void launch_route(const RouterArgs& a, hipStream_t s) {
+  const uint32_t per_group = kRouterWaves * (kWave / LANES);
+  hipLaunchKernelGGL((router_kernel<DT, LANES, PER>), dim3(std::min(kMaxGroups, (a.tokens + per_group - 1) / per_group)),
+                     dim3(kRouterWaves * kWave), 0, s, a);
+}
+
+#ifndef NARROW_MIN
+#define NARROW_MIN 0
+#endif
+// 16 lanes per token up to 256 experts (16 of them a lane), else a wavefront.
+template <int DT>
 void launch_router(const RouterArgs& a, hipStream_t s) {
-  const dim3 grid(std::min(kMaxGroups, (a.tokens + kRouterWaves - 1) / kRouterWaves)), block(kRouterWaves * kWave);
-#define MCCL_LAUNCH_ROUTER(PER)                                                                   \
-  if constexpr (GRAD) hipLaunchKernelGGL((router_grad_kernel<DT, PER>), grid, block, 0, s, a);   \
-  else hipLaunchKernelGGL((router_kernel<DT, PER>), grid, block, 0, s, a)
-  if (a.experts <= 64) { MCCL_LAUNCH_ROUTER(1); }
-  else if (a.experts <= 128) { MCCL_LAUNCH_ROUTER(2); }
-  else if (a.experts <= 256) { MCCL_LAUNCH_ROUTER(4); }
-  else if (a.experts <= 512) { MCCL_LAUNCH_ROUTER(8); }
-  else if (a.experts <= 1024) { MCCL_LAUNCH_ROUTER(16); }
-  else { MCCL_LAUNCH_ROUTER(64); }
-#undef MCCL_LAUNCH_ROUTER
+  if (a.tokens >= NARROW_MIN && a.experts <= 16 * 16) {
+    if (a.experts <= 16) launch_route<DT, 16, 1>(a, s);
+    else if (a.experts <= 32) launch_route<DT, 16, 2>(a, s);
+    else if (a.experts <= 64) launch_route<DT, 16, 4>(a, s);
+    else if (a.experts <= 128) launch_route<DT, 16, 8>(a, s);
+    else launch_route<DT, 16, 16>(a, s);
+  } else if (a.experts <= 256) launch_route<DT, 64, 4>(a, s);
+  else if (a.experts <= 512) launch_route<DT, 64, 8>(a, s);
+  else if (a.experts <= 1024) launch_route<DT, 64, 16>(a, s);
+  else launch_route<DT, 64, 64>(a, s);
+}
+
+template <int DT>
+void launch_router_grad(const RouterArgs& a, hipStream_t s) {
+  auto kernel = a.experts <= 64 ? router_grad_kernel<DT, 1> : a.experts <= 128 ? router_grad_kernel<DT, 2> : a.experts <= 256 ? router_grad_kernel<DT, 4>
+              : a.experts <= 512 ? router_grad_kernel<DT, 8> : a.experts <= 1024 ? router_grad_kernel<DT, 16> : router_grad_kernel<DT, 64>;
+  hipLaunchKernelGGL(kernel, dim3(std::min(kMaxGroups, (a.tokens + kRouterWaves - 1) / kRouterWaves)), dim3(kRouterWaves * kWave), 0, s, a);
 }
 
 int check_router(size_t tokens, size_t experts, int topk, int dtype) {
@@ -349,9 +366,9 @@ int mccl_moe_route(const void* logits, size_t tokens, size_t experts, int topk, 
   a.normalize = normalize ? 1 : 0;
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
-    case MCCL_BF16: launch_router<MCCL_BF16, false>(a, s); break;
-    case MCCL_F16: launch_router<MCCL_F16, false>(a, s); break;
-    default: launch_router<MCCL_F32, false>(a, s); break;
+    case MCCL_BF16: launch_router<MCCL_BF16>(a, s); break;
+    case MCCL_F16: launch_router<MCCL_F16>(a, s); break;
+    default: launch_router<MCCL_F32>(a, s); break;
   }
   return launched("router");
 }
@@ -378,9 +395,9 @@ int mccl_moe_route_grad(const float* grad_weights, const void* logits, const int
   a.normalize = normalize ? 1 : 0;
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
-    case MCCL_BF16: launch_router<MCCL_BF16, true>(a, s); break;
-    case MCCL_F16: launch_router<MCCL_F16, true>(a, s); break;
-    default: launch_router<MCCL_F32, true>(a, s); break;
+    case MCCL_BF16: launch_router_grad<MCCL_BF16>(a, s); break;
+    case MCCL_F16: launch_router_grad<MCCL_F16>(a, s); break;
+    default: launch_router_grad<MCCL_F32>(a, s); break;
   }
   return launched("router gradient");
 }
