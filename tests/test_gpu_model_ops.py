@@ -242,7 +242,8 @@ def route_reference(logits, topk, normalize):
     return torch.where(closed, torch.full_like(ids, -1), ids).int(), w
 
 
-ROUTES = [(1, 1, 1), (7, 5, 5), (16, 64, 6), (33, 65, 3), (50, 100, 8), (200, 256, 8), (9, 257, 8), (40, 512, 4), (5, 1000, 64), (3, 4096, 10)]
+ROUTES = [(1, 1, 1), (7, 5, 5), (16, 64, 6), (33, 65, 3), (50, 100, 8), (200, 256, 8), (9, 257, 8), (40, 512, 4), (5, 1000, 64), (3, 4096, 10),
+          (4097, 16, 2), (4099, 17, 17), (5000, 60, 6), (4500, 100, 20), (4999, 255, 8), (8191, 256, 8)]
 
 
 @pytest.mark.parametrize("dtype", FLOATS, ids=str)

@@ -68,6 +68,19 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return f > -__builtin_inff() ? k : 0u;
 }
 
+// The same for a logit of 16 bits, in 16 bits, and back.
+template <int DT>
+__device__ __forceinline__ uint32_t order_key16(uint16_t u) {
+  constexpr uint32_t kInf = DT == MCCL_BF16 ? 0x7f80u : 0x7c00u;
+  const uint32_t size = u & 0x7fffu;
+  const uint32_t k = (u & 0x8000u) && size ? 0xffffu & ~(uint32_t)u : size | 0x8000u;
+  return size > kInf || u == (0x8000u | kInf) ? 0u : k;
+}
+template <int DT>
+__device__ __forceinline__ float logit_of_key16(uint32_t k) {
+  return Elem<DT>::load((uint16_t)((k & 0x8000u) ? k & 0x7fffu : ~k));
+}
+
 // A lane's PER logits of a row, from column `first` on; -inf behind the row.  Rows begin at any element: the
 // vectors are read at whatever alignment they have.
 template <int DT, int PER>
@@ -88,14 +101,17 @@ __device__ __forceinline__ void load_logits(const typename Elem<DT>::store_t* ro
   }
 }
 
-// LANES lanes per token, PER experts per lane: lane l of the group holds the experts from l * PER on, so that
-// the lowest index among equal logits is the lowest lane's first.  A choice takes the largest key of the
-// group; its owner is the lowest lane that has it, its place the first in that lane.  16 lanes per token
-// serve four tokens with the instructions of one where a lane has room for its share.
+// LANES lanes per token, PER experts per lane: lane l of the group holds the experts from l * PER on; 16
+// lanes per token serve four tokens with the instructions of one.  A choice takes the largest key of the
+// group.  Logits of 16 bits have a key of 32 with the expert's index (the lower the larger) behind the logit:
+// the largest key is the choice.  Keys of fp32 logits fill 32 bits; the choice is the lowest lane that has
+// the largest, and in it the first.
 template <int DT, int LANES, int PER>
 __global__ __launch_bounds__(kRouterWaves * kWave) void router_kernel(const RouterArgs a) {
   using S = typename Elem<DT>::store_t;
+  constexpr bool kPacked = sizeof(S) == 2;
   constexpr uint32_t kTokens = kWave / LANES;  // per wavefront
+  constexpr int kKept = kWave / LANES;         // choices a lane keeps: member, member + LANES, ...
   const uint32_t lane = threadIdx.x % kWave, member = lane % LANES, group = lane / LANES;
   const uint64_t mine = LANES == 64 ? ~0ull : ((1ull << (LANES % 64)) - 1) << (group * LANES);
   const uint32_t step = gridDim.x * kRouterWaves * kTokens;
@@ -107,50 +123,52 @@ __global__ __launch_bounds__(kRouterWaves * kWave) void router_kernel(const Rout
     bool nan = false;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      key[j] = order_key(l[j]);
+      if constexpr (kPacked) {
+        const uint32_t k = order_key16<DT>(Elem<DT>::store(l[j]));
+        key[j] = k ? k << 16 | (0xffffu - (member * PER + j)) : 0u;
+      } else {
+        key[j] = order_key(l[j]);
+      }
       nan |= l[j] != l[j];
     }
     float top = -__builtin_inff();  // the largest logit that can be chosen
-    float my_logit[64 / LANES], my_e[64 / LANES];
-    int32_t my_id[64 / LANES];      // choices member, member + LANES, ...
+    float my_logit[kKept], my_e[kKept];
+    int32_t my_id[kKept];
 #pragma unroll
-    for (int x = 0; x < 64 / LANES; ++x) { my_id[x] = -1; my_logit[x] = 0.0f; }
-    uint32_t best = 0;
-    int at = 0;
-#pragma unroll
-    for (int j = PER - 1; j >= 0; --j) {
-      const bool up = key[j] >= best;
-      best = up ? key[j] : best;
-      at = up ? j : at;
-    }
+    for (int x = 0; x < kKept; ++x) { my_id[x] = -1; my_logit[x] = 0.0f; }
     for (uint32_t k = 0; k < a.topk; ++k) {
+      uint32_t best = key[0];
+#pragma unroll
+      for (int j = 1; j < PER; ++j) best = key[j] > best ? key[j] : best;
       const uint32_t all = group_max<LANES>(best);
-      const uint64_t have = __ballot(best == all) & mine;
-      const uint32_t owner = (uint32_t)__builtin_ctzll(have);
-      const bool owns = lane == owner && all;
-      const int place = LANES == 64 ? __builtin_amdgcn_readlane(at, owner) : __shfl(at, (int)owner);
-      const int32_t id = all ? (int32_t)((owner % LANES) * PER + place) : -1;
-      // the key is the logit: turned back, it needs no look at the owner's registers
-      const float value = bits_to_f32((all & 0x80000000u) ? all ^ 0x80000000u : ~all);
+      int32_t id;
+      float value;
+      if constexpr (kPacked) {
+        id = all ? (int32_t)(0xffffu - (all & 0xffffu)) : -1;
+        value = logit_of_key16<DT>(all >> 16);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) key[j] = key[j] == all ? 0u : key[j];
+      } else {
+        int at = 0;
+#pragma unroll
+        for (int j = PER - 1; j >= 0; --j) at = key[j] == all ? j : at;
+        const uint64_t have = __ballot(best == all) & mine;
+        const uint32_t owner = (uint32_t)__builtin_ctzll(have);
+        const int place = LANES == 64 ? __builtin_amdgcn_readlane(at, owner) : __shfl(at, (int)owner);
+        id = all ? (int32_t)((owner % LANES) * PER + place) : -1;
+        value = bits_to_f32((all & 0x80000000u) ? all ^ 0x80000000u : ~all);
+        const int gone = lane == owner ? at : -1;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) key[j] = j == gone ? 0u : key[j];
+      }
       if (k == 0 && all) top = value;
 #pragma unroll
-      for (int x = 0; x < 64 / LANES; ++x)
+      for (int x = 0; x < kKept; ++x)
         if (k == member + x * LANES) { my_id[x] = id; my_logit[x] = value; }
-      if (owns) {  // the owner's next best
-#pragma unroll
-        for (int j = 0; j < PER; ++j) key[j] = j == at ? 0u : key[j];
-        best = 0;
-#pragma unroll
-        for (int j = PER - 1; j >= 0; --j) {
-          const bool up = key[j] >= best;
-          best = up ? key[j] : best;
-          at = up ? j : at;
-        }
-      }
     }
     float total = 0.0f;
 #pragma unroll
-    for (int x = 0; x < 64 / LANES; ++x) {
+    for (int x = 0; x < kKept; ++x) {
       my_e[x] = my_id[x] >= 0 ? expf(my_logit[x] - top) : 0.0f;
       total += my_e[x];
     }
@@ -163,7 +181,7 @@ __global__ __launch_bounds__(kRouterWaves * kWave) void router_kernel(const Rout
     if (__ballot(nan) & mine) total = __builtin_nanf("");  // the softmax of a row that holds a NaN
     if (t0 + group < a.tokens) {
 #pragma unroll
-      for (int x = 0; x < 64 / LANES; ++x) {
+      for (int x = 0; x < kKept; ++x) {
         const uint32_t k = member + x * LANES;
         if (k < a.topk) {
           a.ids[(size_t)t * a.topk + k] = my_id[x];
@@ -177,74 +195,102 @@ __global__ __launch_bounds__(kRouterWaves * kWave) void router_kernel(const Rout
 // d_logits of sum_k grad_weights[k] * weights[k].  With p = softmax(logits) and s = sum_k g_k w_k:
 //   not normalised (w = p):            d_e = p_e ([e chosen] g_e - s)
 //   normalised (w = softmax of the chosen): d_e = [e chosen] w_e (g_e - s)
-// A wavefront per token; what the chosen experts get goes through LDS to the lanes that write them.
-template <int DT, int PER>
+// LANES lanes per token as in router_kernel; what the chosen experts get goes through LDS to the lanes that
+// write it.
+template <int DT, int LANES, int PER>
 __global__ __launch_bounds__(kRouterWaves * kWave) void router_grad_kernel(const RouterArgs a) {
   using S = typename Elem<DT>::store_t;
+  constexpr uint32_t kTokens = kWave / LANES;
+  constexpr int kKept = kWave / LANES;
+  constexpr int VE = PER < vec_elems<DT>() ? PER : vec_elems<DT>();
+  typedef S vec __attribute__((ext_vector_type(VE)));
+  typedef vec vec_unaligned __attribute__((aligned(sizeof(S))));
   __shared__ float space[kRouterWaves][kWave * PER];
-  const uint32_t lane = threadIdx.x % kWave;
-  float* chosen = space[threadIdx.x / kWave];
-  for (uint32_t t = blockIdx.x * kRouterWaves + threadIdx.x / kWave; t < a.tokens; t += gridDim.x * kRouterWaves) {
+  const uint32_t lane = threadIdx.x % kWave, member = lane % LANES, group = lane / LANES;
+  // Where expert j of a lane lies in its group's space: a lane's few in one vector, more of them across the
+  // lanes, so that the lanes' accesses fall into different banks.
+  constexpr bool kAcross = PER > 4;
+  float* chosen = space[threadIdx.x / kWave] + group * (LANES * PER);
+  const auto at = [](uint32_t who, uint32_t j) { return kAcross ? j * LANES + who : who * PER + j; };
+  const uint32_t step = gridDim.x * kRouterWaves * kTokens;
+  for (uint32_t t0 = (blockIdx.x * kRouterWaves + threadIdx.x / kWave) * kTokens; t0 < a.tokens; t0 += step) {
+    const uint32_t t = t0 + group < a.tokens ? t0 + group : a.tokens - 1;  // the last token again: not stored
     const S* row = (const S*)a.logits + (size_t)t * a.experts;
-    S* out = (S*)a.grad_logits + (size_t)t * a.experts;
-    int32_t id = -1;
-    float g = 0.0f, value = -__builtin_inff();
-    if (lane < a.topk) {
-      id = a.chosen[(size_t)t * a.topk + lane];
-      g = a.grad_weights[(size_t)t * a.topk + lane];
-      if (id < 0 || (uint32_t)id >= a.experts) id = -1;
-      if (id >= 0) value = Elem<DT>::load(row[id]);
+    int32_t id[kKept];
+    float g[kKept], value[kKept], w[kKept];
+#pragma unroll
+    for (int x = 0; x < kKept; ++x) {
+      const uint32_t k = member + x * LANES;
+      id[x] = -1;
+      g[x] = 0.0f;
+      value[x] = -__builtin_inff();
+      if (k < a.topk) {
+        id[x] = a.chosen[(size_t)t * a.topk + k];
+        g[x] = a.grad_weights[(size_t)t * a.topk + k];
+        if (id[x] < 0 || (uint32_t)id[x] >= a.experts) { id[x] = -1; g[x] = 0.0f; }
+        if (id[x] >= 0) value[x] = Elem<DT>::load(row[id[x]]);
+      }
     }
-    if (id < 0) g = 0.0f;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) chosen[lane * PER + j] = 0.0f;
+    for (int j = 0; j < PER; ++j) chosen[at(member, j)] = 0.0f;
     float p[PER];
-    float top, total;
+    float top = -__builtin_inff(), total = 0.0f;
     if (a.normalize) {
-      top = group_max<64>(value);
-      total = group_sum<64>(id >= 0 ? expf(value - top) : 0.0f);
-    } else {
-      load_logits<DT, PER>(row, lane * PER, a.experts, p);
-      top = p[0];
 #pragma unroll
-      for (int j = 1; j < PER; ++j) top = p[j] > top ? p[j] : top;
-      top = group_max<64>(top);
-      total = 0.0f;
+      for (int x = 0; x < kKept; ++x) top = value[x] > top ? value[x] : top;
+      top = group_max<LANES>(top);
+#pragma unroll
+      for (int x = 0; x < kKept; ++x) total += id[x] >= 0 ? expf(value[x] - top) : 0.0f;
+    } else {
+      load_logits<DT, PER>(row, member * PER, a.experts, p);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) top = p[j] > top ? p[j] : top;
+      top = group_max<LANES>(top);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        p[j] = lane * PER + j < a.experts ? expf(p[j] - top) : 0.0f;
+        p[j] = member * PER + j < a.experts ? expf(p[j] - top) : 0.0f;
         total += p[j];
       }
-      total = group_sum<64>(total);
     }
+    total = group_sum<LANES>(total);
     const bool none = top == -__builtin_inff();  // nothing could be chosen: no gradient
-    const float w = id >= 0 && !none ? expf(value - top) / total : 0.0f;
-    const float mean = group_sum<64>(g * w);
-    // an expert that is named more than once gets every share
-    if (id >= 0) atomicAdd(&chosen[id], a.normalize ? w * (g - mean) : w * g);
+    float mean = 0.0f;
+#pragma unroll
+    for (int x = 0; x < kKept; ++x) {
+      w[x] = id[x] >= 0 && !none ? expf(value[x] - top) / total : 0.0f;
+      mean += g[x] * w[x];
+    }
+    mean = group_sum<LANES>(mean);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    union { S e[PER]; } r;
+    // an expert that is named more than once gets every share
+#pragma unroll
+    for (int x = 0; x < kKept; ++x)
+      if (id[x] >= 0) atomicAdd(&chosen[at((uint32_t)id[x] / PER, (uint32_t)id[x] % PER)], a.normalize ? w[x] * (g[x] - mean) : w[x] * g[x]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const float share = mean / total;
+    S r[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const float own = chosen[lane * PER + j];
-      r.e[j] = Elem<DT>::store(a.normalize || none ? own : own - (p[j] / total) * mean);
+      const float own = chosen[at(member, j)];
+      r[j] = Elem<DT>::store(a.normalize || none ? own : own - p[j] * share);
     }
-    if (lane * PER + PER <= a.experts) {
-      constexpr int VE = PER < vec_elems<DT>() ? PER : vec_elems<DT>();
-      typedef S vec __attribute__((ext_vector_type(VE)));
-      typedef vec vec_unaligned __attribute__((aligned(sizeof(S))));
+    if (t0 + group < a.tokens) {
+      S* out = (S*)a.grad_logits + (size_t)t * a.experts + member * PER;
+      if (member * PER + PER <= a.experts) {
 #pragma unroll
-      for (int b = 0; b < PER / VE; ++b) {
-        vec v;
+        for (int b = 0; b < PER; b += VE) {
+          vec v;
 #pragma unroll
-        for (int j = 0; j < VE; ++j) v[j] = r.e[b * VE + j];
-        *(vec_unaligned*)(out + lane * PER + b * VE) = v;
+          for (int j = 0; j < VE; ++j) v[j] = r[b + j];
+          *(vec_unaligned*)(out + b) = v;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (member * PER + j < a.experts) out[j] = r[j];
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (lane * PER + j < a.experts) out[lane * PER + j] = r.e[j];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
