@@ -239,12 +239,13 @@ __global__ __launch_bounds__(kInWaves * kWave) void layer_in_kernel(const LayerA
 // all pairs in LDS, so that the weighted sum needs no other workgroup: work of a wavefront is an expert
 // and one of a.parts parts of inter.
 struct LayerOutLds {
-  uint32_t first, active, lists, y, bytes;
+  uint32_t weights, first, active, lists, y, bytes;
 };
 __host__ __device__ inline LayerOutLds layer_out_lds(uint32_t pairs, uint32_t experts, uint32_t parts, uint32_t rows, uint32_t waves) {
   LayerOutLds l;
   const uint32_t p8 = (pairs + 7) / 8 * 8;
-  l.first = p8 * 2;                             // the experts of the pairs come first, int16
+  l.weights = p8 * 2;                           // the experts of the pairs come first, int16
+  l.first = l.weights + p8 * 4;                 // their weights, fp32
   l.active = l.first + (experts + 3) / 4 * 16;  // first pair of every expert, uint32
   l.lists = l.active + p8 * 2;                  // first pairs of the chosen experts, uint16
   l.y = l.lists + waves * kListSpace * 2;       // a list per wavefront, uint16
@@ -300,11 +301,13 @@ __global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArg
   extern __shared__ char lds[];
   const LayerOutLds l = layer_out_lds(a.pairs, a.experts, a.parts, kRows, WAVES);
   int16_t* expert = (int16_t*)lds;
+  float* weight = (float*)(lds + l.weights);
   uint32_t* first = (uint32_t*)(lds + l.first);
   uint16_t* active = (uint16_t*)(lds + l.active);
   float* y = (float*)(lds + l.y);
   const uint32_t lane = threadIdx.x % kWave, wave = wave_index();
   uint16_t* list = (uint16_t*)(lds + l.lists) + wave * kListSpace;
+  for (uint32_t p = threadIdx.x; p < a.pairs; p += WAVES * kWave) weight[p] = a.weights[p];
   for (uint32_t e = threadIdx.x; e < a.experts; e += WAVES * kWave) first[e] = ~0u;
   stage_experts(a, expert);
   for (uint32_t p = threadIdx.x; p < a.pairs; p += WAVES * kWave)
@@ -344,7 +347,7 @@ __global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArg
       if (expert[p] < 0) continue;
       float v = 0.0f;
       for (uint32_t q = 0; q < a.parts; ++q) v += y[(p * a.parts + q) * kRows + c];
-      sum += a.weights[p] * v;
+      sum += weight[p] * v;
     }
     ((S*)a.out)[(size_t)t * a.hidden + c0 + c] = Elem<DT>::store(sum);
   }
@@ -498,12 +501,15 @@ __global__ __launch_bounds__(256) void layer_join_kernel(const LayerArgs a) {
   const uint32_t t = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (c >= a.hidden) return;
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  // Pairs of other ranks' experts are read too (nobody has written their y) and left out: the loads of several
+  // pairs are in flight together.
+#pragma unroll 4
   for (uint32_t k = 0; k < a.topk; ++k) {
     const uint32_t p = t * a.topk + k;
-    if (local_expert(a, p) < 0) continue;
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t q = 0; q < a.parts; ++q) v += *(const f32x4*)(a.y + ((size_t)q * a.pairs + p) * a.hidden + c);
-    sum += a.weights[p] * v;
+    v = a.weights[p] * v;
+    if (local_expert(a, p) >= 0) sum += v;
   }
   union { S e[4]; uint2 v; } r;
 #pragma unroll

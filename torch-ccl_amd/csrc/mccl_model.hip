@@ -194,7 +194,9 @@ LayerPlan plan_layer(size_t tokens, size_t pairs, size_t experts, size_t hidden,
     p.parts = (uint32_t)((chunks + per - 1) / per);
     p.bytes += p.parts * pairs * hidden * sizeof(float);
   } else {
-    p.parts = (uint32_t)std::min<size_t>((inter + kStepCols - 1) / kStepCols, (16 + pairs - 1) / pairs);
+    // as many parts as give 8 wavefronts something to do; more only add joining (5 tokens x 3 experts, inter 200:
+    // 10.9 us with one part, 12.7 with two)
+    p.parts = (uint32_t)std::min<size_t>((inter + kStepCols - 1) / kStepCols, std::max<size_t>(1, 8 / pairs));
   }
   return p;
 }
@@ -207,6 +209,14 @@ int launch_dense(const LayerArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((layer_dense_kernel<DT, TOKENS, false>), dim3(out_tiles), dim3(kDenseBlock), 0, s, a);
   hipLaunchKernelGGL(layer_join_kernel<DT>, dim3((a.hidden / 4 + 255) / 256, a.tokens), dim3(256), 0, s, a);
   return launched("moe layer");
+}
+
+// Whether a workgroup of the second product takes 16 rows with 8 wavefronts, instead of 8 rows with 16: it
+// reads the tokens half as often, if it fills the 256 compute units evenly (1 token, hidden 4096: 36.5 us
+// against 38.5; 64 tokens x 128 experts 303 against 326; but hidden 5120, 320 workgroups, 240 against 230).
+bool wide_out(size_t hidden, size_t pairs) {
+  const size_t groups = (hidden + 15) / 16, rounds = (groups + 255) / 256;
+  return pairs <= 1024 && groups * 5 >= rounds * 256 * 4;
 }
 
 template <int DT, int NW, int WAVES>
@@ -227,7 +237,7 @@ int launch_layer(const LayerArgs& a, int dense, hipStream_t s) {
   if (a.tokens <= 8) hipLaunchKernelGGL((layer_in_kernel<DT, 8>), in_grid, in_block, 0, s, a);
   else if (a.tokens <= 16) hipLaunchKernelGGL((layer_in_kernel<DT, 16>), in_grid, in_block, 0, s, a);
   else hipLaunchKernelGGL((layer_in_kernel<DT, 32>), in_grid, in_block, 0, s, a);
-  const int rc = a.hidden >= 4096 && a.pairs <= 1024 ? launch_layer_out<DT, 2, 8>(a, s) : launch_layer_out<DT, 1, 16>(a, s);
+  const int rc = wide_out(a.hidden, a.pairs) ? launch_layer_out<DT, 2, 8>(a, s) : launch_layer_out<DT, 1, 16>(a, s);
   return rc != MCCL_OK ? rc : launched("moe layer");
 }
 
