@@ -6,6 +6,7 @@ libmi355ccl.so on the current torch stream.  Argument checks follow the referenc
 live on the GPU.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -318,6 +319,12 @@ _MODEL_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _ID_TYPES = (torch.int32, torch.int64)
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(query, *sizes):
+    """What a workspace query of the C ABI says, which depends on the sizes alone."""
+    return getattr(capi.lib(), query)(*sizes)
+
+
 def _workspace(what, given, nbytes, device):
     """(address, bytes) of the caller's workspace (uint8, large enough) or of one from torch's allocator
     for this call, and the tensor itself, to be kept until the call has been made."""
@@ -362,7 +369,7 @@ def sort_ids(ids, rows, first_row=0, workspace=None):
     n = ids.numel()
     order = torch.empty(n, dtype=torch.int64, device=device)
     offsets = torch.empty(rows + 1, dtype=torch.int64, device=device)
-    ws, ws_bytes, _held = _workspace("sort_ids", workspace, capi.lib().mccl_sort_ids_workspace(n), device)
+    ws, ws_bytes, _held = _workspace("sort_ids", workspace, _workspace_bytes("mccl_sort_ids_workspace", n), device)
     _launch(device, capi.lib().mccl_sort_ids, ids.data_ptr(), _dtype_code(ids.dtype), n, first_row, rows, ws, ws_bytes,
             order.data_ptr(), offsets.data_ptr())
     return order, offsets
@@ -390,7 +397,7 @@ def embedding_grad(grad, sorted_ids, scale=1.0, dtype=None, out=None, accumulate
         out = torch.empty((rows, hidden), dtype=dtype or grad.dtype, device=grad.device)
     _check_shape("embedding_grad", "out", out, (rows, hidden), *((dtype,) if dtype else (grad.dtype, torch.float32)))
     device = _check_gpu("embedding_grad", ("grad", "order", "offsets", "out"), (grad, order, offsets, out))
-    ws, ws_bytes, _held = _workspace("embedding_grad", workspace, capi.lib().mccl_embedding_grad_workspace(n, hidden), device)
+    ws, ws_bytes, _held = _workspace("embedding_grad", workspace, _workspace_bytes("mccl_embedding_grad_workspace", n, hidden), device)
     _launch(device, capi.lib().mccl_embedding_grad, grad.data_ptr(), order.data_ptr(), offsets.data_ptr(), n, rows, hidden, scale,
             _dtype_code(grad.dtype), out.data_ptr(), _dtype_code(out.dtype), bool(accumulate), ws, ws_bytes)
     return out
@@ -460,7 +467,7 @@ def moe_layer(x, w_in, w_out, expert_ids, weights, first_expert=0, activation="s
     _check_shape("moe_layer", "weights", weights, (tokens, topk), torch.float32)
     _check_shape("moe_layer", "out", out, x.shape, x.dtype)
     device = _check_gpu("moe_layer", ("x", "w_in", "w_out", "expert_ids", "weights", "out"), (x, w_in, w_out, expert_ids, weights, out))
-    ws, ws_bytes, _held = _workspace("moe_layer", workspace, capi.lib().mccl_moe_layer_workspace(tokens, topk, experts, hidden, inter), device)
+    ws, ws_bytes, _held = _workspace("moe_layer", workspace, _workspace_bytes("mccl_moe_layer_workspace", tokens, topk, experts, hidden, inter), device)
     _launch(device, capi.lib().mccl_moe_layer, x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), expert_ids.data_ptr(), weights.data_ptr(),
             tokens, topk, experts, first_expert, hidden, inter, _ACTIVATIONS[activation], _dtype_code(x.dtype), out.data_ptr(), ws, ws_bytes)
     return out
