@@ -4,7 +4,8 @@
   libmcclbench.so  HIP-event timing loops around that ABI (bench/mccl_bench.h; lands in bench/).
   _C.*.so          the c10d backend (process_group_ccl.cpp: the group and how a collective runs;
                    pg_sharing.cpp: staging, shared allocations, standing offers; pg_collectives.cpp;
-                   pg_p2p.cpp) and its Python module; host code only, links torch's c10d and
+                   pg_p2p.cpp), the tensor front end of the operators around the collectives
+                   (model_ops.cpp) and the Python module; host code only, links torch's c10d and
                    libmi355ccl.so.
 
 Usage: python torch-ccl_amd/csrc/build.py [--force]
@@ -104,8 +105,8 @@ def build_bench(force=False):
     return BENCH_LIB
 
 
-BACKEND_SRCS = [os.path.join(HERE, f) for f in ("process_group_ccl.cpp", "pg_sharing.cpp", "pg_collectives.cpp", "pg_p2p.cpp", "python_module.cpp")]
-BACKEND_HDRS = [os.path.join(HERE, "process_group_ccl.hpp"), os.path.join(HERE, "pg_internal.hpp"), os.path.join(INCLUDE, "mccl.h")]
+BACKEND_SRCS = [os.path.join(HERE, f) for f in ("process_group_ccl.cpp", "pg_sharing.cpp", "pg_collectives.cpp", "pg_p2p.cpp", "model_ops.cpp", "python_module.cpp")]
+BACKEND_HDRS = [os.path.join(HERE, "process_group_ccl.hpp"), os.path.join(HERE, "pg_internal.hpp"), os.path.join(HERE, "model_ops.hpp"), os.path.join(INCLUDE, "mccl.h")]
 
 
 def backend_lib_path():

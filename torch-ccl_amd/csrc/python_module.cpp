@@ -1,11 +1,13 @@
 // Python module torch_ccl_amd._C: registers the c10d backend "ccl" for ROCm ("cuda") tensors and
 // exposes torch.distributed.ProcessGroupCCL(store, rank, size, timeout) -- the registration
-// contract of the reference's module init (oneccl_bindings_for_pytorch/csrc/init.cpp:123-154).
+// contract of the reference's module init (oneccl_bindings_for_pytorch/csrc/init.cpp:123-154) -- and
+// holds the tensor front end of the operators around the collectives (model_ops.cpp).
 #include <pybind11/chrono.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include "model_ops.hpp"
 #include "process_group_ccl.hpp"
 
 namespace py = pybind11;
@@ -60,6 +62,8 @@ PYBIND11_MODULE(_C, m) {
   m.def("register", [register_backend, creator](const std::string& name) {
     register_backend(name, creator, false, std::vector<std::string>{"cuda"});
   });
+
+  register_model_ops(m);
 
   // a Work without device work behind it, for tests of wait(timeout) that need no GPU
   m.def("_pending_work", &ProcessGroupCCL::pendingWork, py::arg("rank"), py::arg("polls"), py::arg("op_timeout"));

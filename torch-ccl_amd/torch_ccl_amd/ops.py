@@ -6,11 +6,13 @@ libmi355ccl.so on the current torch stream.  Argument checks follow the referenc
 live on the GPU.
 """
 import ctypes
-import functools
 
 import torch
 
 from . import capi
+
+capi.lib()  # fails loudly when the native library is absent; the extension links it
+from . import _C  # noqa: E402
 
 
 def _stream():
@@ -284,75 +286,15 @@ def route_counts(expert_ids, n_experts, workspace=None, out=None):
     return out
 
 
-def _check_gpu(what, names, tensors):
-    """Every tensor on the GPU, contiguous, all on one device; returns that device."""
-    device = tensors[0].device
-    for i, t in enumerate(tensors):
-        if not t.is_cuda:
-            raise RuntimeError("%s: tensors must be on the GPU (got %s)" % (what, t.device))
-        if not t.is_contiguous():
-            raise RuntimeError("%s: %s has to be contiguous" % (what, names[i]))
-        if t.device != device:
-            raise RuntimeError("%s: tensors must share one device" % what)
-    return device
-
-
-def _check_shape(what, name, t, shape, *dtypes):
-    if t.shape != shape or t.dtype not in dtypes:
-        raise RuntimeError("%s: %s must be %s of shape %s (got %s %s)" % (
-            what, name, " or ".join(str(d).replace("torch.", "") for d in dtypes), list(shape), t.dtype, list(t.shape)))
-
-
-def _launch(device, entry, *args):
-    """Calls `entry` of the C ABI on the current stream of `device`, which is made current if it is not.
-    These calls are short: the device is switched only where it has to be (1.3 us) and the stream's
-    handle is taken without its Python object (0.1 us against 2.7)."""
-    index = device.index
-    if torch._C._cuda_getDevice() == index:
-        capi.check(entry(*args, torch._C._cuda_getCurrentRawStream(index)))
-    else:
-        with torch.cuda.device(index):
-            capi.check(entry(*args, torch._C._cuda_getCurrentRawStream(index)))
-
-
-_MODEL_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
-_ID_TYPES = (torch.int32, torch.int64)
-
-
-@functools.lru_cache(maxsize=1024)
-def _workspace_bytes(query, *sizes):
-    """What a workspace query of the C ABI says, which depends on the sizes alone."""
-    return getattr(capi.lib(), query)(*sizes)
-
-
-def _workspace(what, given, nbytes, device):
-    """(address, bytes) of the caller's workspace (uint8, large enough) or of one from torch's allocator
-    for this call, and the tensor itself, to be kept until the call has been made."""
-    if given is None:
-        if nbytes == 0:
-            return None, 0, None
-        given = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    elif given.dtype != torch.uint8 or given.device != device or not given.is_contiguous() or given.numel() < nbytes:
-        raise RuntimeError("%s: workspace must be %d bytes of uint8 on %s" % (what, nbytes, device))
-    return given.data_ptr(), given.numel(), given
-
+# The operators that compute around the collectives.  Their checks, allocations and the call of the C ABI on
+# the current stream of the tensors' device are in the extension: these calls are short enough for the
+# interpreter's share to matter.
 
 def embedding(table, ids, scale=1.0, first_row=0, out=None):
     """out[..., :] = scale * table[ids - first_row] where that row lies in the table, zeros elsewhere
     (another rank's rows of a sharded vocabulary, padding).  table [rows, hidden] in bf16 / f16 / f32,
     ids int32 or int64 of any shape; rounded once to the table's type."""
-    if table.dim() != 2 or table.dtype not in _MODEL_FLOATS:
-        raise RuntimeError("embedding: table must be a matrix in bf16, f16 or f32")
-    if ids.dtype not in _ID_TYPES:
-        raise RuntimeError("embedding: ids must be int32 or int64")
-    shape = tuple(ids.shape) + (table.shape[1],)
-    if out is None:
-        out = torch.empty(shape, dtype=table.dtype, device=table.device)
-    _check_shape("embedding", "out", out, shape, table.dtype)
-    device = _check_gpu("embedding", ("table", "ids", "out"), (table, ids, out))
-    _launch(device, capi.lib().mccl_embedding, table.data_ptr(), table.shape[0], ids.data_ptr(), _dtype_code(ids.dtype), ids.numel(),
-            first_row, table.shape[1], scale, _dtype_code(table.dtype), out.data_ptr())
-    return out
+    return _C.embedding(table, ids, scale, first_row, out)
 
 
 def sort_ids(ids, rows, first_row=0, workspace=None):
@@ -360,19 +302,7 @@ def sort_ids(ids, rows, first_row=0, workspace=None):
     ids - first_row (those outside [0, rows) last), and for every row v the range
     order[offsets[v]:offsets[v + 1]] of its tokens.  For the expert ids of a routing, order // topk is
     the row_index of moe_dispatch_n and offsets.diff() are the pairs per expert."""
-    if ids.dtype not in _ID_TYPES:
-        raise RuntimeError("sort_ids: ids must be int32 or int64")
-    rows = int(rows)
-    if rows < 0:
-        raise RuntimeError("sort_ids: negative row count")
-    device = _check_gpu("sort_ids", ("ids",), (ids,))
-    n = ids.numel()
-    order = torch.empty(n, dtype=torch.int64, device=device)
-    offsets = torch.empty(rows + 1, dtype=torch.int64, device=device)
-    ws, ws_bytes, _held = _workspace("sort_ids", workspace, _workspace_bytes("mccl_sort_ids_workspace", n), device)
-    _launch(device, capi.lib().mccl_sort_ids, ids.data_ptr(), _dtype_code(ids.dtype), n, first_row, rows, ws, ws_bytes,
-            order.data_ptr(), offsets.data_ptr())
-    return order, offsets
+    return _C.sort_ids(ids, rows, first_row, workspace)
 
 
 def embedding_grad(grad, sorted_ids, scale=1.0, dtype=None, out=None, accumulate=False, workspace=None):
@@ -381,71 +311,22 @@ def embedding_grad(grad, sorted_ids, scale=1.0, dtype=None, out=None, accumulate
     [..., hidden]; out [rows, hidden] in grad's type or fp32 (`dtype`).  With accumulate the sums are
     added to `out` and rows without a token stay as they are.  The same bits every time."""
     order, offsets = sorted_ids
-    if grad.dim() < 1 or grad.dtype not in _MODEL_FLOATS:
-        raise RuntimeError("embedding_grad: grad must be bf16, f16 or f32")
-    hidden, n = grad.shape[-1], order.numel()
-    if grad.numel() != n * hidden:
-        raise RuntimeError("embedding_grad: grad must hold one row per sorted id")
-    if offsets.dim() != 1 or offsets.numel() < 1:
-        raise RuntimeError("embedding_grad: offsets must hold rows + 1 entries")
-    _check_shape("embedding_grad", "order", order, (n,), torch.int64)
-    _check_shape("embedding_grad", "offsets", offsets, offsets.shape, torch.int64)
-    rows = offsets.numel() - 1
-    if out is None:
-        if accumulate:
-            raise RuntimeError("embedding_grad: accumulate needs the tensor to add to (out)")
-        out = torch.empty((rows, hidden), dtype=dtype or grad.dtype, device=grad.device)
-    _check_shape("embedding_grad", "out", out, (rows, hidden), *((dtype,) if dtype else (grad.dtype, torch.float32)))
-    device = _check_gpu("embedding_grad", ("grad", "order", "offsets", "out"), (grad, order, offsets, out))
-    ws, ws_bytes, _held = _workspace("embedding_grad", workspace, _workspace_bytes("mccl_embedding_grad_workspace", n, hidden), device)
-    _launch(device, capi.lib().mccl_embedding_grad, grad.data_ptr(), order.data_ptr(), offsets.data_ptr(), n, rows, hidden, scale,
-            _dtype_code(grad.dtype), out.data_ptr(), _dtype_code(out.dtype), bool(accumulate), ws, ws_bytes)
-    return out
+    return _C.embedding_grad(grad, order, offsets, scale, dtype, out, accumulate, workspace)
 
 
-def moe_route(logits, topk, normalize=True, out=None):
+def moe_route(logits, topk, normalize=True, out=(None, None)):
     """(expert_ids int32, weights fp32), both [tokens, topk]: the experts with the largest logits (ties
     to the lowest index) and their softmax probabilities, with `normalize` divided by their sum: what
     route_counts, moe_combine and moe_layer take.  A logit of -inf closes an expert; where fewer than
-    topk are open the rest is id -1 with weight 0.  logits [tokens, experts] in bf16 / f16 / f32."""
-    if logits.dim() != 2 or logits.dtype not in _MODEL_FLOATS:
-        raise RuntimeError("moe_route: logits must be [tokens, experts] in bf16, f16 or f32")
-    tokens, experts = logits.shape
-    shape = (tokens, int(topk))
-    if shape[1] < 1:
-        raise RuntimeError("moe_route: topk must be positive")
-    if out is None:
-        out = (torch.empty(shape, dtype=torch.int32, device=logits.device), torch.empty(shape, dtype=torch.float32, device=logits.device))
-    ids, weights = out
-    _check_shape("moe_route", "expert_ids", ids, shape, torch.int32)
-    _check_shape("moe_route", "weights", weights, shape, torch.float32)
-    device = _check_gpu("moe_route", ("logits", "expert_ids", "weights"), (logits, ids, weights))
-    _launch(device, capi.lib().mccl_moe_route, logits.data_ptr(), tokens, experts, shape[1], bool(normalize), _dtype_code(logits.dtype),
-            ids.data_ptr(), weights.data_ptr())
-    return ids, weights
+    topk are open the rest is id -1 with weight 0.  logits [tokens, experts] in bf16 / f16 / f32; out: the
+    two results' tensors."""
+    return _C.moe_route(logits, topk, normalize, *out)
 
 
 def moe_route_grad(grad_weights, logits, expert_ids, normalize=True, out=None):
     """The gradient in the logits of moe_route()'s weights: grad_weights fp32 and expert_ids int32
     [tokens, topk] (as moe_route chose them; -1 is skipped), in the logits' type."""
-    if logits.dim() != 2 or logits.dtype not in _MODEL_FLOATS:
-        raise RuntimeError("moe_route_grad: logits must be [tokens, experts] in bf16, f16 or f32")
-    tokens, experts = logits.shape
-    if expert_ids.dim() != 2:
-        raise RuntimeError("moe_route_grad: expert_ids must be [tokens, topk]")
-    topk = expert_ids.shape[1]
-    if out is None:
-        out = torch.empty_like(logits)
-    _check_shape("moe_route_grad", "expert_ids", expert_ids, (tokens, topk), torch.int32)
-    _check_shape("moe_route_grad", "grad_weights", grad_weights, (tokens, topk), torch.float32)
-    _check_shape("moe_route_grad", "out", out, logits.shape, logits.dtype)
-    device = _check_gpu("moe_route_grad", ("grad_weights", "logits", "expert_ids", "out"), (grad_weights, logits, expert_ids, out))
-    _launch(device, capi.lib().mccl_moe_route_grad, grad_weights.data_ptr(), logits.data_ptr(), expert_ids.data_ptr(), tokens, experts,
-            topk, bool(normalize), _dtype_code(logits.dtype), out.data_ptr())
-    return out
-
-
-_ACTIVATIONS = {"silu": capi.ACT_SILU, "gelu": capi.ACT_GELU}
+    return _C.moe_route_grad(grad_weights, logits, expert_ids, normalize, out)
 
 
 def moe_layer(x, w_in, w_out, expert_ids, weights, first_expert=0, activation="silu", out=None, workspace=None):
@@ -454,23 +335,7 @@ def moe_layer(x, w_in, w_out, expert_ids, weights, first_expert=0, activation="s
     e = expert_ids[t, k] - first_expert, over the experts this rank holds; an all_reduce adds the ranks'
     parts.  x [tokens, hidden], w_in [experts, 2 * inter, hidden], w_out [experts, hidden, inter] in bf16
     or f16; activation "silu" or "gelu" (exact)."""
-    if activation not in _ACTIVATIONS:
-        raise RuntimeError("moe_layer: activation must be one of %s" % ", ".join(sorted(_ACTIVATIONS)))
-    if x.dim() != 2 or w_in.dim() != 3 or w_out.dim() != 3 or expert_ids.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
-        raise RuntimeError("moe_layer: x [tokens, hidden], w_in [experts, 2 * inter, hidden] and w_out [experts, hidden, inter] in bf16 or f16")
-    (tokens, hidden), (experts, _, inter), topk = x.shape, w_out.shape, expert_ids.shape[1]
-    if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    _check_shape("moe_layer", "w_in", w_in, (experts, 2 * inter, hidden), x.dtype)
-    _check_shape("moe_layer", "w_out", w_out, (experts, hidden, inter), x.dtype)
-    _check_shape("moe_layer", "expert_ids", expert_ids, (tokens, topk), torch.int32)
-    _check_shape("moe_layer", "weights", weights, (tokens, topk), torch.float32)
-    _check_shape("moe_layer", "out", out, x.shape, x.dtype)
-    device = _check_gpu("moe_layer", ("x", "w_in", "w_out", "expert_ids", "weights", "out"), (x, w_in, w_out, expert_ids, weights, out))
-    ws, ws_bytes, _held = _workspace("moe_layer", workspace, _workspace_bytes("mccl_moe_layer_workspace", tokens, topk, experts, hidden, inter), device)
-    _launch(device, capi.lib().mccl_moe_layer, x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), expert_ids.data_ptr(), weights.data_ptr(),
-            tokens, topk, experts, first_expert, hidden, inter, _ACTIVATIONS[activation], _dtype_code(x.dtype), out.data_ptr(), ws, ws_bytes)
-    return out
+    return _C.moe_layer(x, w_in, w_out, expert_ids, weights, first_expert, activation, out, workspace)
 
 
 def empty_staggered(n, shape, dtype, device="cuda", stagger_bytes=4096):
