@@ -68,17 +68,27 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return f > -__builtin_inff() ? k : 0u;
 }
 
-// The same for a logit of 16 bits, in 16 bits, and back.
+// The same for a logit of 16 bits, in the upper half of the result with `low` behind it, and back.  `u`: the
+// logit's bits in the upper half.
 template <int DT>
-__device__ __forceinline__ uint32_t order_key16(uint16_t u) {
-  constexpr uint32_t kInf = DT == MCCL_BF16 ? 0x7f80u : 0x7c00u;
-  const uint32_t size = u & 0x7fffu;
-  const uint32_t k = (u & 0x8000u) && size ? 0xffffu & ~(uint32_t)u : size | 0x8000u;
-  return size > kInf || u == (0x8000u | kInf) ? 0u : k;
+__device__ __forceinline__ uint32_t order_key16(uint32_t u, uint32_t low) {
+  constexpr uint32_t kInf = DT == MCCL_BF16 ? 0x7f800000u : 0x7c000000u;
+  uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+  k &= 0xffff0000u;
+  if (k == 0x7fff0000u) k = 0x80000000u;                                 // -0
+  constexpr uint32_t kLowest = 0xffff0000u & ~(0x80000000u | kInf);      // the key of -inf; NaNs lie below it and above +inf's
+  return k - kLowest - 1u < (0x80000000u | kInf) - kLowest ? k | low : 0u;
 }
 template <int DT>
-__device__ __forceinline__ float logit_of_key16(uint32_t k) {
-  return Elem<DT>::load((uint16_t)((k & 0x8000u) ? k & 0x7fffu : ~k));
+__device__ __forceinline__ float logit_of_key16(uint32_t key) {
+  const uint32_t u = (key & 0x80000000u) ? key ^ 0x80000000u : ~key;
+  if constexpr (DT == MCCL_BF16) return bits_to_f32(u & 0xffff0000u);
+  else return Elem<DT>::load((uint16_t)(u >> 16));
+}
+template <int DT>
+__device__ __forceinline__ uint32_t upper_half(float l) {  // of a value that is one of DT
+  if constexpr (DT == MCCL_BF16) return f32_to_bits(l);
+  else return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)l) << 16;
 }
 
 // A lane's PER logits of a row, from column `first` on; -inf behind the row.  Rows begin at any element: the
@@ -124,8 +134,7 @@ __global__ __launch_bounds__(kRouterWaves * kWave) void router_kernel(const Rout
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       if constexpr (kPacked) {
-        const uint32_t k = order_key16<DT>(Elem<DT>::store(l[j]));
-        key[j] = k ? k << 16 | (0xffffu - (member * PER + j)) : 0u;
+        key[j] = order_key16<DT>(upper_half<DT>(l[j]), 0xffffu - (member * PER + j));
       } else {
         key[j] = order_key(l[j]);
       }
@@ -145,7 +154,7 @@ __global__ __launch_bounds__(kRouterWaves * kWave) void router_kernel(const Rout
       float value;
       if constexpr (kPacked) {
         id = all ? (int32_t)(0xffffu - (all & 0xffffu)) : -1;
-        value = logit_of_key16<DT>(all >> 16);
+        value = logit_of_key16<DT>(all);
 #pragma unroll
         for (int j = 0; j < PER; ++j) key[j] = key[j] == all ? 0u : key[j];
       } else {
