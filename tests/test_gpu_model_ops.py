@@ -225,6 +225,22 @@ def test_embedding_grad_skips_what_a_foreign_plan_points_past(mccl):
     assert out[:, 0].tolist() == [1.0, 1.0]
 
 
+def test_embedding_grad_stays_inside_whatever_the_offsets_say(mccl):
+    """Offsets that fall, end early or point past the end: no row of the result depends on more than the
+    gradient (each is a sum of some of its rows, all ones here: at most their number)."""
+    n, rows, hidden = 700, 40, 24
+    grad = torch.ones(n, hidden, device=DEV)
+    order = torch.randperm(n, generator=gen(3)).to(DEV)
+    for seed in range(6):
+        offsets = torch.randint(-50, n + 200, (rows + 1,), generator=gen(4, seed))
+        if seed % 2:
+            offsets = torch.sort(offsets, descending=True).values
+        out = mccl.embedding_grad(grad, (order, offsets.to(DEV)), out=torch.zeros(rows, hidden, device=DEV))
+        assert out.shape == (rows, hidden)
+    good = mccl.embedding_grad(grad, mccl.sort_ids(torch.arange(n, device=DEV) % rows, rows))
+    assert good[:, 0].sum() == n
+
+
 # ---------------------------------------------------------------------------------------------
 # router
 # ---------------------------------------------------------------------------------------------
@@ -397,7 +413,7 @@ def layer_inputs(g, T, k, E, local, H, I, dtype):
 @pytest.mark.parametrize("T,k,E,local,first,H,I", [
     (1, 1, 1, 1, 0, 8, 8), (1, 8, 64, 64, 0, 256, 64), (2, 2, 4, 4, 0, 40, 24), (5, 3, 34, 34, 0, 520, 200), (16, 2, 3, 3, 0, 64, 128),
     (17, 1, 1, 1, 0, 72, 16), (31, 4, 16, 4, 8, 136, 88), (64, 2, 2, 2, 0, 32, 40), (3, 64, 70, 70, 0, 48, 16), (100, 6, 12, 5, 3, 264, 72),
-    (256, 2, 4, 4, 0, 96, 56), (7, 2, 40, 10, 20, 1032, 328), (33, 1, 2, 1, 1, 1024, 512), (2, 1, 300, 300, 0, 16, 2056)])
+    (256, 2, 4, 4, 0, 96, 56), (256, 8, 128, 128, 0, 64, 16), (256, 16, 300, 300, 0, 16, 8), (3, 2, 4, 4, 0, 4096, 72), (6, 4, 9, 9, 0, 7168, 8), (7, 2, 40, 10, 20, 1032, 328), (33, 1, 2, 1, 1, 1024, 512), (2, 1, 300, 300, 0, 16, 2056)])
 def test_moe_layer(mccl, dtype, activation, T, k, E, local, first, H, I):
     g = gen(T, k, E, H, I)
     x, w_in, w_out, ids, weights = layer_inputs(g, T, k, E, local, H, I, dtype)
@@ -580,6 +596,45 @@ def test_replayed_from_a_graph_on_a_stream_of_their_own(mccl):
             side.synchronize()
             for a, b in zip(held, got):
                 assert torch.equal(a, b)
+
+
+def test_two_streams_at_once_and_results_that_wait_for_each_other(mccl):
+    """Calls of different sizes on two streams at once, each with its own workspace from the allocator, give
+    what they give alone."""
+    g = gen(51)
+    layers = [[t.to(DEV) for t in layer_inputs(g, T, 4, 16, 16, 256, 128, torch.bfloat16)] for T in (3, 40)]
+    ids = [torch.randint(0, 500, (n,), generator=g).to(DEV) for n in (3000, 20000)]
+    ups = [torch.randn(len(i), 136, generator=g).to(DEV) for i in ids]
+    alone = [(mccl.moe_layer(*layers[k]), mccl.embedding_grad(ups[k], mccl.sort_ids(ids[k], 500))) for k in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((mccl.moe_layer(*layers[k]), mccl.embedding_grad(ups[k], mccl.sort_ids(ids[k], 500))))
+        torch.cuda.synchronize()
+        for a, b in zip(got, alone):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_results_go_where_the_caller_says(mccl):
+    """out tensors: the same object comes back, and only it is written."""
+    g = gen(52)
+    x, w_in, w_out, ids, weights = [t.to(DEV) for t in layer_inputs(g, 5, 2, 4, 4, 64, 40, torch.float16)]
+    out = torch.full((7, 64), 9.0, dtype=torch.float16, device=DEV)
+    assert mccl.moe_layer(x, w_in, w_out, ids, weights, out=out[1:6]).data_ptr() == out[1:6].data_ptr()
+    assert torch.equal(out[1:6], mccl.moe_layer(x, w_in, w_out, ids, weights)) and bool((out[0] == 9).all()) and bool((out[6] == 9).all())
+    logits = torch.randn(33, 70, generator=g).to(DEV)
+    held = (torch.full((35, 3), 77, dtype=torch.int32, device=DEV), torch.full((35, 3), 77.0, device=DEV))
+    a, b = mccl.moe_route(logits, 3, out=(held[0][1:34], held[1][1:34]))
+    want = mccl.moe_route(logits, 3)
+    assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+    for h in held:
+        assert bool((h[0] == 77).all()) and bool((h[34] == 77).all())
+    d = torch.full((35, 70), 5.0, device=DEV)
+    mccl.moe_route_grad(b.contiguous(), logits, a.contiguous(), out=d[1:34])
+    assert torch.equal(d[1:34], mccl.moe_route_grad(want[1], logits, want[0])) and bool((d[0] == 5).all()) and bool((d[34] == 5).all())
 
 
 def test_workspaces_of_the_caller_are_used_and_may_be_dirty(mccl):

@@ -611,7 +611,7 @@ __global__ __launch_bounds__(kGradWaves * kWave) void embedding_grad_kernel(cons
           write_partial<DT, VL, SHORT>(slot, c, acc);
         }
         if (last_long) {
-          sum_rows<DT, VL, SHORT>(a, index, last_begin - p0, p1 - p0, c, acc);
+          sum_rows<DT, VL, SHORT>(a, index, last_begin > p0 ? last_begin - p0 : 0, p1 - p0, c, acc);  // before p0 only if offsets fall
           write_partial<DT, VL, SHORT>(slot + a.hidden, c, acc);
         }
       }
