@@ -637,7 +637,9 @@ int mccl_moe_route_grad(const float* grad_weights, const void* logits, const int
  *   out[t] = sum_k weights[t][k] * w_out[e] . (act(w_in[e][0:inter] . x[t]) * (w_in[e][inter:2*inter] . x[t])),
  * e = expert_ids[t][k] - first_expert, over the k whose e lies in [0, experts), ascending k in fp32, one
  * rounding; a token without any gets zeros.  x, out: [tokens][hidden]; w_in: [experts][2 * inter][hidden];
- * w_out: [experts][hidden][inter]; bf16 or f16, hidden and inter multiples of 8, 16-byte aligned.
+ * w_out: [experts][hidden][inter]; bf16 or f16, hidden and inter multiples of 8 up to 2^17, 16-byte
+ * aligned, an expert's w_in at most 2 GiB - 64 KiB.  Sums and the activation are fp32; act(..) * (..) is
+ * rounded to the type once on its way into the second product (f16: infinite above 65504).
  * Every rank that holds `experts` experts from first_expert on calls it with all tokens, and an
  * all_reduce (SUM) adds the ranks' outputs.  At most 256 tokens, topk <= 64 and 4096 pairs: each
  * expert's weights are read once for all of its tokens.  The same bits every time.

@@ -126,6 +126,11 @@ def test_layer_refusals(abi):
     assert call(x=0x10000008) == -1 and "16-byte aligned" in err()
     assert call(w_out=0x200000002) == -1 and "16-byte aligned" in err()
     assert call(ids=0x20000002) == -1 and "misaligned" in err()
+    assert call(H=(1 << 17) + 8) == -1 and call(I=(1 << 17) + 8) == -1 and call(H=1 << 17, I=1 << 12) == -1 and "w_in above" in err()
+    assert call(H=1 << 14, I=1 << 15) == -1 and "w_in above" in err()  # 2 GiB
+    for sizes in ((0, 2, 8, 64, 32), (100, 0, 8, 64, 32), (100, 8, 0, 64, 32), (100, 8, 4, 0, 32), (100, 8, 4, 64, 0)):
+        assert L.mccl_moe_layer_workspace(*sizes) == 0
+    assert call(T=100, k=8, E=4, H=0) == 0 and call(T=100, k=8, E=4, I=0) == -3
     need = L.mccl_moe_layer_workspace(4, 2, 8, 64, 32)
     assert need > 0 and call(ws=0) == -1 and call(wsb=need - 1) == -1 and call(ws=0x40000008) == -1 and "workspace" in err()
     assert call(out=0x10000000) == -1 and "overlaps an input" in err()

@@ -1,6 +1,6 @@
 // Device-side building blocks shared by the kernels of libmi355ccl: geometry constants, the
 // 16-byte vector type, element traits (storage type, accumulation type, conversions) and the
-// reduction chain.  Header-only, included by exactly one translation unit (mccl_kernels.hip).
+// reduction chain.  Header-only, included by the translation units that hold kernels.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -82,9 +82,12 @@ __device__ __forceinline__ float from_neighbour(float v) {
 __device__ __forceinline__ f32x2 add_halves(f32x4 v) { return (f32x2){v[0] + from_neighbour(v[1]), v[2] + from_neighbour(v[3])}; }
 
 // Rows and tokens are read through buffer descriptors: the base is the same for all lanes, a lane has a
-// 32-bit offset, and an offset of kOutside reads zeros without touching memory, which is how columns that do
-// not exist are left out without a branch.
+// 32-bit offset, and an offset with kOutside added reads zeros without touching memory, which is how columns
+// that do not exist are left out without a branch.  A matrix and what the last turn of a loop asks for behind
+// it stay below kOutside, so that no sum of offsets passes 32 bits.
 constexpr uint32_t kOutside = 0x80000000u;
+constexpr size_t kLayerMaxColumns = 1u << 17;          // hidden and inter: 4096 pairs of h are 1 GiB
+constexpr size_t kLayerMaxExpert = kOutside - 65536u;  // bytes of an expert's w_in
 constexpr int kStreamed = 2;  // non-temporal: weights are read once
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t matrix_at(const char* base, uint32_t bytes) {
@@ -120,7 +123,7 @@ __device__ __forceinline__ void multiply_sets(__amdgpu_buffer_rsrc_t rows, const
 }
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t w_in_of(const LayerArgs& a, int e) {
-  const uint32_t bytes = 4 * a.inter * a.hidden;  // below 2 GiB
+  const uint32_t bytes = 4 * a.inter * a.hidden;  // at most kLayerMaxExpert
   return matrix_at(a.w_in + (size_t)e * bytes, bytes);
 }
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t w_out_of(const LayerArgs& a, int e) {
@@ -284,14 +287,6 @@ __device__ __forceinline__ void layer_out_tokens(const LayerArgs& a, int e, uint
       if (lane_holds() && m0 + t * 8 + r < m)
         *(f32x2*)(y + (((size_t)list[m0 + t * 8 + r] * a.parts + part) * NW + n) * kSetRows + lane_row()) = v;
     }
-}
-
-template <int DT, int NW>
-__device__ __forceinline__ void layer_out_expert(const LayerArgs& a, int e, uint32_t c0, uint32_t part, const uint16_t* list, uint32_t m, float* y) {
-  uint32_t m0 = 0;
-  for (; m0 < m && m - m0 > 16; m0 += 32) layer_out_tokens<DT, NW, 4, 2>(a, e, c0, part, list, m0, m, y);
-  for (; m0 < m && m - m0 > 8; m0 += 16) layer_out_tokens<DT, NW, 2, 4>(a, e, c0, part, list, m0, m, y);
-  for (; m0 < m; m0 += 8) layer_out_tokens<DT, NW, 1, 8 / NW>(a, e, c0, part, list, m0, m, y);
 }
 
 template <int DT, int NW, int WAVES>

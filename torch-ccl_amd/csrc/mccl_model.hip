@@ -411,7 +411,7 @@ int mccl_moe_route_grad(const float* grad_weights, const void* logits, const int
 }
 
 size_t mccl_moe_layer_workspace(size_t tokens, int topk, size_t experts, size_t hidden, size_t inter) {
-  if (topk < 1 || tokens == 0 || experts == 0) return 0;
+  if (topk < 1 || tokens == 0 || experts == 0 || hidden == 0 || inter == 0) return 0;
   return plan_layer(tokens, tokens * (size_t)topk, experts, hidden, inter).bytes;
 }
 
@@ -428,8 +428,8 @@ int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int
     return mccl_report_error(MCCL_ERR_INVALID_ARG, "expert count %zu outside [1, %d]", experts, kRouterMaxExperts);
   if (tokens == 0 || hidden == 0) return MCCL_OK;
   if (hidden % 8 || inter % 8 || inter == 0) return mccl_report_error(MCCL_ERR_UNSUPPORTED, "moe_layer needs hidden and inter that are multiples of 8");
-  if (hidden > (1u << 18) || inter > (1u << 18) || 4 * inter * hidden > 0x7fffffffull)
-    return mccl_report_error(MCCL_ERR_INVALID_ARG, "hidden or inter too large: an expert's w_in has to be below 2 GiB");
+  if (hidden > kLayerMaxColumns || inter > kLayerMaxColumns || 4 * inter * hidden > kLayerMaxExpert)
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "hidden or inter above %zu, or an expert's w_in above %zu bytes", kLayerMaxColumns, kLayerMaxExpert);
   if (!x || !w_in || !w_out || !expert_ids || !weights || !out) return mccl_report_error(MCCL_ERR_INVALID_ARG, "null pointer");
   if (misaligned(x, 16) || misaligned(w_in, 16) || misaligned(w_out, 16) || misaligned(out, 16))
     return mccl_report_error(MCCL_ERR_INVALID_ARG, "x, the weights or the output are not 16-byte aligned");
