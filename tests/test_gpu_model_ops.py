@@ -158,7 +158,8 @@ def grad_reference(grad, ids, first, rows, scale):
 @pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float16),
                                              (torch.float16, torch.float32), (torch.float32, torch.float32)], ids=str)
 @pytest.mark.parametrize("n,rows,hidden,hot", [(0, 5, 16, 0.0), (1, 1, 1, 0.0), (64, 3, 40, 1.0), (65, 3, 40, 1.0), (128, 2, 7, 0.5),
-                                               (1000, 40, 521, 0.6), (3000, 500, 264, 0.2), (700, 20, 2056, 0.3), (9000, 7, 130, 0.0)])
+                                               (1000, 40, 521, 0.6), (3000, 500, 264, 0.2), (700, 20, 2056, 0.3), (9000, 7, 130, 0.0),
+                                               (9000, 7000, 2056, 0.1)])
 @pytest.mark.parametrize("accumulate", [False, True])
 def test_embedding_grad(mccl, dtype, out_dtype, n, rows, hidden, hot, accumulate):
     """Rows without a token, with one, with more than one piece of the sorted tokens holds, and rows that

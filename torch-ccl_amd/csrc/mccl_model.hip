@@ -18,6 +18,7 @@ namespace {
 constexpr size_t kMaxHidden = 1u << 23;       // grids of at most 65535 column chunks
 constexpr size_t kMaxGradTokens = 1u << 28;   // and of at most 2^32 threads along their first axis
 constexpr uint32_t kMaxGroups = 1u << 23;     // rows and tokens beyond that walk the grid
+constexpr uint32_t kMaxSmallGroups = 512;     // of the sort of few ids
 
 size_t float_size(int dtype) {
   return dtype == MCCL_F32 ? 4 : (dtype == MCCL_BF16 || dtype == MCCL_F16) ? 2 : 0;
@@ -61,11 +62,13 @@ SortPlan plan_sort(size_t n) {
 
 template <typename ID>
 int launch_sort(const ID* ids, size_t n, int64_t first_row, size_t rows, char* ws, int64_t* order, int64_t* offsets, hipStream_t s) {
-  const unsigned offset_groups = (unsigned)((rows + 1 + kSortBlock - 1) / kSortBlock);
   if (n <= (size_t)kSortSmall) {
-    const unsigned rank_groups = (unsigned)((n + kSortBlock - 1) / kSortBlock);
-    hipLaunchKernelGGL(sort_small_kernel<ID>, dim3(rank_groups + offset_groups), dim3(kSortBlock), 0, s, ids, (uint32_t)n, first_row,
-                       (uint32_t)rows, rank_groups, order, offsets);
+    const unsigned rank_groups = (unsigned)((n + kWave - 1) / kWave), groups = rank_groups + (unsigned)(rows / kWave + 1);
+    // 4 wavefronts share the keys, or 8 (16 ids over 32000 rows 3.5 us against 5.3, 512 over 60000 8.1 against 8.3,
+    // 1000 over 900 6.3 against 4.7)
+    const unsigned waves = n <= 512 ? 4 : 8;
+    hipLaunchKernelGGL((waves == 4 ? sort_small_kernel<ID, 4> : sort_small_kernel<ID, 8>), dim3(std::min(groups, kMaxSmallGroups)),
+                       dim3(waves * kWave), 0, s, ids, (uint32_t)n, first_row, (uint32_t)rows, rank_groups, groups, order, offsets);
     return launched("sort");
   }
   const SortPlan p = plan_sort(n);
@@ -100,7 +103,7 @@ int launch_sort(const ID* ids, size_t n, int64_t first_row, size_t rows, char* w
   }
   uint32_t every_log2 = 0;
   while (((a.n - 1) >> every_log2) + 1 > kSortSamples) ++every_log2;
-  hipLaunchKernelGGL(sort_offsets_kernel, dim3(offset_groups), dim3(kSortBlock), 0, s, a.key_out, a.n, every_log2, a.rows, offsets);
+  hipLaunchKernelGGL(sort_offsets_kernel, dim3((unsigned)(rows / kSortBlock + 1)), dim3(kSortBlock), 0, s, a.key_out, a.n, every_log2, a.rows, offsets);
   return launched("sort");
 }
 
@@ -114,21 +117,28 @@ void launch_embedding(const EmbeddingArgs& a, int id_dtype, hipStream_t s) {
   hipLaunchKernelGGL(kernel, grid, block, 0, s, a);
 }
 
+// Below so many (row or piece, chunk of columns) pairs a wavefront has one pair and a row's chunks are spread over
+// workgroups: then the time is that of the longest chain of loads (2000 tokens into 2000 x 7168 bf16 24 us
+// against 38, 1500 into 600 x 4096 15 against 20).  From about there on it makes no difference (8192 tokens into
+// 3000 x 4096 28 us both ways), and one wavefront takes two chunks, which halves the loads of indices.
+constexpr uint32_t kGradSpread = 32768;
 size_t grad_pieces(size_t n) { return n > (size_t)kGradPiece ? (n + kGradPiece - 1) / kGradPiece : 0; }
 
 template <int DT, int OUT>
 void launch_embedding_grad(EmbeddingGradArgs a, hipStream_t s) {
   constexpr uint32_t kChunk = kWave * vec_elems<DT>();
   const bool narrow = a.hidden < (uint32_t)vec_elems<DT>();
-  const uint32_t chunks = (a.hidden + kChunk - 1) / kChunk;
-  const uint32_t units = chunks > 4 ? (chunks + 1) / 2 : chunks;  // of one wavefront: two chunks where there are many
+  const uint32_t chunks = (a.hidden + kChunk - 1) / kChunk, pieces = (uint32_t)grad_pieces(a.n);
+  const bool spread = (uint64_t)(std::min(a.rows, a.n) + pieces) * chunks < kGradSpread;
+  const bool pairs = chunks > 4 && !spread;
+  const uint32_t units = pairs ? (chunks + 1) / 2 : chunks;  // of one wavefront
   a.sharing_log2 = units >= 4 ? 2 : units >= 2 ? 1 : 0;
   const uint32_t per_group = kGradWaves >> a.sharing_log2;
-  const uint32_t pieces = (uint32_t)grad_pieces(a.n);
+  a.column_groups = spread ? (units + (1u << a.sharing_log2) - 1) >> a.sharing_log2 : 1;
   a.piece_groups = (pieces + per_group - 1) / per_group;
-  const uint32_t row_groups = std::min(kMaxGroups, (a.rows + per_group - 1) / per_group);
-  auto kernel = narrow ? embedding_grad_kernel<DT, OUT, 1, true> : chunks > 4 ? embedding_grad_kernel<DT, OUT, 2, false> : embedding_grad_kernel<DT, OUT, 1, false>;
-  hipLaunchKernelGGL(kernel, dim3(a.piece_groups + row_groups), dim3(kGradWaves * kWave), 0, s, a);
+  a.row_groups = std::min(kMaxGroups, (a.rows + per_group - 1) / per_group);
+  auto kernel = narrow ? embedding_grad_kernel<DT, OUT, 1, true> : pairs ? embedding_grad_kernel<DT, OUT, 2, false> : embedding_grad_kernel<DT, OUT, 1, false>;
+  hipLaunchKernelGGL(kernel, dim3(a.piece_groups + a.row_groups, a.column_groups), dim3(kGradWaves * kWave), 0, s, a);
   auto join = narrow ? embedding_grad_join_kernel<DT, OUT, true> : embedding_grad_join_kernel<DT, OUT, false>;
   if (pieces) hipLaunchKernelGGL(join, dim3(pieces, chunks), dim3(kJoinWaves * kWave), 0, s, a);
 }
