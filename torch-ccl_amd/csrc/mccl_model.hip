@@ -129,7 +129,7 @@ void launch_embedding_grad(EmbeddingGradArgs a, hipStream_t s) {
   constexpr uint32_t kChunk = kWave * vec_elems<DT>();
   const bool narrow = a.hidden < (uint32_t)vec_elems<DT>();
   const uint32_t chunks = (a.hidden + kChunk - 1) / kChunk, pieces = (uint32_t)grad_pieces(a.n);
-  const bool spread = (uint64_t)(std::min(a.rows, a.n) + pieces) * chunks < kGradSpread;
+  const bool spread = ((uint64_t)a.rows + pieces) * chunks < kGradSpread;
   const bool pairs = chunks > 4 && !spread;
   const uint32_t units = pairs ? (chunks + 1) / 2 : chunks;  // of one wavefront
   a.sharing_log2 = units >= 4 ? 2 : units >= 2 ? 1 : 0;
@@ -190,7 +190,12 @@ struct LayerPlan {
   size_t h_bytes, bytes;
 };
 
-constexpr size_t kDensePairs = 16;  // per expert
+// Pairs per expert above which the tokens go through LDS (layer_dense_kernel) instead of being read again by every
+// workgroup.  Both ways, tokens spread evenly: 8 experts of 4096 x 1792 with 8 / 16 / 24 / 32 / 48 pairs each
+// 62 / 74 / 81 / 117 / 157 us from memory and 72 / 76 / 79 / 82 / 88 through LDS; 32 experts of 2048 x 768 with
+// 8 / 16 / 24 / 32 pairs 61 / 76 / 95 / 125 and 75 / 81 / 87 / 91; 2 experts of 4096 x 8192 with 8 / 16 / 24 / 48
+// pairs 77 / 81 / 105 / 171 and 87 / 88 / 90 / 97.  Uneven routing moves the crossing down.
+constexpr size_t kDensePairs = 16;
 LayerPlan plan_layer(size_t tokens, size_t pairs, size_t experts, size_t hidden, size_t inter) {
   LayerPlan p{};
   if (pairs > kDensePairs * experts || pairs > kFewMaxPairs)
@@ -204,9 +209,10 @@ LayerPlan plan_layer(size_t tokens, size_t pairs, size_t experts, size_t hidden,
     p.parts = (uint32_t)((chunks + per - 1) / per);
     p.bytes += p.parts * pairs * hidden * sizeof(float);
   } else {
-    // as many parts as give 8 wavefronts something to do; more only add joining (5 tokens x 3 experts, inter 200:
-    // 10.9 us with one part, 12.7 with two)
-    p.parts = (uint32_t)std::min<size_t>((inter + kStepCols - 1) / kStepCols, std::max<size_t>(1, 8 / pairs));
+    // as many parts as give 16 wavefronts something to do, of 4 steps or more: where few experts can be chosen,
+    // wavefronts would have nothing to do (8 tokens on one of 2 experts of 14336: 60 us against 88 with one part),
+    // while parts of few steps only add joining (5 tokens x 3 experts, inter 200: 9.0 against 12.7)
+    p.parts = (uint32_t)std::max<size_t>(1, std::min<size_t>((inter + kStepCols - 1) / kStepCols / 4, 16 / std::min(pairs, experts)));
   }
   return p;
 }
