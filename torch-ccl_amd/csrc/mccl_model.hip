@@ -185,7 +185,7 @@ int check_router(size_t tokens, size_t experts, int topk, int dtype) {
 
 // How a layer is run, from its sizes alone (the routing is only known on the device).
 struct LayerPlan {
-  int dense;       // tokens of a tile of layer_dense_kernel, 0: few tokens per expert
+  int dense;       // tokens of a tile of layer_dense_kernel, 0: layer_in_kernel and layer_out_kernel
   uint32_t parts;  // of inter, in the second product
   size_t h_bytes, bytes;
 };
@@ -196,10 +196,15 @@ struct LayerPlan {
 // 8 / 16 / 24 / 32 pairs 61 / 76 / 95 / 125 and 75 / 81 / 87 / 91; 2 experts of 4096 x 8192 with 8 / 16 / 24 / 48
 // pairs 77 / 81 / 105 / 171 and 87 / 88 / 90 / 97.  Uneven routing moves the crossing down.
 constexpr size_t kDensePairs = 16;
+// And above which a tile has 128 tokens instead of 64.  An expert with more than a tile reads its weights again (64
+// pairs and more each: 2 experts of 4096 x 8192, 96 pairs each, 117 us with 128 and 175 with 64); with less the
+// smaller tile is 2 to 5 percent faster (48 pairs 96 against 100).  Uneven routing puts some experts over 64 from
+// an average of 32 on (160 tokens on 8 experts of 4096 x 7168, 40 each, 306 us against 318).
+constexpr size_t kWideTilePairs = 32;
 LayerPlan plan_layer(size_t tokens, size_t pairs, size_t experts, size_t hidden, size_t inter) {
   LayerPlan p{};
   if (pairs > kDensePairs * experts || pairs > kFewMaxPairs)
-    p.dense = tokens <= 32 ? 32 : (tokens <= 64 || pairs <= 48 * experts) ? 64 : 128;
+    p.dense = (tokens <= 64 || pairs <= kWideTilePairs * experts) ? 64 : 128;
   p.h_bytes = up16(pairs * inter * 2);
   p.bytes = p.h_bytes;
   if (p.dense) {
@@ -248,8 +253,10 @@ int launch_layer_out(const LayerArgs& a, hipStream_t s) {
 
 template <int DT>
 int launch_layer(const LayerArgs& a, int dense, hipStream_t s) {
-  if (dense) return dense == 32 ? launch_dense<DT, 32>(a, s) : dense == 64 ? launch_dense<DT, 64>(a, s) : launch_dense<DT, 128>(a, s);
+  if (dense) return dense == 64 ? launch_dense<DT, 64>(a, s) : launch_dense<DT, 128>(a, s);
   const dim3 in_grid((a.inter + kInRows - 1) / kInRows, a.by_pair ? a.pairs : a.experts), in_block(kInWaves * kWave);
+  // the fewest sums that serve all tokens of an expert at once (58 tokens, 15 on each of 23 experts of 4016 x 624: 111 us
+  // with sums for 32 tokens, 137 for 16; 64 tokens, 4 on each of 128: 302 and 310)
   if (a.tokens <= 8) hipLaunchKernelGGL((layer_in_kernel<DT, 8>), in_grid, in_block, 0, s, a);
   else if (a.tokens <= 16) hipLaunchKernelGGL((layer_in_kernel<DT, 16>), in_grid, in_block, 0, s, a);
   else hipLaunchKernelGGL((layer_in_kernel<DT, 32>), in_grid, in_block, 0, s, a);
