@@ -145,18 +145,23 @@ __global__ __launch_bounds__(kRouterWaves * kWave) void router_kernel(const Rout
     int32_t my_id[kKept];
 #pragma unroll
     for (int x = 0; x < kKept; ++x) { my_id[x] = -1; my_logit[x] = 0.0f; }
+    uint32_t all = 0;  // the key of the last choice
     for (uint32_t k = 0; k < a.topk; ++k) {
-      uint32_t best = key[0];
+      // Packed keys are distinct: the next is the largest key below the last, which is the largest difference to it,
+      // as those not below it do not wrap.  (all = 0 at first: the largest key.)
+      uint32_t best = kPacked ? key[0] - all : key[0];
 #pragma unroll
-      for (int j = 1; j < PER; ++j) best = key[j] > best ? key[j] : best;
-      const uint32_t all = group_max<LANES>(best);
+      for (int j = 1; j < PER; ++j) {
+        const uint32_t next = kPacked ? key[j] - all : key[j];
+        best = next > best ? next : best;
+      }
+      const uint32_t largest = group_max<LANES>(best) + (kPacked ? all : 0u);
+      all = !kPacked || k == 0 || largest < all ? largest : 0u;
       int32_t id;
       float value;
       if constexpr (kPacked) {
         id = all ? (int32_t)(0xffffu - (all & 0xffffu)) : -1;
         value = logit_of_key16<DT>(all);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) key[j] = key[j] == all ? 0u : key[j];
       } else {
         int at = 0;
 #pragma unroll
