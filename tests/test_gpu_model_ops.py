@@ -113,7 +113,7 @@ def test_embedding_rows_past_4_gib(mccl):
 # ---------------------------------------------------------------------------------------------
 # sort
 # ---------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("n", [0, 1, 2, 64, 255, 256, 257, 2047, 2048, 2049, 4096, 5000, 65537, 1_000_003])
+@pytest.mark.parametrize("n", [0, 1, 2, 64, 255, 256, 257, 2047, 2048, 2049, 4096, 5000, 65537, 196_608, 196_609, 1_000_003])
 @pytest.mark.parametrize("rows,first", [(1, 0), (8, -2), (255, 0), (256, 1), (50_000, 10), (3_000_000, 0)])
 def test_sort_ids_is_the_stable_order(mccl, n, rows, first):
     g = gen(n, rows)

@@ -161,7 +161,14 @@ __device__ __forceinline__ uint32_t list_pairs(const int16_t* expert, uint32_t p
 // ------------------------------------------------------------------------------------------
 // h[pair][i] = act(w_in[e][i] . x[t]) * (w_in[e][inter + i] . x[t])
 // ------------------------------------------------------------------------------------------
-// A workgroup takes 16 gate rows and their 16 up rows of one expert; its wavefronts share the columns.
+// A workgroup takes 16 gate rows and their 16 up rows of one expert; its wavefronts share the columns, in fp32 until
+// the gate is applied.  h is then rounded once to the layer's type, which the second product's matrix
+// instructions take: against 64 bits the result is off by 1.4 times its own last rounding (0.0024 in bf16) and
+// would be by 1.0 with h in fp32, for twice the second product's instructions and h's reads.
+// Bound by reading the weights: 15.7 experts of 7168 x 2048, 32 tokens, 132 us, 7.0 TB/s; 8 experts of 4096 x 1024,
+// 1 token, 23 us, 5.9 TB/s (a workgroup reads 256 KiB there, and its start and end are a fifth of its time).
+// 8 and 16 wavefronts a workgroup, two halves of the loads in turns, and 4 workgroups a compute unit by fewer registers
+// are no faster (1 token 36.0, 37.8, 36.4 and 36.0 us for the layer; 32 tokens 214, 228, 230 and 225 against 211).
 constexpr int kInWaves = 4;
 constexpr int kInRows = 2 * kSetRows;
 
@@ -240,7 +247,9 @@ __global__ __launch_bounds__(kInWaves * kWave) void layer_in_kernel(const LayerA
 // ------------------------------------------------------------------------------------------
 // A workgroup takes kSetRows * NW rows of w_out of every expert that was chosen and keeps the products of
 // all pairs in LDS, so that the weighted sum needs no other workgroup: work of a wavefront is an expert
-// and one of a.parts parts of inter.
+// and one of a.parts parts of inter.  Sums in fp32, the pairs of a token in ascending order, one rounding.
+// Bound by reading the weights: 15.7 experts of 7168 x 2048, 32 tokens, 74 us, 6.3 TB/s; 8 of 4096 x 1024, 1 token,
+// 14 us, 4.7 TB/s; below some 20 MB by its chain: ids, lists, h, products, sums (3 experts of 520 x 200 5.5 us).
 struct LayerOutLds {
   uint32_t weights, first, active, lists, y, bytes;
 };
@@ -356,6 +365,11 @@ __global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArg
 // product: 64 gate rows and their up rows) or one part of inter (second product: 128 rows).  Its tokens go
 // through LDS, a chunk of columns of TOKENS of them at a time.  While a chunk is multiplied, the rows and
 // tokens of the next one are on their way into registers.
+// 160 tokens on 8 experts of 4096 x 7168, 40 each: 206 us for the first product (4.6 TB/s, 183 TFLOP/s) and 99 for
+// the second.  A workgroup reads at the memory's rate once it runs; what is lost is its start, its end and the last
+// round of workgroups, which not all compute units have (448 tiles of the first product on 256 units that hold one
+// or two each).  A workgroup that goes on to its next tile by itself, loads three chunks ahead, and 4 wavefronts
+// instead of 8 were slower.
 constexpr int kDenseWaves = 8;
 constexpr int kDenseBlock = kDenseWaves * kWave;
 constexpr uint32_t kDenseInRows = kDenseWaves * kSetRows, kDenseOutRows = 2 * kDenseInRows;
@@ -489,7 +503,8 @@ __global__ __launch_bounds__(kDenseBlock, 2) void layer_dense_kernel(const Layer
   }
 }
 
-// out[t] = sum_k weights[t][k] * (sum over the parts of y[t * topk + k]), ascending.
+// out[t] = sum_k weights[t][k] * (sum over the parts of y[t * topk + k]), ascending.  y comes from the caches: 160 tokens
+// x 2 x 4096 5 us, two thirds of it the launch and the ids.
 template <int DT>
 __global__ __launch_bounds__(256) void layer_join_kernel(const LayerArgs a) {
   using S = typename Elem<DT>::store_t;

@@ -150,21 +150,24 @@ void launch_route(const RouterArgs& a, hipStream_t s) {
                      dim3(std::min(kMaxGroups, (a.tokens + per_group - 1) / per_group)), dim3(kRouterWaves * kWave), 0, s, a);
 }
 
-// Up to 256 experts a batch takes 16 lanes per token, of 16 experts at most: 32768 tokens x 256 experts 16 us
-// and 9.9 for the gradient, against 25 and 11 with a wavefront per token; x 64 experts 7.4 and 5.3 against 16
-// and 8.5.  Few tokens are bound by one wavefront's time, which is shorter where it has one token and less
-// per lane: 256 tokens x 256 experts 3.4 us against 4.8.  They meet between 2048 (4.0 against 4.9) and 8192
-// tokens (x 128 experts 4.4 against 3.8).
+// A batch takes 16 lanes per token, of 16 experts at most: 32768 tokens x 256 experts bf16 11.6 us and 10.1 for the
+// gradient, against 18.7 and 11.9 with a wavefront per token; x 64 experts 6.3 and 5.3 against 13.7 and 8.4.  Few
+// tokens are bound by one wavefront's time, which is shorter where it has one token and less per lane: 256 tokens x
+// 256 experts 3.3 us against 3.9.  They meet at 4096 tokens (4.2 against 4.6, the gradient 4.0 against 3.7; 2048
+// tokens 4.0 against 3.7; x 128 experts 3.3 against 3.5).  16 experts of fp32 are a cache line's half per lane, which
+// the gradient, reading and writing them, does slower than a wavefront per token: 32768 x 256 18.7 us against 14.5
+// (x 128 9.1 against 11.5).
 constexpr uint32_t kRouterBatch = 4096;
 
 template <int DT, bool GRAD>
 void launch_router(const RouterArgs& a, hipStream_t s) {
-  if (a.tokens >= kRouterBatch && a.experts <= 16 * 16) {
+  constexpr bool kSixteen = !(GRAD && DT == MCCL_F32);  // experts per lane of 16 lanes, or at most 8
+  if (a.tokens >= kRouterBatch && a.experts <= 16 * (kSixteen ? 16 : 8)) {
     if (a.experts <= 16) launch_route<DT, GRAD, 16, 1>(a, s);
     else if (a.experts <= 32) launch_route<DT, GRAD, 16, 2>(a, s);
     else if (a.experts <= 64) launch_route<DT, GRAD, 16, 4>(a, s);
     else if (a.experts <= 128) launch_route<DT, GRAD, 16, 8>(a, s);
-    else launch_route<DT, GRAD, 16, 16>(a, s);
+    else if constexpr (kSixteen) launch_route<DT, GRAD, 16, 16>(a, s);
   } else if (a.experts <= 64) launch_route<DT, GRAD, 64, 1>(a, s);
   else if (a.experts <= 128) launch_route<DT, GRAD, 64, 2>(a, s);
   else if (a.experts <= 256) launch_route<DT, GRAD, 64, 4>(a, s);

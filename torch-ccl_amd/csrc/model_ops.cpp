@@ -1,7 +1,7 @@
 // Tensor front end of the operators that compute around the collectives (embedding, router,
 // mixture-of-experts layer): checks, output and workspace allocation, and the call of the C ABI on the
 // current stream of the tensors' device.  In C++ because these calls are short: an interpreter's share of a
-// decode step's layer, 14 us of host time, was more than its kernels' 11.
+// decode step's layer, 14 us of host time, was more than its kernels' 10.
 #include "model_ops.hpp"
 
 #include <ATen/ATen.h>
