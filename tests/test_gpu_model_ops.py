@@ -619,6 +619,36 @@ def test_two_streams_at_once_and_results_that_wait_for_each_other(mccl):
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def test_layer_with_most_pairs_replays_from_a_graph(mccl):
+    """2048 pairs over many experts: more LDS than a kernel has by default, also under capture."""
+    tensors = [t.to(DEV) for t in layer_inputs(gen(53), 256, 8, 200, 200, 64, 32, torch.bfloat16)]
+    alone = mccl.moe_layer(*tensors)
+    out = torch.zeros_like(alone)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mccl.moe_layer(*tensors, out=out)
+    for _ in range(3):
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, alone)
+        assert torch.equal(mccl.moe_layer(*tensors), alone)
+
+
+def test_views_that_are_not_contiguous_are_refused(mccl):
+    table, ids = torch.zeros(16, 32, device=DEV), torch.zeros(8, dtype=torch.int64, device=DEV)
+    for call in (lambda: mccl.embedding(table[:, ::2], ids), lambda: mccl.embedding(table, ids[::2]), lambda: mccl.sort_ids(ids[::2], 4),
+                 lambda: mccl.embedding_grad(table[::2], mccl.sort_ids(ids, 4)), lambda: mccl.moe_route(table.t(), 2),
+                 lambda: mccl.moe_route(table, 2, out=(torch.zeros(16, 4, dtype=torch.int32, device=DEV)[:, ::2], None))):
+        with pytest.raises(RuntimeError, match="contiguous"):
+            call()
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        mccl.embedding(table, ids.cpu())
+    big = torch.zeros(5000, dtype=torch.int64, device=DEV)
+    with pytest.raises(RuntimeError, match="workspace must be"):
+        mccl.sort_ids(big, 4, workspace=torch.zeros(16, dtype=torch.uint8, device=DEV))
+
+
 def test_results_go_where_the_caller_says(mccl):
     """out tensors: the same object comes back, and only it is written."""
     g = gen(52)

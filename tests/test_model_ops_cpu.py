@@ -128,6 +128,7 @@ def test_layer_refusals(abi):
     assert call(ids=0x20000002) == -1 and "misaligned" in err()
     assert call(H=(1 << 17) + 8) == -1 and call(I=(1 << 17) + 8) == -1 and call(H=1 << 17, I=1 << 12) == -1 and "w_in above" in err()
     assert call(H=1 << 14, I=1 << 15) == -1 and "w_in above" in err()  # 2 GiB
+    assert call(T=256, k=16, E=4096, H=8, I=1 << 17) == -1 and "too many rows" in err()
     for sizes in ((0, 2, 8, 64, 32), (100, 0, 8, 64, 32), (100, 8, 0, 64, 32), (100, 8, 4, 0, 32), (100, 8, 4, 64, 0)):
         assert L.mccl_moe_layer_workspace(*sizes) == 0
     assert call(T=100, k=8, E=4, H=0) == 0 and call(T=100, k=8, E=4, I=0) == -3

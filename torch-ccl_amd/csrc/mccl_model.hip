@@ -18,6 +18,7 @@ namespace {
 constexpr size_t kMaxHidden = 1u << 23;       // grids of at most 65535 column chunks
 constexpr size_t kMaxGradTokens = 1u << 28;   // and of at most 2^32 threads along their first axis
 constexpr uint32_t kMaxGroups = 1u << 23;     // rows and tokens beyond that walk the grid
+constexpr size_t kMaxDenseTiles = 1u << 22;   // of layer_dense_kernel, 512 threads each
 constexpr uint32_t kMaxSmallGroups = 512;     // of the sort of few ids
 
 size_t float_size(int dtype) {
@@ -462,6 +463,8 @@ int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int
   if (misaligned(expert_ids, 4) || misaligned(weights, 4)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "expert ids or weights misaligned");
   const size_t pairs = tokens * (size_t)topk, row = tokens * hidden * 2;
   const LayerPlan plan = plan_layer(tokens, pairs, experts, hidden, inter);
+  if (plan.dense && std::max((inter + kDenseInRows - 1) / kDenseInRows, (hidden + kDenseOutRows - 1) / kDenseOutRows * plan.parts) * experts > kMaxDenseTiles)
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "%zu experts of %zu x %zu are too many rows for one launch", experts, hidden, inter);
   const size_t need = plan.bytes;
   if (!workspace || misaligned(workspace, 16) || workspace_bytes < need)
     return mccl_report_error(MCCL_ERR_INVALID_ARG, "workspace is null, not 16-byte aligned or smaller than %zu bytes", need);
