@@ -374,13 +374,27 @@ constexpr int kDenseWaves = 8;
 constexpr int kDenseBlock = kDenseWaves * kWave;
 constexpr uint32_t kDenseInRows = kDenseWaves * kSetRows, kDenseOutRows = 2 * kDenseInRows;
 
+// With 16 tokens to a product the matrix instruction is used in full: its 16 rows are the wavefront's two sets of 8,
+// the even ones of the first.  The rows are still loaded by lane pairs, 128 bytes of each, of which a lane has one
+// 16-byte piece of a row of either set; the pair exchanges what the other's row needs, and each has two pieces of one
+// row: columns of two products.
+__device__ __forceinline__ void exchange_sets(const u32x4& first, const u32x4& second, u32x4& even, u32x4& odd) {
+  const bool takes_first = threadIdx.x % 2 == 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t got = f32_to_bits(from_neighbour(bits_to_f32(takes_first ? second[i] : first[i])));
+    even[i] = takes_first ? first[i] : got;
+    odd[i] = takes_first ? got : second[i];
+  }
+}
+
 // Steps of columns in a chunk: as many as the registers have room for beside the sums of TOKENS tokens.
-constexpr int dense_steps(int tokens) { return tokens > 64 ? 2 : 4; }
+constexpr int dense_steps(int tokens) { return 2; }
 // Tokens that one thread stages a 16-byte piece of.
 constexpr int dense_share(int tokens) { return tokens * dense_steps(tokens) * 8 / kDenseBlock; }
 
 template <int DT, int TOKENS, bool IN>
-__global__ __launch_bounds__(kDenseBlock, 2) void layer_dense_kernel(const LayerArgs a) {
+__global__ __launch_bounds__(kDenseBlock, 4) void layer_dense_kernel(const LayerArgs a) {
   using S = typename Elem<DT>::store_t;
   constexpr int kSteps = dense_steps(TOKENS), kPieces = kSteps * 8, kShare = dense_share(TOKENS), kStaged = kDenseBlock / kPieces;
   constexpr uint32_t kCols = kSteps * kStepCols, kRowBytes = kCols * 2;
@@ -418,8 +432,9 @@ __global__ __launch_bounds__(kDenseBlock, 2) void layer_dense_kernel(const Layer
   // the 8 tokens which a load from LDS takes at the same columns lie in different banks.
   const __amdgpu_buffer_rsrc_t tokens = IN ? matrix_at(a.x, a.tokens * a.hidden * 2) : matrix_at(a.h, a.pairs * a.inter * 2);
   const uint32_t piece = threadIdx.x % kPieces, staged = threadIdx.x / kPieces;
-  const uint32_t put = staged * kRowBytes + (piece / 8) * 128 + ((piece ^ (staged * 2)) % 8) * 16;
-  const uint32_t get = r * kRowBytes + ((col / 8) ^ (r * 2 % 8)) * 16;
+  const uint32_t put = staged * kRowBytes + (piece / 8) * 128 + ((piece ^ staged) % 8) * 16;
+  const uint32_t token = threadIdx.x % 16;  // of 16, where the sums are too
+  const uint32_t get = token * kRowBytes + ((threadIdx.x % kWave / 16 * 2) ^ (token % 8)) * 16;  // its neighbour piece: ^ 16
 
   u32x4 wv[2][kSteps][2], tv[kShare];
   stage_experts(a, expert);
@@ -438,11 +453,9 @@ __global__ __launch_bounds__(kDenseBlock, 2) void layer_dense_kernel(const Layer
 #pragma unroll
       for (int i = 0; i < kShare; ++i) tv[i] = __builtin_amdgcn_raw_buffer_load_b128(tokens, from[i] | out, k * 2, 0);
     };
-    f32x4 acc[2][TOKENS / 8];
+    f32x4 acc[TOKENS / 16];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int g = 0; g < TOKENS / 8; ++g) acc[n][g] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int g = 0; g < TOKENS / 16; ++g) acc[g] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     const auto stage = [&]() {
       char* buf = space + (turns & 1) * (TOKENS * kRowBytes);
 #pragma unroll
@@ -450,22 +463,23 @@ __global__ __launch_bounds__(kDenseBlock, 2) void layer_dense_kernel(const Layer
       __syncthreads();
     };
     const auto product = [&](const u32x4(&v)[kSteps][2]) {
-      const char* buf = space + (turns & 1) * (TOKENS * kRowBytes) + get;
+      const char* buf = space + (turns & 1) * (TOKENS * kRowBytes);
       __builtin_amdgcn_sched_barrier(0);  // the loads go first
+      u32x4 rows_of[kSteps][2];
 #pragma unroll
-      for (int g = 0; g < TOKENS / 8; g += 2) {  // 16 tokens: as many loads from LDS in flight
-        if (g * 8u >= used) break;
-        u32x4 b[2][kSteps];
+      for (int u = 0; u < kSteps; ++u) exchange_sets(v[u][0], v[u][1], rows_of[u][0], rows_of[u][1]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int u = 0; u < kSteps; ++u) b[i][u] = *(const u32x4*)(buf + (g + i) * 8 * kRowBytes + u * 128);
+      for (int g = 0; g < TOKENS / 16; ++g) {
+        if (g * 16u >= used) break;
+        u32x4 b[kSteps][2];
 #pragma unroll
         for (int u = 0; u < kSteps; ++u)
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2; ++i) b[u][i] = *(const u32x4*)(buf + g * 16 * kRowBytes + u * 128 + (get ^ (i * 16)));
 #pragma unroll
-            for (int n = 0; n < 2; ++n) acc[n][g + i] = mfma_16x16x32<DT>(v[u][n], b[i][u], acc[n][g + i]);
+        for (int u = 0; u < kSteps; ++u)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) acc[g] = mfma_16x16x32<DT>(rows_of[u][i], b[u][i], acc[g]);
       }
       ++turns;
     };
@@ -482,11 +496,11 @@ __global__ __launch_bounds__(kDenseBlock, 2) void layer_dense_kernel(const Layer
       if (c + 1 < c1) product(wv[1]);
     }
 #pragma unroll
-    for (int g = 0; g < TOKENS / 8; ++g) {
-      if (g * 8u >= used) break;
-      const f32x2 v0 = add_halves(acc[0][g]), v1 = add_halves(acc[1][g]);
-      if (!lane_holds() || g * 8 + r >= used) continue;
-      const uint32_t pair = list[m0 + g * 8 + r], row = row0 + lane_row();
+    for (int g = 0; g < TOKENS / 16; ++g) {
+      if (g * 16 + token >= used) break;
+      // rows 4 * (lane / 16) .. + 3 of the product: of either set two rows
+      const f32x2 v0 = {acc[g][0], acc[g][2]}, v1 = {acc[g][1], acc[g][3]};
+      const uint32_t pair = list[m0 + g * 16 + token], row = row0 + lane_row();
       if constexpr (IN) {
         if (row < a.inter) {  // inter is a multiple of 8: both rows or none
           union { S e[2]; uint32_t v; } h;
