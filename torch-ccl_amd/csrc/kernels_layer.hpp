@@ -363,13 +363,16 @@ __global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArg
 // The same products where an expert has so many tokens that reading them again for every 16 rows costs
 // more than the weights.  A tile is 8 wavefronts x 2 sets of rows of an expert, over all of hidden (first
 // product: 64 gate rows and their up rows) or one part of inter (second product: 128 rows).  Its tokens go
-// through LDS, a chunk of columns of TOKENS of them at a time.  While a chunk is multiplied, the rows and
-// tokens of the next one are on their way into registers.
-// 160 tokens on 8 experts of 4096 x 7168, 40 each: 206 us for the first product (4.6 TB/s, 183 TFLOP/s) and 99 for
-// the second.  A workgroup reads at the memory's rate once it runs; what is lost is its start, its end and the last
-// round of workgroups, which not all compute units have (448 tiles of the first product on 256 units that hold one
-// or two each).  A workgroup that goes on to its next tile by itself, loads three chunks ahead, and 4 wavefronts
-// instead of 8 were slower.
+// through LDS, a chunk of columns of 128 of them at a time.  While a chunk is multiplied, the rows and tokens of the
+// next one are on their way into registers.
+// 160 tokens on 8 experts of 4096 x 7168, 40 each: 185 us for the first product (5.1 TB/s, 203 TFLOP/s) and 92 for
+// the second; 128 tokens on each of 2 experts of 4096 x 8192 115 us in all.  Two workgroups fit on a compute unit by
+// registers (128) and LDS (80 KiB); with the products of few tokens, half of whose sums are not used, it was one and
+// the layer took 307 us instead of 280.
+// What is lost is a workgroup's start and end and the join.  A workgroup that goes on to its next tile by itself,
+// loads three chunks ahead, and 4 wavefronts instead of 8 were slower; a tile of 64 tokens is 1 or 2 percent faster
+// or 4 slower below 64 tokens an expert and reads the weights twice above (64 pairs on each of 8 experts of 4096 x
+// 1792 132 us against 90).
 constexpr int kDenseWaves = 8;
 constexpr int kDenseBlock = kDenseWaves * kWave;
 constexpr uint32_t kDenseInRows = kDenseWaves * kSetRows, kDenseOutRows = 2 * kDenseInRows;
@@ -388,17 +391,16 @@ __device__ __forceinline__ void exchange_sets(const u32x4& first, const u32x4& s
   }
 }
 
-// Steps of columns in a chunk: as many as the registers have room for beside the sums of TOKENS tokens.
-constexpr int dense_steps(int tokens) { return 2; }
-// Tokens that one thread stages a 16-byte piece of.
-constexpr int dense_share(int tokens) { return tokens * dense_steps(tokens) * 8 / kDenseBlock; }
+constexpr int kDenseTokens = 128;                                                  // of a tile
+constexpr int kDenseSteps = 2;                                                     // of columns in a chunk
+constexpr int kDenseShare = kDenseTokens * kDenseSteps * 8 / kDenseBlock;          // tokens that one thread stages a piece of
 
-template <int DT, int TOKENS, bool IN>
+template <int DT, bool IN>
 __global__ __launch_bounds__(kDenseBlock, 4) void layer_dense_kernel(const LayerArgs a) {
   using S = typename Elem<DT>::store_t;
-  constexpr int kSteps = dense_steps(TOKENS), kPieces = kSteps * 8, kShare = dense_share(TOKENS), kStaged = kDenseBlock / kPieces;
+  constexpr int kSteps = kDenseSteps, kPieces = kSteps * 8, kShare = kDenseShare, kStaged = kDenseBlock / kPieces;
   constexpr uint32_t kCols = kSteps * kStepCols, kRowBytes = kCols * 2;
-  __shared__ __align__(16) char space[2 * TOKENS * kRowBytes];  // two chunks of the tokens
+  __shared__ __align__(16) char space[2 * kDenseTokens * kRowBytes];  // two chunks of the tokens
   __shared__ int16_t expert[kLayerMaxPairs];
   __shared__ uint16_t list[kLayerMaxPairs];
   const uint32_t wave = wave_index(), r = lane_member(), col = lane_column();
@@ -440,8 +442,8 @@ __global__ __launch_bounds__(kDenseBlock, 4) void layer_dense_kernel(const Layer
   stage_experts(a, expert);
   uint32_t m = 0, turns = 0;
   for (uint32_t from = 0; from < a.pairs;) m += list_pairs(expert, a.pairs, (int)e, from, list + m);
-  for (uint32_t m0 = 0; m0 < m; m0 += TOKENS) {
-    const uint32_t used = m - m0 < TOKENS ? m - m0 : TOKENS;
+  for (uint32_t m0 = 0; m0 < m; m0 += kDenseTokens) {
+    const uint32_t used = m - m0 < kDenseTokens ? m - m0 : kDenseTokens;
     uint32_t from[kShare];
 #pragma unroll
     for (int i = 0; i < kShare; ++i) {
@@ -453,23 +455,23 @@ __global__ __launch_bounds__(kDenseBlock, 4) void layer_dense_kernel(const Layer
 #pragma unroll
       for (int i = 0; i < kShare; ++i) tv[i] = __builtin_amdgcn_raw_buffer_load_b128(tokens, from[i] | out, k * 2, 0);
     };
-    f32x4 acc[TOKENS / 16];
+    f32x4 acc[kDenseTokens / 16];
 #pragma unroll
-    for (int g = 0; g < TOKENS / 16; ++g) acc[g] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int g = 0; g < kDenseTokens / 16; ++g) acc[g] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     const auto stage = [&]() {
-      char* buf = space + (turns & 1) * (TOKENS * kRowBytes);
+      char* buf = space + (turns & 1) * (kDenseTokens * kRowBytes);
 #pragma unroll
       for (int i = 0; i < kShare; ++i) *(u32x4*)(buf + put + i * kStaged * kRowBytes) = tv[i];
       __syncthreads();
     };
     const auto product = [&](const u32x4(&v)[kSteps][2]) {
-      const char* buf = space + (turns & 1) * (TOKENS * kRowBytes);
+      const char* buf = space + (turns & 1) * (kDenseTokens * kRowBytes);
       __builtin_amdgcn_sched_barrier(0);  // the loads go first
       u32x4 rows_of[kSteps][2];
 #pragma unroll
       for (int u = 0; u < kSteps; ++u) exchange_sets(v[u][0], v[u][1], rows_of[u][0], rows_of[u][1]);
 #pragma unroll
-      for (int g = 0; g < TOKENS / 16; ++g) {
+      for (int g = 0; g < kDenseTokens / 16; ++g) {
         if (g * 16u >= used) break;
         u32x4 b[kSteps][2];
 #pragma unroll
@@ -492,11 +494,11 @@ __global__ __launch_bounds__(kDenseBlock, 4) void layer_dense_kernel(const Layer
       product(wv[0]);
       if (c + 1 < c1) stage();
       load_tokens(c + 2);
-      load_rows(c + 2 < c1 || m0 + TOKENS >= m ? c + 2 : c0, wv[0]);  // behind the last chunk the first, for the next tokens
+      load_rows(c + 2 < c1 || m0 + kDenseTokens >= m ? c + 2 : c0, wv[0]);  // behind the last chunk the first, for the next tokens
       if (c + 1 < c1) product(wv[1]);
     }
 #pragma unroll
-    for (int g = 0; g < TOKENS / 16; ++g) {
+    for (int g = 0; g < kDenseTokens / 16; ++g) {
       if (g * 16 + token >= used) break;
       // rows 4 * (lane / 16) .. + 3 of the product: of either set two rows
       const f32x2 v0 = {acc[g][0], acc[g][2]}, v1 = {acc[g][1], acc[g][3]};

@@ -189,32 +189,27 @@ int check_router(size_t tokens, size_t experts, int topk, int dtype) {
 
 // How a layer is run, from its sizes alone (the routing is only known on the device).
 struct LayerPlan {
-  int dense;       // tokens of a tile of layer_dense_kernel, 0: layer_in_kernel and layer_out_kernel
+  bool dense;      // layer_dense_kernel, or layer_in_kernel and layer_out_kernel
   uint32_t parts;  // of inter, in the second product
   size_t h_bytes, bytes;
 };
 
 // Pairs per expert above which the tokens go through LDS (layer_dense_kernel) instead of being read again by every
 // workgroup.  Both ways, tokens spread evenly: 8 experts of 4096 x 1792 with 8 / 16 / 24 / 32 / 48 pairs each
-// 62 / 74 / 81 / 117 / 157 us from memory and 72 / 76 / 79 / 82 / 88 through LDS; 32 experts of 2048 x 768 with
-// 8 / 16 / 24 / 32 pairs 61 / 76 / 95 / 125 and 75 / 81 / 87 / 91; 2 experts of 4096 x 8192 with 8 / 16 / 24 / 48
-// pairs 77 / 81 / 105 / 171 and 87 / 88 / 90 / 97.  Uneven routing moves the crossing down.
+// 61 / 73 / 81 / 117 / 157 us from memory and 72 / 75 / 77 / 79 / 86 through LDS; 32 experts of 2048 x 768 with
+// 8 / 16 / 24 / 32 pairs 59 / 75 / 95 / 125 and 68 / 71 / 74 / 77; 2 experts of 4096 x 8192 with 8 / 16 / 24 / 48
+// pairs 65 / 69 / 105 / 171 and 89 / 89 / 91 / 94.
 constexpr size_t kDensePairs = 16;
-// And above which a tile has 128 tokens instead of 64.  An expert with more than a tile reads its weights again (64
-// pairs and more each: 2 experts of 4096 x 8192, 96 pairs each, 117 us with 128 and 175 with 64); with less the
-// smaller tile is 2 to 5 percent faster (48 pairs 96 against 100).  Uneven routing puts some experts over 64 from
-// an average of 32 on (160 tokens on 8 experts of 4096 x 7168, 40 each, 306 us against 318).
-constexpr size_t kWideTilePairs = 32;
-LayerPlan plan_layer(size_t tokens, size_t pairs, size_t experts, size_t hidden, size_t inter) {
+LayerPlan plan_layer(size_t pairs, size_t experts, size_t hidden, size_t inter) {
   LayerPlan p{};
-  if (pairs > kDensePairs * experts || pairs > kFewMaxPairs)
-    p.dense = (tokens <= 64 || pairs <= kWideTilePairs * experts) ? 64 : 128;
+  p.dense = pairs > kDensePairs * experts || pairs > kFewMaxPairs;
   p.h_bytes = up16(pairs * inter * 2);
   p.bytes = p.h_bytes;
   if (p.dense) {
     const size_t groups = (hidden + kDenseOutRows - 1) / kDenseOutRows * experts;
-    const size_t cols = dense_steps(p.dense) * kStepCols, chunks = (inter + cols - 1) / cols;
-    const size_t per = (chunks + std::min<size_t>({chunks, 8, (512 + groups - 1) / groups}) - 1) / std::min<size_t>({chunks, 8, (512 + groups - 1) / groups});
+    const size_t cols = kDenseSteps * kStepCols, chunks = (inter + cols - 1) / cols;
+    // parts that give every compute unit the two workgroups it has room for; more are only joined
+    const size_t wanted = std::min<size_t>({chunks, 8, (512 + groups - 1) / groups}), per = (chunks + wanted - 1) / wanted;
     p.parts = (uint32_t)((chunks + per - 1) / per);
     p.bytes += p.parts * pairs * hidden * sizeof(float);
   } else {
@@ -226,12 +221,12 @@ LayerPlan plan_layer(size_t tokens, size_t pairs, size_t experts, size_t hidden,
   return p;
 }
 
-template <int DT, int TOKENS>
+template <int DT>
 int launch_dense(const LayerArgs& a, hipStream_t s) {
   const uint32_t in_tiles = (a.inter + kDenseInRows - 1) / kDenseInRows * a.experts;
   const uint32_t out_tiles = (a.hidden + kDenseOutRows - 1) / kDenseOutRows * a.experts * a.parts;
-  hipLaunchKernelGGL((layer_dense_kernel<DT, TOKENS, true>), dim3(in_tiles), dim3(kDenseBlock), 0, s, a);
-  hipLaunchKernelGGL((layer_dense_kernel<DT, TOKENS, false>), dim3(out_tiles), dim3(kDenseBlock), 0, s, a);
+  hipLaunchKernelGGL((layer_dense_kernel<DT, true>), dim3(in_tiles), dim3(kDenseBlock), 0, s, a);
+  hipLaunchKernelGGL((layer_dense_kernel<DT, false>), dim3(out_tiles), dim3(kDenseBlock), 0, s, a);
   hipLaunchKernelGGL(layer_join_kernel<DT>, dim3((a.hidden / 4 + 255) / 256, a.tokens), dim3(256), 0, s, a);
   return launched("moe layer");
 }
@@ -256,8 +251,8 @@ int launch_layer_out(const LayerArgs& a, hipStream_t s) {
 }
 
 template <int DT>
-int launch_layer(const LayerArgs& a, int dense, hipStream_t s) {
-  if (dense) return dense == 64 ? launch_dense<DT, 64>(a, s) : launch_dense<DT, 128>(a, s);
+int launch_layer(const LayerArgs& a, bool dense, hipStream_t s) {
+  if (dense) return launch_dense<DT>(a, s);
   const dim3 in_grid((a.inter + kInRows - 1) / kInRows, a.by_pair ? a.pairs : a.experts), in_block(kInWaves * kWave);
   // the fewest sums that serve all tokens of an expert at once (58 tokens, 15 on each of 23 experts of 4016 x 624: 111 us
   // with sums for 32 tokens, 137 for 16; 64 tokens, 4 on each of 128: 302 and 310)
@@ -439,7 +434,7 @@ int mccl_moe_route_grad(const float* grad_weights, const void* logits, const int
 
 size_t mccl_moe_layer_workspace(size_t tokens, int topk, size_t experts, size_t hidden, size_t inter) {
   if (topk < 1 || tokens == 0 || experts == 0 || hidden == 0 || inter == 0) return 0;
-  return plan_layer(tokens, tokens * (size_t)topk, experts, hidden, inter).bytes;
+  return plan_layer(tokens * (size_t)topk, experts, hidden, inter).bytes;
 }
 
 int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int32_t* expert_ids, const float* weights, size_t tokens,
@@ -462,7 +457,7 @@ int mccl_moe_layer(const void* x, const void* w_in, const void* w_out, const int
     return mccl_report_error(MCCL_ERR_INVALID_ARG, "x, the weights or the output are not 16-byte aligned");
   if (misaligned(expert_ids, 4) || misaligned(weights, 4)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "expert ids or weights misaligned");
   const size_t pairs = tokens * (size_t)topk, row = tokens * hidden * 2;
-  const LayerPlan plan = plan_layer(tokens, pairs, experts, hidden, inter);
+  const LayerPlan plan = plan_layer(pairs, experts, hidden, inter);
   if (plan.dense && std::max((inter + kDenseInRows - 1) / kDenseInRows, (hidden + kDenseOutRows - 1) / kDenseOutRows * plan.parts) * experts > kMaxDenseTiles)
     return mccl_report_error(MCCL_ERR_INVALID_ARG, "%zu experts of %zu x %zu are too many rows for one launch", experts, hidden, inter);
   const size_t need = plan.bytes;
