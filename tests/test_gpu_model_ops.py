@@ -682,3 +682,80 @@ def test_workspaces_of_the_caller_are_used_and_may_be_dirty(mccl):
     up = torch.randn(4000, 72, generator=g).to(DEV)
     ws = torch.full((capi.lib().mccl_embedding_grad_workspace(4000, 72),), 0xFF, dtype=torch.uint8, device=DEV)
     assert torch.equal(mccl.embedding_grad(up, a, workspace=ws), mccl.embedding_grad(up, b))
+
+# ---------------------------------------------------------------------------------------------
+# the layer between its two products
+# ---------------------------------------------------------------------------------------------
+def layer_reference_unrounded(x, w_in, w_out, ids, weights, first, activation, dtype):
+    """layer_reference without a rounding of act(..) * (..) to the layer's type: what the second product
+    takes holds 2^-16 of it or better (two parts of 8 bits each), next to the fp32 roundings."""
+    T, H = x.shape
+    E, I = w_out.shape[0], w_out.shape[2]
+    out, tol, size = (torch.zeros(T, H, dtype=torch.float64) for _ in range(3))
+    for t in range(T):
+        for k in range(ids.shape[1]):
+            e = int(ids[t, k]) - first
+            if not 0 <= e < E:
+                continue
+            a, b, xt, w = w_in[e].double(), w_out[e].double(), x[t].double(), float(weights[t, k])
+            s, ds = a @ xt, (H + 1) * U * (a.abs() @ xt.abs())
+            act = act64(s[:I], activation)
+            h = act * s[I:]
+            dh = (1.2 * ds[:I] + 8 * U * act.abs()) * (s[I:].abs() + ds[I:]) + act.abs() * ds[I:]
+            dh = dh + 2.0 ** -16 * (h.abs() + dh)
+            y, dy = b @ h, b.abs() @ dh + 4 * (I + 1) * U * (b.abs() @ (h.abs() + dh))  # four products of parts each
+            out[t] += w * y
+            size[t] += abs(w) * (y.abs() + dy)
+            tol[t] += abs(w) * dy
+    tol = tol + (ids.shape[1] + 1) * U * size
+    return out, tol + half_step(dtype) * (out.abs() + tol) + torch.finfo(dtype).smallest_normal * half_step(dtype)
+
+
+LAYERS_BOTH_WAYS = [(1, 1, 1, 64, 64), (5, 1, 1, 40, 200), (9, 2, 3, 264, 136), (17, 1, 1, 72, 88), (40, 2, 2, 136, 264), (64, 8, 128, 64, 72), (130, 1, 1, 264, 392)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("T,k,E,H,I", LAYERS_BOTH_WAYS)
+def test_moe_layer_rounds_to_its_type_once(mccl, dtype, activation, T, k, E, H, I):
+    x, w_in, w_out, ids, weights = layer_inputs(gen(61, T, k, E, H, I), T, k, E, E, H, I, dtype)
+    out = mccl.moe_layer(x.to(DEV), w_in.to(DEV), w_out.to(DEV), ids.to(DEV), weights.to(DEV), activation=activation)
+    want, tol = layer_reference_unrounded(x, w_in, w_out, ids, weights, 0, activation, dtype)
+    within(out, want, tol, "layer")
+
+
+@pytest.mark.parametrize("T,k,E,H,I", LAYERS_BOTH_WAYS)
+def test_moe_layer_between_its_products_has_the_range_of_fp32(mccl, T, k, E, H, I):
+    """act(..) * (..) around 10^6, which f16 has no number for, and an output that it has."""
+    dtype = torch.float16
+    x, w_in, w_out, ids, weights = layer_inputs(gen(62, T, k, E, H, I), T, k, E, E, H, I, dtype)
+    x, w_out = 2.0 ** 10 * x, (2.0 ** -10 * w_out.double()).to(dtype)
+    assert torch.isfinite(x).all()
+    out = mccl.moe_layer(x.to(DEV), w_in.to(DEV), w_out.to(DEV), ids.to(DEV), weights.to(DEV))
+    want, tol = layer_reference_unrounded(x, w_in, w_out, ids, weights, 0, "silu", dtype)
+    assert float(want.abs().max()) < 65504 / 2
+    within(out, want, tol, "layer")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("T,k,E", [(3, 1, 1), (40, 2, 2)])
+def test_moe_layer_of_weights_that_are_not_finite(mccl, dtype, T, k, E):
+    """An infinite weight of the second product makes its row of the output infinite with the sign that the
+    formula gives, a NaN makes it NaN, and the other rows stay as they are."""
+    H, I = 72, 40
+    x, w_in, w_out, ids, weights = layer_inputs(gen(63, T, k, E), T, k, E, E, H, I, dtype)
+    args = [x.to(DEV), w_in.to(DEV), w_out.to(DEV), ids.to(DEV), weights.to(DEV)]
+    clean = mccl.moe_layer(*args)
+    bad = w_out.clone()
+    bad[0, 5, 7], bad[0, 6, 0], bad[0, 20, I - 1] = float("inf"), float("-inf"), float("nan")
+    args[2] = bad.to(DEV)
+    out = mccl.moe_layer(*args).cpu()
+    rows = [c for c in range(H) if c not in (5, 6, 20)]
+    assert torch.equal(out[:, rows], clean.cpu()[:, rows])
+    s = torch.einsum("ij,tj->ti", w_in[0].double(), x.double())
+    h = act64(s[:, :I], "silu") * s[:, I:]
+    for t in range(T):
+        if 0 not in ids[t].tolist():
+            continue
+        assert out[t, 20].isnan()
+        assert float(out[t, 5]) == math.copysign(math.inf, float(h[t, 7])) and float(out[t, 6]) == -math.copysign(math.inf, float(h[t, 0]))

@@ -9,11 +9,11 @@ namespace {
 constexpr int kLayerMaxTokens = 256;
 constexpr int kLayerMaxPairs = 4096;
 constexpr uint32_t kFewMaxPairs = 2048;  // of layer_in_kernel and layer_out_kernel
-constexpr int kLayerMaxExperts = 4096;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // 16 x 16 += (16 x 32) . (32 x 16): lane l holds 8 values of row (column) l % 16, from 8 * (l / 16) on of the
 // 32, and gets rows 4 * (l / 16) .. + 3 of column l % 16.
@@ -31,7 +31,7 @@ struct LayerArgs {
   const char* w_out;    // [experts][hidden][inter]
   const int32_t* ids;   // [tokens][topk]
   const float* weights; // [tokens][topk]
-  char* h;              // workspace [pairs][inter]
+  char* h;              // workspace [2][pairs][inter]: the high, then the low parts
   float* y;             // workspace [parts][pairs][hidden], where the products of a pair meet in memory
   char* out;
   uint32_t tokens, topk, pairs, experts, hidden, inter;
@@ -56,6 +56,55 @@ __device__ __forceinline__ float activate(float v, int activation) {
 }
 
 // ------------------------------------------------------------------------------------------
+// what the second product takes
+// ------------------------------------------------------------------------------------------
+// h = act(gate) * up is an fp32 value, and the second product's matrix instructions take 16 bits.  Rounded to the
+// layer's type, it made the result's error 1.4 times that of its own last rounding (0.0024 against 0.0017 in bf16), and
+// in f16 infinite above 65504.  So h is kept as the sum of two bf16: its upper 8 significant bits as they are, and what they leave,
+// rounded: 2^-16 of h at the most, over fp32's range.  The second product adds the products of both parts.
+// Where nothing is left (h has 8 bits, or is infinite) the low part is the smallest normal number of h's sign, so that
+// an infinite weight meets no zero that h does not have; what it adds elsewhere is below 2^-100 of any weight's.
+// That costs nothing for up to 4 pairs of an expert (1 token 36.4 us for the layer with and without, 32 tokens on an
+// expert-parallel shard 213 and 212) and up to a tenth for more in bf16 (64 tokens on 128 experts 322 and 302, 160 on 8
+// wide ones 307 and 287); the f16 weights' split a few percent more.
+struct Parts {
+  uint16_t high, low;
+};
+__device__ __forceinline__ Parts split(float h) {
+  const uint32_t bits = f32_to_bits(h), high = bits >> 16;
+  const float rest = h - bits_to_f32(high << 16);
+  const uint32_t least = (high & 0x8000u) | ((high & 0x7fffu) ? 0x0080u : 0u);
+  return {(uint16_t)high, rest < 0.0f || rest > 0.0f ? Elem<MCCL_BF16>::store(rest) : (uint16_t)least};
+}
+
+// f16 weights for the products with such parts: 8 values as the sum of two bf16, exactly (8 and 3 significant bits).
+// An infinite weight leaves 256 instead of infinity - infinity.
+__device__ __forceinline__ uint32_t bf16_pair(f16x2 v) {  // of values that bf16 has
+  return __builtin_amdgcn_perm(f32_to_bits((float)v[1]), f32_to_bits((float)v[0]), 0x07060302u);
+}
+__device__ __forceinline__ void split_f16(const u32x4& w, u32x4& high, u32x4& low) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t pair = w[i], upper_bits = pair & 0xfff8fff8u;
+    const f16x2 all = __builtin_bit_cast(f16x2, pair), upper = __builtin_bit_cast(f16x2, upper_bits);
+    high[i] = bf16_pair(upper);
+    low[i] = bf16_pair(__builtin_elementwise_min(all - upper, (f16x2){(_Float16)256.0f, (_Float16)256.0f}));
+  }
+}
+
+// c += weights . parts
+template <int DT>
+__device__ __forceinline__ f32x4 mfma_parts(u32x4 w, u32x4 parts, f32x4 c) {
+  if constexpr (DT == MCCL_BF16) {
+    return mfma_16x16x32<MCCL_BF16>(w, parts, c);
+  } else {
+    u32x4 high, low;
+    split_f16(w, high, low);
+    return mfma_16x16x32<MCCL_BF16>(high, parts, mfma_16x16x32<MCCL_BF16>(low, parts, c));
+  }
+}
+
+// ------------------------------------------------------------------------------------------
 // products of 8 weight rows with 8 tokens
 // ------------------------------------------------------------------------------------------
 // The matrix instruction takes 16 rows of 32 columns: given 16 weight rows, a load would read 64 bytes
@@ -76,8 +125,9 @@ __device__ __forceinline__ uint32_t lane_column() { return (threadIdx.x % 2 + (t
 __device__ __forceinline__ uint32_t lane_row() { return (threadIdx.x % kWave) / 16 * 2; }
 __device__ __forceinline__ bool lane_holds() { return threadIdx.x % 2 == 0; }
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+template <int CTRL = 0xb1>  // lanes 1 0 3 2
 __device__ __forceinline__ float from_neighbour(float v) {
-  return bits_to_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_to_bits(v), 0xb1, 0xf, 0xf, true));  // lanes 1 0 3 2
+  return bits_to_f32((uint32_t)__builtin_amdgcn_update_dpp(0, (int)f32_to_bits(v), CTRL, 0xf, 0xf, true));
 }
 __device__ __forceinline__ f32x2 add_halves(f32x4 v) { return (f32x2){v[0] + from_neighbour(v[1]), v[2] + from_neighbour(v[3])}; }
 
@@ -86,7 +136,7 @@ __device__ __forceinline__ f32x2 add_halves(f32x4 v) { return (f32x2){v[0] + fro
 // that do not exist are left out without a branch.  A matrix and what the last turn of a loop asks for behind
 // it stay below kOutside, so that no sum of offsets passes 32 bits.
 constexpr uint32_t kOutside = 0x80000000u;
-constexpr size_t kLayerMaxColumns = 1u << 17;          // hidden and inter: 4096 pairs of h are 1 GiB
+constexpr size_t kLayerMaxColumns = 1u << 17;          // hidden and inter: 4096 pairs of a part of h are 1 GiB
 constexpr size_t kLayerMaxExpert = kOutside - 65536u;  // bytes of an expert's w_in
 constexpr int kStreamed = 2;  // non-temporal: weights are read once
 
@@ -97,7 +147,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t matrix_at(const char* base, ui
 // acc[w][t] += rows . tokens over the steps [s0, s1) below column `depth`: this lane's rows lie w[...] bytes into
 // `rows`, its tokens b[...] into `tokens`, both at the lane's column.  The loads of STEPS steps are issued
 // before the first product.
-template <int DT, int NW, int NT, int STEPS>
+// PARTS: the tokens are rows of h.
+template <int DT, bool PARTS, int NW, int NT, int STEPS>
 __device__ __forceinline__ void multiply_sets(__amdgpu_buffer_rsrc_t rows, const uint32_t (&w)[NW], __amdgpu_buffer_rsrc_t tokens,
                                               const uint32_t (&b)[NT], uint32_t s0, uint32_t s1, uint32_t depth, f32x4 (&acc)[NW][NT]) {
   const uint32_t end = s1 * kStepCols < depth ? s1 * kStepCols : depth, col = lane_column();
@@ -118,7 +169,7 @@ __device__ __forceinline__ void multiply_sets(__amdgpu_buffer_rsrc_t rows, const
 #pragma unroll
       for (int n = 0; n < NW; ++n)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[n][t] = mfma_16x16x32<DT>(wv[u][n], bv[u][t], acc[n][t]);
+        for (int t = 0; t < NT; ++t) acc[n][t] = PARTS ? mfma_parts<DT>(wv[u][n], bv[u][t], acc[n][t]) : mfma_16x16x32<DT>(wv[u][n], bv[u][t], acc[n][t]);
   }
 }
 
@@ -162,9 +213,7 @@ __device__ __forceinline__ uint32_t list_pairs(const int16_t* expert, uint32_t p
 // h[pair][i] = act(w_in[e][i] . x[t]) * (w_in[e][inter + i] . x[t])
 // ------------------------------------------------------------------------------------------
 // A workgroup takes 16 gate rows and their 16 up rows of one expert; its wavefronts share the columns, in fp32 until
-// the gate is applied.  h is then rounded once to the layer's type, which the second product's matrix
-// instructions take: against 64 bits the result is off by 1.4 times its own last rounding (0.0024 in bf16) and
-// would be by 1.0 with h in fp32, for twice the second product's instructions and h's reads.
+// the gate is applied, and h leaves in two parts.
 // Bound by reading the weights: 15.7 experts of 7168 x 2048, 32 tokens, 132 us, 7.0 TB/s; 8 experts of 4096 x 1024,
 // 1 token, 23 us, 5.9 TB/s (a workgroup reads 256 KiB there, and its start and end are a fifth of its time).
 // 8 and 16 wavefronts a workgroup, two halves of the loads in turns, and 4 workgroups a compute unit by fewer registers
@@ -175,7 +224,6 @@ constexpr int kInRows = 2 * kSetRows;
 template <int DT, int NT, int STEPS>
 __device__ __forceinline__ void layer_in_tokens(const LayerArgs& a, int e, uint32_t i0, const uint16_t* list, uint32_t m0, uint32_t m,
                                                 float (*sums)[4][NT][8][8]) {
-  using S = typename Elem<DT>::store_t;
   const uint32_t wave = wave_index();
   const uint32_t r = lane_member(), col = lane_column();
   uint32_t w[4], b[NT];
@@ -196,7 +244,7 @@ __device__ __forceinline__ void layer_in_tokens(const LayerArgs& a, int e, uint3
     for (int t = 0; t < NT; ++t) acc[n][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   const uint32_t steps = (a.hidden + kStepCols - 1) / kStepCols, per = (steps + kInWaves - 1) / kInWaves;
   const uint32_t s0 = wave * per, s1 = s0 + per < steps ? s0 + per : steps;
-  multiply_sets<DT, 4, NT, STEPS>(w_in_of(a, e), w, matrix_at(a.x, a.tokens * a.hidden * 2), b, s0, s1, a.hidden, acc);
+  multiply_sets<DT, false, 4, NT, STEPS>(w_in_of(a, e), w, matrix_at(a.x, a.tokens * a.hidden * 2), b, s0, s1, a.hidden, acc);
 #pragma unroll
   for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -214,7 +262,10 @@ __device__ __forceinline__ void layer_in_tokens(const LayerArgs& a, int e, uint3
       g += sums[p][row / 8][token / 8][token % 8][row % 8];
       u += sums[p][2 + row / 8][token / 8][token % 8][row % 8];
     }
-    ((S*)a.h)[(size_t)list[m0 + token] * a.inter + i0 + row] = Elem<DT>::store(activate(g, a.activation) * u);
+    const Parts h = split(activate(g, a.activation) * u);
+    uint16_t* at = (uint16_t*)a.h + (size_t)list[m0 + token] * a.inter + i0 + row;
+    at[0] = h.high;
+    at[(size_t)a.pairs * a.inter] = h.low;
   }
   __syncthreads();
 }
@@ -249,7 +300,8 @@ __global__ __launch_bounds__(kInWaves * kWave) void layer_in_kernel(const LayerA
 // all pairs in LDS, so that the weighted sum needs no other workgroup: work of a wavefront is an expert
 // and one of a.parts parts of inter.  Sums in fp32, the pairs of a token in ascending order, one rounding.
 // Bound by reading the weights: 15.7 experts of 7168 x 2048, 32 tokens, 74 us, 6.3 TB/s; 8 of 4096 x 1024, 1 token,
-// 14 us, 4.7 TB/s; below some 20 MB by its chain: ids, lists, h, products, sums (3 experts of 520 x 200 5.5 us).
+// 14 us, 4.7 TB/s; from 5 pairs of an expert on h's reads, which every workgroup makes for its 8 or 16 rows, are as many as
+// the weights'; below some 20 MB by its chain: ids, lists, h, products, sums (10 experts of 520 x 200 f16 6.2 us).
 struct LayerOutLds {
   uint32_t weights, first, active, lists, y, bytes;
 };
@@ -265,6 +317,9 @@ __host__ __device__ inline LayerOutLds layer_out_lds(uint32_t pairs, uint32_t ex
   return l;
 }
 
+// The 8 tokens of a set are the high and the low parts of 4 pairs, next to each other.
+constexpr int kSetPairs = 4;
+
 template <int DT, int NW, int NT, int STEPS>
 __device__ __forceinline__ void layer_out_tokens(const LayerArgs& a, int e, uint32_t c0, uint32_t part, const uint16_t* list, uint32_t m0,
                                                  uint32_t m, float* y) {
@@ -277,8 +332,8 @@ __device__ __forceinline__ void layer_out_tokens(const LayerArgs& a, int e, uint
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const uint32_t mine = m0 + t * 8 + r;
-    b[t] = (list[mine < m ? mine : m - 1] * a.inter + col) * 2;
+    const uint32_t mine = m0 + t * kSetPairs + r / 2;
+    b[t] = ((list[mine < m ? mine : m - 1] + r % 2 * a.pairs) * a.inter + col) * 2;
   }
   f32x4 acc[NW][NT];
 #pragma unroll
@@ -287,14 +342,17 @@ __device__ __forceinline__ void layer_out_tokens(const LayerArgs& a, int e, uint
     for (int t = 0; t < NT; ++t) acc[n][t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
   const uint32_t steps = (a.inter + kStepCols - 1) / kStepCols, per = (steps + a.parts - 1) / a.parts;
   const uint32_t s0 = part * per, s1 = s0 + per < steps ? s0 + per : steps;
-  multiply_sets<DT, NW, NT, STEPS>(w_out_of(a, e), w, matrix_at(a.h, a.pairs * a.inter * 2), b, s0, s1, a.inter, acc);
+  multiply_sets<DT, true, NW, NT, STEPS>(w_out_of(a, e), w, matrix_at(a.h, a.pairs * a.inter * 4), b, s0, s1, a.inter, acc);
 #pragma unroll
   for (int n = 0; n < NW; ++n)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const f32x2 v = add_halves(acc[n][t]);
-      if (lane_holds() && m0 + t * 8 + r < m)
-        *(f32x2*)(y + (((size_t)list[m0 + t * 8 + r] * a.parts + part) * NW + n) * kSetRows + lane_row()) = v;
+      f32x2 v = add_halves(acc[n][t]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[i] += from_neighbour<0x4e>(v[i]);  // lanes 2 3 0 1: the other part
+      const uint32_t mine = m0 + t * kSetPairs + r / 2;
+      if (threadIdx.x % 4 == 0 && mine < m)
+        *(f32x2*)(y + (((size_t)list[mine] * a.parts + part) * NW + n) * kSetRows + lane_row()) = v;
     }
 }
 
@@ -336,9 +394,9 @@ __global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArg
     while (from < a.pairs) {
       const uint32_t m = list_pairs(expert, a.pairs, e, from, list);
       uint32_t m0 = 0;
-      for (; m0 < m && m - m0 > 16; m0 += 32) layer_out_tokens<DT, NW, 4, 2>(a, e, c0, part, list, m0, m, y);
-      for (; m0 < m && m - m0 > 8; m0 += 16) layer_out_tokens<DT, NW, 2, 4>(a, e, c0, part, list, m0, m, y);
-      for (; m0 < m; m0 += 8) layer_out_tokens<DT, NW, 1, 8 / NW>(a, e, c0, part, list, m0, m, y);
+      for (; m0 < m && m - m0 > 8; m0 += 16) layer_out_tokens<DT, NW, 4, 2>(a, e, c0, part, list, m0, m, y);
+      for (; m0 < m && m - m0 > 4; m0 += 8) layer_out_tokens<DT, NW, 2, 4>(a, e, c0, part, list, m0, m, y);
+      for (; m0 < m; m0 += 4) layer_out_tokens<DT, NW, 1, 8 / NW>(a, e, c0, part, list, m0, m, y);
     }
   }
   __syncthreads();
@@ -365,14 +423,14 @@ __global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArg
 // product: 64 gate rows and their up rows) or one part of inter (second product: 128 rows).  Its tokens go
 // through LDS, a chunk of columns of 128 of them at a time.  While a chunk is multiplied, the rows and tokens of the
 // next one are on their way into registers.
-// 160 tokens on 8 experts of 4096 x 7168, 40 each: 185 us for the first product (5.1 TB/s, 203 TFLOP/s) and 92 for
-// the second; 128 tokens on each of 2 experts of 4096 x 8192 115 us in all.  Two workgroups fit on a compute unit by
-// registers (128) and LDS (80 KiB); with the products of few tokens, half of whose sums are not used, it was one and
-// the layer took 307 us instead of 280.
-// What is lost is a workgroup's start and end and the join.  A workgroup that goes on to its next tile by itself,
-// loads three chunks ahead, and 4 wavefronts instead of 8 were slower; a tile of 64 tokens is 1 or 2 percent faster
-// or 4 slower below 64 tokens an expert and reads the weights twice above (64 pairs on each of 8 experts of 4096 x
-// 1792 132 us against 90).
+// 160 tokens on 8 experts of 4096 x 7168 f16, 40 each: 194 us for the first product (4.9 TB/s, 194 TFLOP/s) and 147 for
+// the second (3.2 TB/s); 96 tokens on each of 2 experts of 4096 x 8192 bf16 122 us in all.  Two workgroups fit on a
+// compute unit by registers (128) and LDS (80 KiB); with the products of few tokens, half of whose sums are not used,
+// it was one and the layer took a tenth longer.
+// What is lost is a workgroup's start and end, the join, and in the second product the turns, whose tokens are twice
+// the bytes.  A workgroup that goes on to its next tile by itself, loads three chunks ahead, and 4 wavefronts instead of
+// 8 were slower; a first product with tiles of 64 tokens is 1 or 2 percent faster or 4 slower below 64 tokens an
+// expert and reads the weights twice above.
 constexpr int kDenseWaves = 8;
 constexpr int kDenseBlock = kDenseWaves * kWave;
 constexpr uint32_t kDenseInRows = kDenseWaves * kSetRows, kDenseOutRows = 2 * kDenseInRows;
@@ -391,16 +449,33 @@ __device__ __forceinline__ void exchange_sets(const u32x4& first, const u32x4& s
   }
 }
 
-constexpr int kDenseTokens = 128;                                                  // of a tile
-constexpr int kDenseSteps = 2;                                                     // of columns in a chunk
-constexpr int kDenseShare = kDenseTokens * kDenseSteps * 8 / kDenseBlock;          // tokens that one thread stages a piece of
+// How the tokens of a turn, up to a barrier, lie in LDS: 32 KiB of them, twice.
+//   first product            128 tokens of 128 columns
+//   second, up to 64 pairs    64 pairs of 128 columns in both parts
+//   second, more             128 pairs of 64 columns in both parts: a chunk of weights takes two turns
+// The last form costs more where it is not needed (16 pairs on each of 8 experts of 4096 x 1792 81 us for the layer against
+// 87): a turn is no shorter than a load of tokens takes, whatever it multiplies.  Tiles of 64 alone read the weights twice
+// for 65 pairs (160 tokens on 8 experts of 4096 x 7168 356 us against 325).
+constexpr int kDenseTokens = 128;  // of a tile
+constexpr int kDenseSteps = 2;     // of 64 columns in a chunk of weights
+constexpr int kDenseShare = 4;     // 16-byte pieces of tokens that one thread stages per turn
+
+template <bool IN, int TOKENS>
+struct Staging {
+  static constexpr int kGroups = TOKENS / 16;                                    // of a product's tokens
+  static constexpr int kParts = IN ? 1 : 2;                                      // of a token that are staged
+  static constexpr int kSteps = 128 * kDenseSteps / (kParts * TOKENS);           // of a turn
+  static constexpr int kTurns = kDenseSteps / kSteps;                            // of a chunk
+  static constexpr int kPieces = kSteps * 8;                                     // of a token's row, side by side
+  static constexpr int kApart = kDenseBlock / kPieces;                           // tokens from one of a thread's to its next
+  static constexpr uint32_t kCols = kSteps * kStepCols, kRowBytes = kCols * 2 * kParts;
+  static_assert(TOKENS * kRowBytes == 32 * 1024 && kDenseShare * kApart == TOKENS * kParts, "LDS and threads are filled");
+};
 
 template <int DT, bool IN>
 __global__ __launch_bounds__(kDenseBlock, 4) void layer_dense_kernel(const LayerArgs a) {
-  using S = typename Elem<DT>::store_t;
-  constexpr int kSteps = kDenseSteps, kPieces = kSteps * 8, kShare = kDenseShare, kStaged = kDenseBlock / kPieces;
-  constexpr uint32_t kCols = kSteps * kStepCols, kRowBytes = kCols * 2;
-  __shared__ __align__(16) char space[2 * kDenseTokens * kRowBytes];  // two chunks of the tokens
+  constexpr uint32_t kCols = kDenseSteps * kStepCols;
+  __shared__ __align__(16) char space[2][32 * 1024];  // the tokens of two turns
   __shared__ int16_t expert[kLayerMaxPairs];
   __shared__ uint16_t list[kLayerMaxPairs];
   const uint32_t wave = wave_index(), r = lane_member(), col = lane_column();
@@ -421,94 +496,122 @@ __global__ __launch_bounds__(kDenseBlock, 4) void layer_dense_kernel(const Layer
   const uint32_t end = c1 * kCols < depth ? c1 * kCols : depth;
   const __amdgpu_buffer_rsrc_t rows = IN ? w_in_of(a, (int)e) : w_out_of(a, (int)e);
   // Columns from `end` on (whole chunks too) are outside and not read.
-  const auto load_rows = [&](uint32_t c, u32x4(&v)[kSteps][2]) {
+  const auto load_rows = [&](uint32_t c, u32x4(&v)[kDenseSteps][2]) {
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) {
+    for (int u = 0; u < kDenseSteps; ++u) {
       const uint32_t k = c * kCols + u * kStepCols, out = k + col < end ? 0 : kOutside;
 #pragma unroll
       for (int n = 0; n < 2; ++n) v[u][n] = __builtin_amdgcn_raw_buffer_load_b128(rows, w[n] | out, k * 2, kStreamed);
     }
   };
-
-  // Staging: a thread's piece of a token's 128 bytes, which are stored in an order turned by the token so that
-  // the 8 tokens which a load from LDS takes at the same columns lie in different banks.
-  const __amdgpu_buffer_rsrc_t tokens = IN ? matrix_at(a.x, a.tokens * a.hidden * 2) : matrix_at(a.h, a.pairs * a.inter * 2);
-  const uint32_t piece = threadIdx.x % kPieces, staged = threadIdx.x / kPieces;
-  const uint32_t put = staged * kRowBytes + (piece / 8) * 128 + ((piece ^ staged) % 8) * 16;
+  const uint32_t h_bytes = a.pairs * a.inter * 2;
+  const __amdgpu_buffer_rsrc_t tokens[2] = {IN ? matrix_at(a.x, a.tokens * a.hidden * 2) : matrix_at(a.h, h_bytes), matrix_at(a.h + h_bytes, h_bytes)};
   const uint32_t token = threadIdx.x % 16;  // of 16, where the sums are too
-  const uint32_t get = token * kRowBytes + ((threadIdx.x % kWave / 16 * 2) ^ (token % 8)) * 16;  // its neighbour piece: ^ 16
 
-  u32x4 wv[2][kSteps][2], tv[kShare];
   stage_experts(a, expert);
   uint32_t m = 0, turns = 0;
   for (uint32_t from = 0; from < a.pairs;) m += list_pairs(expert, a.pairs, (int)e, from, list + m);
-  for (uint32_t m0 = 0; m0 < m; m0 += kDenseTokens) {
-    const uint32_t used = m - m0 < kDenseTokens ? m - m0 : kDenseTokens;
-    uint32_t from[kShare];
+
+  // The products of `used` tokens of the list, from m0 on.
+  const auto multiply = [&](auto staging, uint32_t m0, uint32_t used) {
+    using G = decltype(staging);
+    // Staging: a thread's pieces of its tokens' rows.  The 8 pieces of 128 bytes are stored in an order turned by the
+    // token so that the 8 tokens which a load from LDS takes at the same columns lie in different banks.
+    uint32_t thread = threadIdx.x;
+    asm("" : "+v"(thread));  // the addresses of either form are made where it begins: all of them at once do not fit the registers
+    const uint32_t piece = thread % G::kPieces, staged = thread / G::kPieces;
+    const uint32_t put = staged * G::kRowBytes + (piece / 8) * 128 + ((piece ^ staged) % 8) * 16;
+    const uint32_t get = thread % 16 * G::kRowBytes + ((thread % kWave / 16 * 2) ^ (thread % 8)) * 16;  // its neighbour piece: ^ 16
+    uint32_t from[kDenseShare / G::kParts];
 #pragma unroll
-    for (int i = 0; i < kShare; ++i) {
-      const uint32_t at = i * kStaged + staged, pair = list[m0 + (at < used ? at : 0)];
+    for (int i = 0; i < kDenseShare / G::kParts; ++i) {
+      const uint32_t at = i * G::kApart + staged, pair = list[m0 + (at < used ? at : 0)];
       from[i] = at < used ? ((IN ? pair / a.topk : pair) * depth + piece * 8) * 2 : kOutside;
     }
-    const auto load_tokens = [&](uint32_t c) {
-      const uint32_t k = c * kCols, out = k + piece * 8 < end ? 0 : kOutside;
+    u32x4 wv[2][kDenseSteps][2], tv[kDenseShare];
+    const auto load_tokens = [&](uint32_t turn) {
+      const uint32_t k = turn * G::kCols, out = k + piece * 8 < end ? 0 : kOutside;
 #pragma unroll
-      for (int i = 0; i < kShare; ++i) tv[i] = __builtin_amdgcn_raw_buffer_load_b128(tokens, from[i] | out, k * 2, 0);
+      for (int i = 0; i < kDenseShare; ++i) tv[i] = __builtin_amdgcn_raw_buffer_load_b128(tokens[i % G::kParts], from[i / G::kParts] | out, k * 2, 0);
     };
-    f32x4 acc[kDenseTokens / 16];
-#pragma unroll
-    for (int g = 0; g < kDenseTokens / 16; ++g) acc[g] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     const auto stage = [&]() {
-      char* buf = space + (turns & 1) * (kDenseTokens * kRowBytes);
+      char* buf = space[turns & 1];
 #pragma unroll
-      for (int i = 0; i < kShare; ++i) *(u32x4*)(buf + put + i * kStaged * kRowBytes) = tv[i];
+      for (int i = 0; i < kDenseShare; ++i)
+        *(u32x4*)(buf + put + i / G::kParts * G::kApart * G::kRowBytes + i % G::kParts * (G::kCols * 2)) = tv[i];
       __syncthreads();
     };
-    const auto product = [&](const u32x4(&v)[kSteps][2]) {
-      const char* buf = space + (turns & 1) * (kDenseTokens * kRowBytes);
+    f32x4 acc[G::kGroups];
+#pragma unroll
+    for (int g = 0; g < G::kGroups; ++g) acc[g] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    const auto product = [&](const u32x4(&v)[kDenseSteps][2], int turn) {
+      const char* buf = space[turns & 1];
       __builtin_amdgcn_sched_barrier(0);  // the loads go first
-      u32x4 rows_of[kSteps][2];
+      // First product: the steps of a turn in turn for every 16 tokens; second: both parts, step by step, as f16 rows are split
+      // for a step at a time (both steps at once take more registers than there are).
+      constexpr int kAtOnce = IN ? G::kSteps : 1;
 #pragma unroll
-      for (int u = 0; u < kSteps; ++u) exchange_sets(v[u][0], v[u][1], rows_of[u][0], rows_of[u][1]);
+      for (int u0 = 0; u0 < G::kSteps; u0 += kAtOnce) {
+        u32x4 rows_of[kAtOnce][2];
 #pragma unroll
-      for (int g = 0; g < kDenseTokens / 16; ++g) {
-        if (g * 16u >= used) break;
-        u32x4 b[kSteps][2];
+        for (int u = 0; u < kAtOnce; ++u)
+          exchange_sets(v[turn * G::kSteps + u0 + u][0], v[turn * G::kSteps + u0 + u][1], rows_of[u][0], rows_of[u][1]);
 #pragma unroll
-        for (int u = 0; u < kSteps; ++u)
+        for (int g = 0; g < G::kGroups; ++g) {
+          if (g * 16u >= used) break;
+          u32x4 b[2][2];  // of a step or of a part, and the two pieces
 #pragma unroll
-          for (int i = 0; i < 2; ++i) b[u][i] = *(const u32x4*)(buf + g * 16 * kRowBytes + u * 128 + (get ^ (i * 16)));
+          for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int u = 0; u < kSteps; ++u)
+            for (int i = 0; i < 2; ++i)
+              b[n][i] = *(const u32x4*)(buf + g * 16 * G::kRowBytes + (IN ? n : n * G::kSteps + u0) * 128 + (get ^ (i * 16)));
 #pragma unroll
-          for (int i = 0; i < 2; ++i) acc[g] = mfma_16x16x32<DT>(rows_of[u][i], b[u][i], acc[g]);
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if constexpr (IN) acc[g] = mfma_16x16x32<DT>(rows_of[n][i], b[n][i], acc[g]);
+              else acc[g] = mfma_parts<DT>(rows_of[0][i], b[n][i], acc[g]);
+            }
+        }
       }
       ++turns;
     };
-    load_tokens(c0);
-    if (m0 == 0) load_rows(c0, wv[0]);
+    load_tokens(c0 * G::kTurns);
+    load_rows(c0, wv[0]);
     for (uint32_t c = c0; c < c1; c += 2) {
-      stage();
-      load_tokens(c + 1);
-      load_rows(c + 1, wv[1]);
-      product(wv[0]);
-      if (c + 1 < c1) stage();
-      load_tokens(c + 2);
-      load_rows(c + 2 < c1 || m0 + kDenseTokens >= m ? c + 2 : c0, wv[0]);  // behind the last chunk the first, for the next tokens
-      if (c + 1 < c1) product(wv[1]);
+#pragma unroll
+      for (int turn = 0; turn < G::kTurns; ++turn) {
+        stage();
+        load_tokens(c * G::kTurns + turn + 1);
+        if (turn == 0) load_rows(c + 1, wv[1]);
+        product(wv[0], turn);
+      }
+#pragma unroll
+      for (int turn = 0; turn < G::kTurns; ++turn) {
+        if (c + 1 < c1) stage();
+        load_tokens((c + 1) * G::kTurns + turn + 1);
+        if (turn == 0) load_rows(c + 2, wv[0]);
+        if (c + 1 < c1) product(wv[1], turn);
+      }
     }
 #pragma unroll
-    for (int g = 0; g < kDenseTokens / 16; ++g) {
+    for (int g = 0; g < G::kGroups; ++g) {
       if (g * 16 + token >= used) break;
       // rows 4 * (lane / 16) .. + 3 of the product: of either set two rows
       const f32x2 v0 = {acc[g][0], acc[g][2]}, v1 = {acc[g][1], acc[g][3]};
       const uint32_t pair = list[m0 + g * 16 + token], row = row0 + lane_row();
       if constexpr (IN) {
         if (row < a.inter) {  // inter is a multiple of 8: both rows or none
-          union { S e[2]; uint32_t v; } h;
+          uint32_t high = 0, low = 0;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) h.e[c] = Elem<DT>::store(activate(v0[c], a.activation) * v1[c]);
-          *(uint32_t*)((S*)a.h + (size_t)pair * a.inter + row) = h.v;
+          for (int c = 0; c < 2; ++c) {
+            const Parts h = split(activate(v0[c], a.activation) * v1[c]);
+            high |= (uint32_t)h.high << (c * 16);
+            low |= (uint32_t)h.low << (c * 16);
+          }
+          char* at = a.h + ((size_t)pair * a.inter + row) * 2;
+          *(uint32_t*)at = high;
+          *(uint32_t*)(at + h_bytes) = low;
         }
       } else {
         float* y = a.y + ((size_t)part * a.pairs + pair) * a.hidden + row;
@@ -516,6 +619,13 @@ __global__ __launch_bounds__(kDenseBlock, 4) void layer_dense_kernel(const Layer
         if (row + kSetRows < a.hidden) *(f32x2*)(y + kSetRows) = v1;
       }
     }
+  };
+
+  for (uint32_t m0 = 0; m0 < m; m0 += kDenseTokens) {
+    const uint32_t used = m - m0 < kDenseTokens ? m - m0 : kDenseTokens;
+    if constexpr (IN) multiply(Staging<true, 128>{}, m0, used);
+    else if (used <= 64) multiply(Staging<false, 64>{}, m0, used);
+    else multiply(Staging<false, 128>{}, m0, used);
   }
 }
 

@@ -195,26 +195,28 @@ struct LayerPlan {
 };
 
 // Pairs per expert above which the tokens go through LDS (layer_dense_kernel) instead of being read again by every
-// workgroup.  Both ways, tokens spread evenly: 8 experts of 4096 x 1792 with 8 / 16 / 24 / 32 / 48 pairs each
-// 61 / 73 / 81 / 117 / 157 us from memory and 72 / 75 / 77 / 79 / 86 through LDS; 32 experts of 2048 x 768 with
-// 8 / 16 / 24 / 32 pairs 59 / 75 / 95 / 125 and 68 / 71 / 74 / 77; 2 experts of 4096 x 8192 with 8 / 16 / 24 / 48
-// pairs 65 / 69 / 105 / 171 and 89 / 89 / 91 / 94.
-constexpr size_t kDensePairs = 16;
+// workgroup.  Both ways, tokens spread evenly over experts that are all here: 8 experts of 4096 x 1792 with 8 / 12 / 16 / 24
+// / 48 pairs each 76 / 76 / 89 / 112 / 202 us from memory and 75 / 79 / 81 / 90 / 109 through LDS; 32 experts of 2048 x 768
+// with 8 / 12 / 16 / 24 pairs 68 / 84 / 98 / 136 and 69 / 72 / 76 / 87; 2 experts of 4096 x 8192 with 8 / 12 / 16 / 24 / 48
+// pairs 69 / 75 / 79 / 98 / 180 and 86 / 91 / 88 / 89 / 95.  The pairs are those of all ranks: where only a part of the
+// experts is here, the experts of this rank have fewer of them and the change comes too early.
+constexpr size_t kDensePairs = 12;
 LayerPlan plan_layer(size_t pairs, size_t experts, size_t hidden, size_t inter) {
   LayerPlan p{};
   p.dense = pairs > kDensePairs * experts || pairs > kFewMaxPairs;
-  p.h_bytes = up16(pairs * inter * 2);
+  p.h_bytes = up16(pairs * inter * 4);
   p.bytes = p.h_bytes;
   if (p.dense) {
     const size_t groups = (hidden + kDenseOutRows - 1) / kDenseOutRows * experts;
     const size_t cols = kDenseSteps * kStepCols, chunks = (inter + cols - 1) / cols;
-    // parts that give every compute unit the two workgroups it has room for; more are only joined
+    // parts that give every compute unit the two workgroups it has room for; more are joined at a loss (24 pairs on each of
+    // 32 experts of 2048 x 768 87 us, with twice the parts 92) or gain little (160 tokens on 8 of 4096 x 7168 325 and 314)
     const size_t wanted = std::min<size_t>({chunks, 8, (512 + groups - 1) / groups}), per = (chunks + wanted - 1) / wanted;
     p.parts = (uint32_t)((chunks + per - 1) / per);
     p.bytes += p.parts * pairs * hidden * sizeof(float);
   } else {
     // as many parts as give 16 wavefronts something to do, of 4 steps or more: where few experts can be chosen,
-    // wavefronts would have nothing to do (8 tokens on one of 2 experts of 14336: 60 us against 88 with one part),
+    // wavefronts would have nothing to do (8 tokens on one of 2 experts of 14336: 65 us against 88 with one part),
     // while parts of few steps only add joining (5 tokens x 3 experts, inter 200: 9.0 against 12.7)
     p.parts = (uint32_t)std::max<size_t>(1, std::min<size_t>((inter + kStepCols - 1) / kStepCols / 4, 16 / std::min(pairs, experts)));
   }
@@ -232,8 +234,8 @@ int launch_dense(const LayerArgs& a, hipStream_t s) {
 }
 
 // Whether a workgroup of the second product takes 16 rows with 8 wavefronts, instead of 8 rows with 16: it
-// reads the tokens half as often, if it fills the 256 compute units evenly (1 token, hidden 4096: 36.5 us
-// against 38.5; 64 tokens x 128 experts 303 against 326; but hidden 5120, 320 workgroups, 240 against 230).
+// reads the tokens half as often, if it fills the 256 compute units evenly (1 token, hidden 4096: 36.4 us
+// against 38.9; 64 tokens x 128 experts 322 against 361; but hidden 5120, 320 workgroups, 244 against 237).
 bool wide_out(size_t hidden, size_t pairs) {
   const size_t groups = (hidden + 15) / 16, rounds = (groups + 255) / 256;
   return pairs <= 1024 && groups * 5 >= rounds * 256 * 4;
@@ -254,8 +256,8 @@ template <int DT>
 int launch_layer(const LayerArgs& a, bool dense, hipStream_t s) {
   if (dense) return launch_dense<DT>(a, s);
   const dim3 in_grid((a.inter + kInRows - 1) / kInRows, a.by_pair ? a.pairs : a.experts), in_block(kInWaves * kWave);
-  // the fewest sums that serve all tokens of an expert at once (58 tokens, 15 on each of 23 experts of 4016 x 624: 111 us
-  // with sums for 32 tokens, 137 for 16; 64 tokens, 4 on each of 128: 302 and 310)
+  // the fewest sums that serve all tokens of an expert at once (40 tokens, 10 on each of 23 experts of 4016 x 624: 115 us
+  // with sums for 32 tokens, 117 for 16; 64 tokens, 4 on each of 128: 322 and 330)
   if (a.tokens <= 8) hipLaunchKernelGGL((layer_in_kernel<DT, 8>), in_grid, in_block, 0, s, a);
   else if (a.tokens <= 16) hipLaunchKernelGGL((layer_in_kernel<DT, 16>), in_grid, in_block, 0, s, a);
   else hipLaunchKernelGGL((layer_in_kernel<DT, 32>), in_grid, in_block, 0, s, a);
