@@ -624,8 +624,9 @@ int mccl_embedding_grad(const void* grad, const int64_t* order, const int64_t* o
  *
  * mccl_moe_route_grad: the gradient in the logits of sum grad_weights * weights for the chosen experts:
  * with s = sum_k grad_weights[k] * weights[k], p_e * ([e chosen] g_e - s), or with normalize the same
- * over the chosen experts alone (zero elsewhere).  Ids outside [0, experts) are skipped.  Written in
- * the logits' type.
+ * over the chosen experts alone (zero elsewhere).  Ids outside [0, experts) are skipped.  A row whose
+ * weights are NaN gives NaN: to every expert, or with normalize to the chosen ones.  Written in the
+ * logits' type.
  */
 int mccl_moe_route(const void* logits, size_t tokens, size_t experts, int topk, int normalize, int dtype,
                    int32_t* expert_ids, float* weights, void* stream);

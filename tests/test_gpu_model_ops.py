@@ -759,3 +759,34 @@ def test_moe_layer_of_weights_that_are_not_finite(mccl, dtype, T, k, E):
             continue
         assert out[t, 20].isnan()
         assert float(out[t, 5]) == math.copysign(math.inf, float(h[t, 7])) and float(out[t, 6]) == -math.copysign(math.inf, float(h[t, 0]))
+
+
+# ---------------------------------------------------------------------------------------------
+# the router's gradient of rows that are not finite
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", FLOATS, ids=str)
+@pytest.mark.parametrize("tokens,experts", [(5, 5), (7, 300), (4100, 16), (4100, 250)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_route_gradient_of_rows_that_are_not_finite(mccl, dtype, tokens, experts, bad):
+    """The weights of a row that holds a NaN or +inf are NaN, and so is what depends on them: the chosen experts'
+    gradients with normalize (zero elsewhere), every expert's without.  Other rows are not touched by it."""
+    g = gen(71, tokens, experts)
+    topk = 3
+    logits = torch.randn(tokens, experts, generator=g).to(dtype)
+    marked = torch.arange(tokens) % 4 == 1
+    at = torch.randint(0, experts, (tokens,), generator=g)
+    broken = logits.clone()
+    broken[marked, at[marked]] = bad
+    up = torch.randn(tokens, topk, generator=g).to(DEV)
+    for normalize in (True, False):
+        ids, w = mccl.moe_route(broken.to(DEV), topk, normalize=normalize)
+        assert w[marked].isnan().all()
+        d = mccl.moe_route_grad(up, broken.to(DEV), ids, normalize=normalize).cpu()
+        chosen = torch.zeros(tokens, experts, dtype=torch.bool).scatter(1, ids.cpu().long(), True)
+        if normalize:
+            assert d[marked][chosen[marked]].isnan().all() and not d[marked][~chosen[marked]].any()
+        else:
+            assert d[marked].isnan().all()
+        clean_ids, _ = mccl.moe_route(logits.to(DEV), topk, normalize=normalize)
+        clean = mccl.moe_route_grad(up, logits.to(DEV), clean_ids, normalize=normalize).cpu()
+        assert torch.equal(d[~marked], clean[~marked])
