@@ -605,7 +605,8 @@ int mccl_sort_ids(const void* ids, int id_dtype, size_t n, int64_t first_row, si
  * offsets[v] <= j < offsets[v + 1], fp32 sums in an order that only depends on the offsets (the
  * same bits every time), one rounding.  Rows without a token become zero; with accumulate != 0 the sum
  * is added to what out holds instead, and rows without a token are not touched.  grad: [n][hidden] in
- * bf16 / f16 / f32, out: [rows][hidden] in the same type or f32, n at most 2^28.  order must hold indices below n (others
+ * bf16 / f16 / f32, out: [rows][hidden] in the same type or f32, n at most 2^28.  offsets may be those of
+ * a range of rows of a larger order (offsets + first, rows of them); order must hold indices below n (others
  * are skipped).  workspace: mccl_embedding_grad_workspace(n, hidden) bytes (0 for few tokens).
  */
 size_t mccl_embedding_grad_workspace(size_t n, size_t hidden);

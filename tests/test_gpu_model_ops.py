@@ -790,3 +790,34 @@ def test_route_gradient_of_rows_that_are_not_finite(mccl, dtype, tokens, experts
         clean_ids, _ = mccl.moe_route(logits.to(DEV), topk, normalize=normalize)
         clean = mccl.moe_route_grad(up, logits.to(DEV), clean_ids, normalize=normalize).cpu()
         assert torch.equal(d[~marked], clean[~marked])
+
+
+# ---------------------------------------------------------------------------------------------
+# plans that are a part of another, or none that a sort gives
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("n,hidden", [(40, 24), (700, 24), (5000, 136), (5000, 7)])
+@pytest.mark.parametrize("skip", [0, 3, 64, 70, 200])
+def test_embedding_grad_of_a_range_of_rows_of_a_larger_plan(mccl, n, hidden, skip, accumulate):
+    """One sort of the whole vocabulary, and the gradient of rows [first, first + 6) by their offsets alone: the same bits
+    as those rows of the whole gradient where both cut the tokens alike, and within the sum's roundings of the
+    definition.  `skip` tokens come before the range, whose first row holds most of the others."""
+    g = gen(81, n, hidden, skip, int(accumulate))
+    rows, first, count = 20, 9, 6
+    ids = torch.full((n,), first)
+    ids[torch.rand(n, generator=g) < 0.4] = first + 3
+    some = torch.rand(n, generator=g) < 0.1
+    ids[some] = torch.randint(first, rows, (int(some.sum()),), generator=g)
+    ids[:min(skip, n)] = torch.randint(0, first, (min(skip, n),), generator=g)
+    ids = ids[torch.randperm(n, generator=g)]
+    up = torch.randn(n, hidden, generator=g)
+    order, offsets = mccl.sort_ids(ids.to(DEV), rows)
+    old = torch.randn(count, hidden, generator=g)
+    out = old.to(DEV) if accumulate else torch.full((count, hidden), float("nan"), device=DEV)
+    mccl.embedding_grad(up.to(DEV), (order, offsets[first:first + count + 1].contiguous()), out=out, accumulate=accumulate)
+    want, tol = grad_reference(up, ids, first, count, 1.0)
+    if accumulate:
+        want, tol = want + old.double(), tol + U * (want + old.double()).abs()
+    within(out, want, tol + 2 * U * want.abs(), "range")
+    if not accumulate:
+        assert torch.equal(out, mccl.embedding_grad(up.to(DEV), (order, offsets))[first:first + count])

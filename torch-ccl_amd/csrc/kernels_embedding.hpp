@@ -636,8 +636,9 @@ __global__ __launch_bounds__(kGradWaves * kWave) void embedding_grad_kernel(cons
       const int index = token_at(a, p0 + lane, p1);
       const uint32_t first = row_of_position(a, p0), last = row_of_position(a, p1 - 1);
       const uint32_t first_begin = offset_at(a, first), first_end = offset_at(a, first + 1), last_begin = offset_at(a, last);
-      const bool first_long = first_end - first_begin > kGradPiece;
-      const bool last_long = last != first && offset_at(a, last + 1) - last_begin > kGradPiece;
+      // Before the first row begins (the offsets of a range of rows of a larger plan) the search returns it all the same.
+      const bool first_long = first_begin <= p0 && first_end - first_begin > kGradPiece;
+      const bool last_long = last_begin > p0 && last_begin < p1 && offset_at(a, last + 1) - last_begin > kGradPiece;
       if (last_long) begins = last;
       else if (first_long && first_begin == p0) begins = first;
       for (uint32_t col = first_col; col < a.hidden; col += stride) {
@@ -648,7 +649,7 @@ __global__ __launch_bounds__(kGradWaves * kWave) void embedding_grad_kernel(cons
           write_partial<DT, VL, SHORT>(slot, c, acc);
         }
         if (last_long) {
-          sum_rows<DT, VL, SHORT>(a, index, last_begin > p0 ? last_begin - p0 : 0, p1 - p0, c, acc);  // before p0 only if offsets fall
+          sum_rows<DT, VL, SHORT>(a, index, last_begin - p0, p1 - p0, c, acc);
           write_partial<DT, VL, SHORT>(slot + a.hidden, c, acc);
         }
       }

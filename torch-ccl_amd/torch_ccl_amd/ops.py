@@ -307,7 +307,8 @@ def sort_ids(ids, rows, first_row=0, workspace=None):
 
 def embedding_grad(grad, sorted_ids, scale=1.0, dtype=None, out=None, accumulate=False, workspace=None):
     """The gradient of embedding() in its table, and of gather_rows() in its source: row v is scale
-    times the sum of grad's rows for the tokens of v, as sort_ids() of the same ids gave them.  grad
+    times the sum of grad's rows for the tokens of v, as sort_ids() of the same ids gave them (or, for a
+    range of its rows, the order with the range's part of the offsets).  grad
     [..., hidden]; out [rows, hidden] in grad's type or fp32 (`dtype`).  With accumulate the sums are
     added to `out` and rows without a token stay as they are.  The same bits every time."""
     order, offsets = sorted_ids
