@@ -607,7 +607,8 @@ int mccl_sort_ids(const void* ids, int id_dtype, size_t n, int64_t first_row, si
  * is added to what out holds instead, and rows without a token are not touched.  grad: [n][hidden] in
  * bf16 / f16 / f32, out: [rows][hidden] in the same type or f32, n at most 2^28.  offsets may be those of
  * a range of rows of a larger order (offsets + first, rows of them); order must hold indices below n (others
- * are skipped).  workspace: mccl_embedding_grad_workspace(n, hidden) bytes (0 for few tokens).
+ * are skipped); where offsets fall, a row becomes a sum of some rows of grad or stays as it was.
+ * workspace: mccl_embedding_grad_workspace(n, hidden) bytes (0 for few tokens).
  */
 size_t mccl_embedding_grad_workspace(size_t n, size_t hidden);
 int mccl_embedding_grad(const void* grad, const int64_t* order, const int64_t* offsets, size_t n, size_t rows,

@@ -821,3 +821,28 @@ def test_embedding_grad_of_a_range_of_rows_of_a_larger_plan(mccl, n, hidden, ski
     within(out, want, tol + 2 * U * want.abs(), "range")
     if not accumulate:
         assert torch.equal(out, mccl.embedding_grad(up.to(DEV), (order, offsets))[first:first + count])
+
+
+@pytest.mark.parametrize("hidden", [24, 7, 2056])
+@pytest.mark.parametrize("way", ["any", "falling", "steps back"])
+def test_embedding_grad_adds_nothing_that_no_call_wrote(mccl, way, hidden):
+    """Offsets that no sort gives, over a workspace full of NaN: with rows of ones every result is a number of
+    gradient rows, so a whole number from 0 to n, or what was there before (zero here)."""
+    from torch_ccl_amd import capi
+    n, rows = 1000, 12
+    grad = torch.ones(n, hidden, device=DEV)
+    order = torch.randperm(n, generator=gen(82)).to(DEV)
+    ws = torch.empty(capi.lib().mccl_embedding_grad_workspace(n, hidden), dtype=torch.uint8, device=DEV)
+    for seed in range(40):
+        g = gen(83, seed)
+        offsets = torch.randint(-50, n + 100, (rows + 1,), generator=g)
+        if way == "falling":
+            offsets = torch.sort(offsets, descending=True).values
+        elif way == "steps back":
+            offsets = torch.sort(offsets).values
+            i = int(torch.randint(1, rows, (1,), generator=g))
+            offsets[i] -= 300
+        ws.fill_(255)
+        out = mccl.embedding_grad(grad, (order, offsets.to(DEV)), out=torch.zeros(rows, hidden, device=DEV), workspace=ws).cpu()
+        assert torch.isfinite(out).all(), (way, seed)
+        assert bool((out == out.round()).all()) and float(out.min()) >= 0 and float(out.max()) <= n, (way, seed)

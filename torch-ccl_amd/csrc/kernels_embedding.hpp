@@ -433,7 +433,7 @@ struct EmbeddingGradArgs {
   const int64_t* offsets;
   char* out;
   float* partial;        // [pieces][2][hidden]
-  uint32_t* long_row;    // [pieces]: the long row that begins in the piece, kNoRow if none does
+  uint32_t* long_row;    // [pieces][2]: the long rows whose sums the slots hold, kNoRow if none's
   uint32_t rows;
   uint32_t n;
   uint32_t piece_groups; // workgroups that take pieces: the first ones; 0 where no row can be longer than a piece
@@ -630,7 +630,7 @@ __global__ __launch_bounds__(kGradWaves * kWave) void embedding_grad_kernel(cons
     const uint32_t in_table = offset_at(a, a.rows);
     const uint32_t p0 = piece * kGradPiece;
     if (p0 >= a.n) return;
-    uint32_t begins = kNoRow;
+    uint32_t in_slot[2] = {kNoRow, kNoRow};
     if (p0 < in_table) {
       const uint32_t p1 = p0 + kGradPiece < in_table ? p0 + kGradPiece : in_table;
       const int index = token_at(a, p0 + lane, p1);
@@ -639,8 +639,8 @@ __global__ __launch_bounds__(kGradWaves * kWave) void embedding_grad_kernel(cons
       // Before the first row begins (the offsets of a range of rows of a larger plan) the search returns it all the same.
       const bool first_long = first_begin <= p0 && first_end - first_begin > kGradPiece;
       const bool last_long = last_begin > p0 && last_begin < p1 && offset_at(a, last + 1) - last_begin > kGradPiece;
-      if (last_long) begins = last;
-      else if (first_long && first_begin == p0) begins = first;
+      if (first_long) in_slot[0] = first;
+      if (last_long) in_slot[1] = last;
       for (uint32_t col = first_col; col < a.hidden; col += stride) {
         const GradColumns<DT, VL, SHORT> c(col + lane * VE, a.hidden);
         float* slot = a.partial + (size_t)piece * 2 * a.hidden;
@@ -654,13 +654,14 @@ __global__ __launch_bounds__(kGradWaves * kWave) void embedding_grad_kernel(cons
         }
       }
     }
-    if (lane == 0 && first_col == 0) a.long_row[piece] = begins;
+    if (lane < 2 && first_col == 0) a.long_row[piece * 2 + lane] = lane ? in_slot[1] : in_slot[0];
   }
 }
 
 // Adds the pieces of the long row that begins in a workgroup's piece, a chunk of columns per workgroup:
 // kJoinWaves wavefronts take every kJoinWaves-th piece each, kJoinLoads of them at a time, and their sums
-// are added in the order of the wavefronts.
+// are added in the order of the wavefronts.  Every piece of such a row but the one it begins in has it in slot 0; where
+// offsets fall one may not, and is left out.
 constexpr int kJoinWaves = 8;
 constexpr int kJoinLoads = 4;
 
@@ -670,19 +671,23 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void embedding_grad_join_kernel
   __shared__ float sum[kJoinWaves][VE * kWave];
   const uint32_t lane = threadIdx.x % kWave, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
   const uint32_t piece = blockIdx.x;
-  const uint32_t v = a.long_row[piece];
+  const uint32_t inside = a.long_row[piece * 2 + 1], v = inside != kNoRow ? inside : a.long_row[piece * 2];
   if (v == kNoRow) return;
   const uint32_t j0 = offset_at(a, v), j1 = offset_at(a, v + 1), last = (j1 - 1) / kGradPiece;
+  if (j0 / kGradPiece != piece) return;  // it begins in an earlier piece
   const GradColumns<DT, 1, SHORT> c((blockIdx.y * kWave + lane) * VE, a.hidden);
   float acc[1][VE];
 #pragma unroll
   for (int e = 0; e < VE; ++e) acc[0][e] = 0.0f;
-  const auto slot = [&](uint32_t p) { return a.partial + ((size_t)p * 2 + (p == piece && j0 != p * kGradPiece ? 1 : 0)) * a.hidden + c.col[0]; };
+  const auto slot_of = [&](uint32_t p) { return (size_t)p * 2 + (p == piece && inside != kNoRow ? 1 : 0); };
   const auto add = [&](auto count, uint32_t p) {
     float f[count][VE];
+    bool held[count];
 #pragma unroll
     for (int g = 0; g < count; ++g) {
-      const float* from = slot(p + g * kJoinWaves);
+      const size_t slot = slot_of(p + g * kJoinWaves);
+      const float* from = a.partial + slot * a.hidden + c.col[0];
+      held[g] = a.long_row[slot] == v;
 #pragma unroll
       for (int b = 0; b < VE; b += 4) {
         if constexpr (SHORT) {
@@ -699,7 +704,7 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void embedding_grad_join_kernel
 #pragma unroll
     for (int g = 0; g < count; ++g)
 #pragma unroll
-      for (int e = 0; e < VE; ++e) acc[0][e] += f[g][e];
+      for (int e = 0; e < VE; ++e) acc[0][e] += held[g] ? f[g][e] : 0.0f;
   };
   uint32_t p = piece + wave;
   for (; p + (kJoinLoads - 1) * kJoinWaves <= last; p += kJoinLoads * kJoinWaves) add(std::integral_constant<int, kJoinLoads>{}, p);

@@ -332,7 +332,7 @@ int mccl_sort_ids(const void* ids, int id_dtype, size_t n, int64_t first_row, si
   return launch_sort((const int64_t*)ids, n, first_row, rows, (char*)workspace, order, offsets, s);
 }
 
-size_t mccl_embedding_grad_workspace(size_t n, size_t hidden) { return grad_pieces(n) * (2 * hidden * sizeof(float) + sizeof(uint32_t)); }
+size_t mccl_embedding_grad_workspace(size_t n, size_t hidden) { return grad_pieces(n) * 2 * (hidden * sizeof(float) + sizeof(uint32_t)); }
 
 int mccl_embedding_grad(const void* grad, const int64_t* order, const int64_t* offsets, size_t n, size_t rows, size_t hidden,
                         float scale, int dtype, void* out, int out_dtype, int accumulate, void* workspace, size_t workspace_bytes,
