@@ -583,7 +583,8 @@ int mccl_moe_combine(const void* const* x, const size_t* x_rows, int n, const in
  * lies in [0, rows); a row of zeros elsewhere.  table: [rows][hidden], ids: int32 or int64 (id_dtype
  * MCCL_I32 / MCCL_I64), out: [n][hidden]; bf16 / f16 / f32, any row length, element alignment.  With
  * first_row a rank looks up its shard of a vocabulary and an all_reduce (SUM) adds the ranks' rows;
- * ids that mean nothing (-1 for padding) give zeros on every rank.
+ * ids that mean nothing (-1 for padding) give zeros on every rank.  first_row + rows is at most 2^63, here
+ * and in mccl_sort_ids.
  */
 int mccl_embedding(const void* table, size_t rows, const void* ids, int id_dtype, size_t n, int64_t first_row,
                    size_t hidden, float scale, int dtype, void* out, void* stream);

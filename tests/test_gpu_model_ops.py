@@ -846,3 +846,16 @@ def test_embedding_grad_adds_nothing_that_no_call_wrote(mccl, way, hidden):
         out = mccl.embedding_grad(grad, (order, offsets.to(DEV)), out=torch.zeros(rows, hidden, device=DEV), workspace=ws).cpu()
         assert torch.isfinite(out).all(), (way, seed)
         assert bool((out == out.round()).all()) and float(out.min()) >= 0 and float(out.max()) <= n, (way, seed)
+
+
+def test_a_shard_at_the_end_of_the_id_type(mccl):
+    info = torch.iinfo(torch.int64)
+    table = torch.arange(1.0, 6.0, device=DEV)[:, None].repeat(1, 8)
+    ids = torch.tensor([info.max, info.min, info.max - 3, info.min + 1, -1, 0], device=DEV)
+    assert mccl.embedding(table[:4], ids, first_row=info.max - 3)[:, 0].tolist() == [4, 0, 1, 0, 0, 0]
+    order, offsets = mccl.sort_ids(ids, 4, first_row=info.max - 3)
+    assert order.tolist() == [2, 0, 1, 3, 4, 5] and offsets.tolist() == [0, 1, 1, 1, 2]
+    with pytest.raises(RuntimeError, match="pass 2"):
+        mccl.embedding(table, ids, first_row=info.max - 3)
+    with pytest.raises(RuntimeError, match="pass 2"):
+        mccl.sort_ids(ids, 5, first_row=info.max - 3)

@@ -182,3 +182,23 @@ def test_the_front_end_refuses_what_it_is_not_for(mccl):
         mccl.moe_layer(x, w_in, w_out, ids, w[:, :1])
     with pytest.raises(RuntimeError, match="bf16 or f16"):
         mccl.moe_layer(x.float(), w_in, w_out, ids, w)
+
+
+def test_rows_past_the_largest_id_are_refused(abi):
+    """Their row numbers would wrap around to the smallest ids."""
+    L, capi, err = abi
+    last = (1 << 63) - 1
+
+    def embedding(first, rows, n=4):
+        return L.mccl_embedding(vp(0x10000000), rows, vp(0x20000000), capi.I64, n, first, 64, 1.0, capi.BF16, None, None)
+
+    def sort(first, rows):
+        return L.mccl_sort_ids(vp(0x10000001), capi.I64, 4, first, rows, None, 0, vp(0x20000000), vp(0x30000000), None)
+
+    for call, fits in ((embedding, "null"), (sort, "ids not aligned")):
+        for first, rows in ((last, 2), (last - 3, 5), (1, 1 << 63), (last // 2 + 2, last // 2 + 1)):
+            if call is sort and rows > 0x7fffffff:
+                continue
+            assert call(first, rows) == -1 and "pass 2^63" in err()
+        for first, rows in ((last, 1), (last - 3, 4), (last, 0), (-1, 10), (-last - 1, 10)):
+            assert call(first, rows) == -1 and fits in err()  # refused for something else that comes later

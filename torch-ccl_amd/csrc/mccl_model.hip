@@ -38,6 +38,13 @@ int check_ids(const void* ids, int id_dtype) {
   return MCCL_OK;
 }
 
+// The device counts an id's row modulo 2^64: with rows past the largest id, the smallest ones would come out inside.
+int check_rows(int64_t first_row, size_t rows) {
+  if (first_row > 0 && rows > (uint64_t)(INT64_MAX - first_row) + 1)
+    return mccl_report_error(MCCL_ERR_INVALID_ARG, "rows [%lld, +%zu) pass 2^63", (long long)first_row, rows);
+  return MCCL_OK;
+}
+
 size_t up16(size_t b) { return (b + 15) & ~(size_t)15; }
 
 int sort_passes(uint64_t rows) {
@@ -275,6 +282,7 @@ int mccl_embedding(const void* table, size_t rows, const void* ids, int id_dtype
   if (!es) return mccl_report_error(MCCL_ERR_UNSUPPORTED, "embedding is defined for bf16, f16 and f32");
   if (n == 0 || hidden == 0) return MCCL_OK;
   int rc = check_ids(ids, id_dtype);
+  if (rc == MCCL_OK) rc = check_rows(first_row, rows);
   if (rc != MCCL_OK) return rc;
   if (!out || (rows && !table)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "null pointer");
   if (misaligned(table, es) || misaligned(out, es)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "table or output not aligned to its element size");
@@ -313,8 +321,10 @@ int mccl_sort_ids(const void* ids, int id_dtype, size_t n, int64_t first_row, si
   if (n > 0x7fffffffull) return mccl_report_error(MCCL_ERR_INVALID_ARG, "too many ids");
   if (rows > 0x7fffffffull) return mccl_report_error(MCCL_ERR_INVALID_ARG, "too many rows");
   if (!offsets || misaligned(offsets, 8)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "offsets pointer is null or misaligned");
+  int rc = check_rows(first_row, rows);
+  if (rc != MCCL_OK) return rc;
   if (n) {
-    int rc = check_ids(ids, id_dtype);
+    rc = check_ids(ids, id_dtype);
     if (rc != MCCL_OK) return rc;
     if (!order || misaligned(order, 8)) return mccl_report_error(MCCL_ERR_INVALID_ARG, "order pointer is null or misaligned");
   }
