@@ -859,3 +859,46 @@ def test_a_shard_at_the_end_of_the_id_type(mccl):
         mccl.embedding(table, ids, first_row=info.max - 3)
     with pytest.raises(RuntimeError, match="pass 2"):
         mccl.sort_ids(ids, 5, first_row=info.max - 3)
+
+
+# ---------------------------------------------------------------------------------------------
+# autograd around the calls
+# ---------------------------------------------------------------------------------------------
+def calls_with_out(mccl, g):
+    """(name, tensors written, the call) of every operator that writes into tensors of the caller."""
+    table, ids = torch.randn(9, 16, generator=g).to(DEV), torch.randint(0, 9, (5,), generator=g).to(DEV)
+    logits = torch.randn(5, 8, generator=g).to(DEV)
+    x, w_in, w_out, chosen, w = [t.to(DEV) for t in layer_inputs(g, 5, 2, 8, 8, 16, 8, torch.bfloat16)]
+    plan = mccl.sort_ids(ids, 9)
+    outs = [torch.zeros(5, 16, device=DEV), torch.zeros(9, 16, device=DEV), torch.zeros(9, 16, device=DEV),
+            (torch.zeros(5, 2, dtype=torch.int32, device=DEV), torch.zeros(5, 2, device=DEV)), torch.zeros(5, 8, device=DEV), torch.zeros_like(x)]
+    up = torch.randn(5, 16, generator=g).to(DEV)
+    return [("embedding", outs[:1], lambda: mccl.embedding(table, ids, out=outs[0])),
+            ("embedding_grad", outs[1:2], lambda: mccl.embedding_grad(up, plan, out=outs[1])),
+            ("accumulate", outs[2:3], lambda: mccl.embedding_grad(up, plan, out=outs[2], accumulate=True)),
+            ("moe_route", list(outs[3]), lambda: mccl.moe_route(logits, 2, out=outs[3])),
+            ("moe_route_grad", outs[4:5], lambda: mccl.moe_route_grad(w, logits, chosen, out=outs[4])),
+            ("moe_layer", outs[5:6], lambda: mccl.moe_layer(x, w_in, w_out, chosen, w, out=outs[5]))]
+
+
+def test_writing_into_a_tensor_that_autograd_keeps_is_noticed(mccl):
+    for name, written, call in calls_with_out(mccl, gen(91)):
+        before = [t._version for t in written]
+        call()
+        assert all(t._version > b for t, b in zip(written, before)), name
+    out = torch.ones(5, 16, device=DEV)
+    leaf = torch.ones(5, 16, device=DEV, requires_grad=True)
+    loss = (leaf * out).sum()  # keeps out for leaf's gradient
+    mccl.embedding(torch.zeros(3, 16, device=DEV), torch.zeros(5, dtype=torch.int64, device=DEV), out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_tensors_of_inference_mode_are_written_too(mccl):
+    with torch.inference_mode():
+        calls = calls_with_out(mccl, gen(92))
+    for name, written, call in calls:
+        call()
+        with torch.inference_mode():
+            call()
+        assert all(t.is_inference() for t in written), name

@@ -111,6 +111,11 @@ struct Workspace {
   Tensor held;
 };
 
+// The caller's tensors have new values: autograd notices where it has kept one for a backward pass.
+void written(const MaybeTensor& given) {
+  if (given && !given->is_inference()) given->unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor embedding(const Tensor& table, const Tensor& ids, double scale, int64_t first_row, const MaybeTensor& given) {
   const char* what = "embedding";
   if (table.dim() != 2 || !is_float(table)) refuse(what, "table must be a matrix in bf16, f16 or f32");
@@ -123,6 +128,7 @@ Tensor embedding(const Tensor& table, const Tensor& ids, double scale, int64_t f
   const Tensor out = given ? *given : at::empty(shape, table.options().memory_format(std::nullopt));
   check(mccl_embedding(table.data_ptr(), table.size(0), ids.data_ptr(), code_of(ids.scalar_type()), ids.numel(), first_row, table.size(1),
                        (float)scale, code_of(table.scalar_type()), out.data_ptr(), on.stream));
+  written(given);
   return out;
 }
 
@@ -162,6 +168,7 @@ Tensor embedding_grad(const Tensor& grad, const Tensor& order, const Tensor& off
   const Workspace ws(what, workspace, mccl_embedding_grad_workspace(n, hidden), grad.device());
   check(mccl_embedding_grad(grad.data_ptr(), order.data_ptr<int64_t>(), offsets.data_ptr<int64_t>(), n, rows, hidden, (float)scale,
                             code_of(grad.scalar_type()), out.data_ptr(), code_of(type), accumulate, ws.data(), ws.size(), on.stream));
+  written(given);
   return out;
 }
 
@@ -179,6 +186,8 @@ std::tuple<Tensor, Tensor> moe_route(const Tensor& logits, int64_t topk, bool no
   const Tensor weights = given_weights ? *given_weights : at::empty({tokens, topk}, at::TensorOptions(at::kFloat).device(logits.device()));
   check(mccl_moe_route(logits.data_ptr(), tokens, logits.size(1), (int)topk, normalize, code_of(logits.scalar_type()),
                        ids.data_ptr<int32_t>(), weights.data_ptr<float>(), on.stream));
+  written(given_ids);
+  written(given_weights);
   return {ids, weights};
 }
 
@@ -195,6 +204,7 @@ Tensor moe_route_grad(const Tensor& grad_weights, const Tensor& logits, const Te
   const Tensor out = given ? *given : at::empty(logits.sizes(), logits.options().memory_format(std::nullopt));
   check(mccl_moe_route_grad(grad_weights.data_ptr<float>(), logits.data_ptr(), ids.data_ptr<int32_t>(), tokens, logits.size(1), (int)topk,
                             normalize, code_of(logits.scalar_type()), out.data_ptr(), on.stream));
+  written(given);
   return out;
 }
 
@@ -218,6 +228,7 @@ Tensor moe_layer(const Tensor& x, const Tensor& w_in, const Tensor& w_out, const
   check(mccl_moe_layer(x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), ids.data_ptr<int32_t>(), weights.data_ptr<float>(), tokens, (int)topk,
                        experts, first_expert, hidden, inter, activation == "silu" ? MCCL_ACT_SILU : MCCL_ACT_GELU, code_of(type),
                        out.data_ptr(), ws.data(), ws.size(), on.stream));
+  written(given);
   return out;
 }
 
