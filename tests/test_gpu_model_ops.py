@@ -902,3 +902,34 @@ def test_tensors_of_inference_mode_are_written_too(mccl):
         with torch.inference_mode():
             call()
         assert all(t.is_inference() for t in written), name
+
+
+def test_inputs_that_require_grad_are_told_that_they_get_none(mccl):
+    import warnings
+    g = gen(93)
+    table, ids = torch.randn(9, 16, generator=g).to(DEV), torch.randint(0, 9, (5,), generator=g).to(DEV)
+    logits, up = torch.randn(5, 8, generator=g).to(DEV), torch.randn(5, 16, generator=g).to(DEV)
+    x, w_in, w_out, chosen, w = [t.to(DEV) for t in layer_inputs(g, 5, 2, 8, 8, 16, 8, torch.bfloat16)]
+    plan = mccl.sort_ids(ids, 9)
+
+    def calls(want):
+        wants = lambda t, name: t.detach().requires_grad_(name == want)
+        return {"table": lambda: mccl.embedding(wants(table, "table"), ids),
+                "grad": lambda: mccl.embedding_grad(wants(up, "grad"), plan),
+                "logits": lambda: mccl.moe_route(wants(logits, "logits"), 2)[1],
+                "grad_weights": lambda: mccl.moe_route_grad(wants(w, "grad_weights"), logits, chosen),
+                "x": lambda: mccl.moe_layer(wants(x, "x"), w_in, w_out, chosen, w),
+                "w_in": lambda: mccl.moe_layer(x, wants(w_in, "w_in"), w_out, chosen, w),
+                "w_out": lambda: mccl.moe_layer(x, w_in, wants(w_out, "w_out"), chosen, w),
+                "weights": lambda: mccl.moe_layer(x, w_in, w_out, chosen, wants(w, "weights"))}
+
+    for name in calls(None):
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            alone = calls(None)[name]()
+            with torch.no_grad():
+                calls(name)[name]()
+            with pytest.raises(UserWarning, match="%s requires grad" % name):
+                calls(name)[name]()
+        with pytest.warns(UserWarning, match="no autograd node"):
+            assert torch.equal(calls(name)[name](), alone), name

@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <initializer_list>
@@ -83,6 +84,19 @@ void check_shape(const char* what, const char* name, const Tensor& t, at::IntArr
   refuse(what, why.str());
 }
 
+// The calls are no autograd nodes.  Who passes a tensor that wants a gradient, and has not switched gradients off, is told
+// so once per place in the program: the result has none.
+void check_grad(const char* what, std::initializer_list<Named> inputs) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Named& n : inputs) {
+    if (!n.t.requires_grad()) continue;
+    const std::string why = std::string(what) + ": " + n.name + " requires grad, but the call is no autograd node and its result has no "
+                            "gradient (gradients are calls of their own; torch.no_grad() or detach() says that none is meant)";
+    if (PyErr_WarnEx(PyExc_UserWarning, why.c_str(), 2)) throw py::error_already_set();
+    return;
+  }
+}
+
 void check(int rc) {
   if (rc != MCCL_OK) throw std::runtime_error("mccl error " + std::to_string(rc) + ": " + mccl_last_error());
 }
@@ -124,6 +138,7 @@ Tensor embedding(const Tensor& table, const Tensor& ids, double scale, int64_t f
   shape.push_back(table.size(1));
   if (given) check_shape(what, "out", *given, shape, {table.scalar_type()});
   check_gpu(what, {{"table", table}, {"ids", ids}, {"out", given ? *given : table}});
+  check_grad(what, {{"table", table}});
   const OnDevice on(table);
   const Tensor out = given ? *given : at::empty(shape, table.options().memory_format(std::nullopt));
   check(mccl_embedding(table.data_ptr(), table.size(0), ids.data_ptr(), code_of(ids.scalar_type()), ids.numel(), first_row, table.size(1),
@@ -163,6 +178,7 @@ Tensor embedding_grad(const Tensor& grad, const Tensor& order, const Tensor& off
   if (accumulate && !given) refuse(what, "accumulate needs the tensor to add to (out)");
   if (given) check_shape(what, "out", *given, {rows, hidden}, {type});
   check_gpu(what, {{"grad", grad}, {"order", order}, {"offsets", offsets}, {"out", given ? *given : grad}});
+  check_grad(what, {{"grad", grad}});
   const OnDevice on(grad);
   const Tensor out = given ? *given : at::empty({rows, hidden}, at::TensorOptions(type).device(grad.device()));
   const Workspace ws(what, workspace, mccl_embedding_grad_workspace(n, hidden), grad.device());
@@ -181,6 +197,7 @@ std::tuple<Tensor, Tensor> moe_route(const Tensor& logits, int64_t topk, bool no
   if (given_ids) check_shape(what, "expert_ids", *given_ids, {tokens, topk}, {at::kInt});
   if (given_weights) check_shape(what, "weights", *given_weights, {tokens, topk}, {at::kFloat});
   check_gpu(what, {{"logits", logits}, {"expert_ids", given_ids ? *given_ids : logits}, {"weights", given_weights ? *given_weights : logits}});
+  check_grad(what, {{"logits", logits}});
   const OnDevice on(logits);
   const Tensor ids = given_ids ? *given_ids : at::empty({tokens, topk}, at::TensorOptions(at::kInt).device(logits.device()));
   const Tensor weights = given_weights ? *given_weights : at::empty({tokens, topk}, at::TensorOptions(at::kFloat).device(logits.device()));
@@ -200,6 +217,7 @@ Tensor moe_route_grad(const Tensor& grad_weights, const Tensor& logits, const Te
   check_shape(what, "grad_weights", grad_weights, {tokens, topk}, {at::kFloat});
   if (given) check_shape(what, "out", *given, logits.sizes(), {logits.scalar_type()});
   check_gpu(what, {{"grad_weights", grad_weights}, {"logits", logits}, {"expert_ids", ids}, {"out", given ? *given : logits}});
+  check_grad(what, {{"grad_weights", grad_weights}, {"logits", logits}});
   const OnDevice on(logits);
   const Tensor out = given ? *given : at::empty(logits.sizes(), logits.options().memory_format(std::nullopt));
   check(mccl_moe_route_grad(grad_weights.data_ptr<float>(), logits.data_ptr(), ids.data_ptr<int32_t>(), tokens, logits.size(1), (int)topk,
@@ -222,6 +240,7 @@ Tensor moe_layer(const Tensor& x, const Tensor& w_in, const Tensor& w_out, const
   check_shape(what, "weights", weights, {tokens, topk}, {at::kFloat});
   if (given) check_shape(what, "out", *given, x.sizes(), {type});
   check_gpu(what, {{"x", x}, {"w_in", w_in}, {"w_out", w_out}, {"expert_ids", ids}, {"weights", weights}, {"out", given ? *given : x}});
+  check_grad(what, {{"x", x}, {"w_in", w_in}, {"w_out", w_out}, {"weights", weights}});
   const OnDevice on(x);
   const Tensor out = given ? *given : at::empty({tokens, hidden}, at::TensorOptions(type).device(x.device()));
   const Workspace ws(what, workspace, mccl_moe_layer_workspace(tokens, (int)topk, experts, hidden, inter), x.device());

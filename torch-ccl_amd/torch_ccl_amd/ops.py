@@ -288,7 +288,8 @@ def route_counts(expert_ids, n_experts, workspace=None, out=None):
 
 # The operators that compute around the collectives.  Their checks, allocations and the call of the C ABI on
 # the current stream of the tensors' device are in the extension: these calls are short enough for the
-# interpreter's share to matter.
+# interpreter's share to matter.  They are no autograd nodes: gradients are calls of their own, and a call with
+# a tensor that requires grad, outside torch.no_grad(), warns that its result has none.
 
 def embedding(table, ids, scale=1.0, first_row=0, out=None):
     """out[..., :] = scale * table[ids - first_row] where that row lies in the table, zeros elsewhere
