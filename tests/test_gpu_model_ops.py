@@ -933,3 +933,24 @@ def test_inputs_that_require_grad_are_told_that_they_get_none(mccl):
                 calls(name)[name]()
         with pytest.warns(UserWarning, match="no autograd node"):
             assert torch.equal(calls(name)[name](), alone), name
+
+
+def test_moe_layer_on_a_rank_without_experts_is_zero(mccl):
+    """Its part of the all_reduce, also into a tensor of the caller and from a graph."""
+    x, w_in, w_out, ids, weights = [t.to(DEV) for t in layer_inputs(gen(94), 6, 2, 4, 4, 64, 40, torch.bfloat16)]
+    none = (w_in[:0], w_out[:0])
+    assert mccl.moe_layer(x, *none, ids, weights).shape == x.shape and not mccl.moe_layer(x, *none, ids, weights, first_expert=4).any()
+    out = torch.full_like(x, 5.0)
+    assert mccl.moe_layer(x, *none, ids, weights, out=out).data_ptr() == out.data_ptr() and not out.any()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mccl.moe_layer(x, *none, ids, weights, out=out)
+    for _ in range(3):
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not out.any()
+    with pytest.raises(RuntimeError, match="w_in must be"):
+        mccl.moe_layer(x, w_in, w_out[:0], ids, weights)
+    with pytest.raises(RuntimeError, match="at most 256"):  # as on the ranks that hold some
+        mccl.moe_layer(x[:1].repeat(257, 1), *none, ids[:1].repeat(257, 1), weights[:1].repeat(257, 1))

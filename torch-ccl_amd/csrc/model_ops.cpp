@@ -243,9 +243,15 @@ Tensor moe_layer(const Tensor& x, const Tensor& w_in, const Tensor& w_out, const
   check_grad(what, {{"x", x}, {"w_in", w_in}, {"w_out", w_out}, {"weights", weights}});
   const OnDevice on(x);
   const Tensor out = given ? *given : at::empty({tokens, hidden}, at::TensorOptions(type).device(x.device()));
+  const int act = activation == "silu" ? MCCL_ACT_SILU : MCCL_ACT_GELU;
+  if (experts == 0) {  // a rank that holds none: zeros for the sum, within the limits on tokens that the other ranks have
+    check(mccl_moe_layer(nullptr, nullptr, nullptr, nullptr, nullptr, tokens, (int)topk, 1, first_expert, 0, inter, act, code_of(type), nullptr,
+                         nullptr, 0, on.stream));
+    return out.zero_();
+  }
   const Workspace ws(what, workspace, mccl_moe_layer_workspace(tokens, (int)topk, experts, hidden, inter), x.device());
   check(mccl_moe_layer(x.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), ids.data_ptr<int32_t>(), weights.data_ptr<float>(), tokens, (int)topk,
-                       experts, first_expert, hidden, inter, activation == "silu" ? MCCL_ACT_SILU : MCCL_ACT_GELU, code_of(type),
+                       experts, first_expert, hidden, inter, act, code_of(type),
                        out.data_ptr(), ws.data(), ws.size(), on.stream));
   written(given);
   return out;

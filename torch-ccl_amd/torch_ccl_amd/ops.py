@@ -335,7 +335,7 @@ def moe_layer(x, w_in, w_out, expert_ids, weights, first_expert=0, activation="s
     """A mixture-of-experts layer for a few tokens (at most 256), routing already made (moe_route):
     out[t] = sum_k weights[t, k] * w_out[e] @ (act(w_in[e, :inter] @ x[t]) * (w_in[e, inter:] @ x[t])) with
     e = expert_ids[t, k] - first_expert, over the experts this rank holds; an all_reduce adds the ranks'
-    parts.  x [tokens, hidden], w_in [experts, 2 * inter, hidden], w_out [experts, hidden, inter] in bf16
+    parts, zeros from one that holds none.  x [tokens, hidden], w_in [experts, 2 * inter, hidden], w_out [experts, hidden, inter] in bf16
     or f16; activation "silu" or "gelu" (exact)."""
     return _C.moe_layer(x, w_in, w_out, expert_ids, weights, first_expert, activation, out, workspace)
 
