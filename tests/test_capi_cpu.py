@@ -365,3 +365,18 @@ def test_ctypes_structures_match_the_header(mccl, tmp_path):
         ctype, fields = layouts[cname]
         assert ctypes.sizeof(ctype) == int(size), cname
         assert [getattr(ctype, f).offset for f in fields] == [int(o) for o in offsets], cname
+
+
+@pytest.mark.parametrize("kernel,allowed", [("sort_offsets_kernel", False), ("embedding_kernelILi8ExLb0EE", False), ("embedding_grad_kernelILi8ELi6ELi2ELb0EE", False),
+                                            ("embedding_grad_join_kernelILi8ELi6ELb0EE", False), ("layer_out_kernelILi8ELi2ELi8EE", False),
+                                            ("layer_join_kernelILi8EE", False), ("layer_in_kernelILi8ELi8EE", True), ("layer_dense_kernelILi8ELb1EE", True),
+                                            ("router_kernelILi8ELi16ELi16EE", True), ("router_grad_kernelILi8ELi16ELi16EE", True)])
+def test_isa_guard_lets_only_kernels_with_exp_fuse(tmp_path, kernel, allowed):
+    """Sums and scalings round on their own in every kernel that evaluates no exp, erf or division."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("check_isa", os.path.join(PKG, "csrc", "check_isa.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    asm = tmp_path / "kernel.s"
+    asm.write_text("_ZN12_GLOBAL__N_1%d%s:\n\tv_add_f32_e32 v0, v1, v2\n\tv_fma_f32 v0, v1, v2, v3\n" % (len(kernel), kernel))
+    assert bool(mod.scan(str(asm))) != allowed

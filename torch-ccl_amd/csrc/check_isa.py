@@ -9,7 +9,8 @@ arithmetic instruction rather than a compare or mask operation.
 The same scan enforces two numeric rules of the kernels: no packed-fp32 arithmetic
 (v_pk_add/mul/fma_f32) anywhere, and no fused multiply-add outside the AVG kernels (whose
 division by the rank count expands to a correctly rounded sequence that uses v_fma_f32) and the
-kernels that evaluate exp, erf and divisions (embedding, router, mixture-of-experts layer): every
+kernels that evaluate exp, erf and divisions (router and its gradient, the activation of the
+mixture-of-experts layer): every
 add and every product of the reduction chains must round on its own.  Scratch (register spill)
 instructions are flagged as well.
 
@@ -49,7 +50,7 @@ _PACKED = re.compile(r"^v_pk_(add|mul|fma)_f32")
 _FMA = re.compile(r"^(v_fma_f32|v_fmac_f32|v_mad_f32|v_fma_f64|v_fmac_f64)")
 _AVG_KERNEL = re.compile(r"(reduce_(vec|elem)_kernel|allreduce_fused_kernel|xrank_reduce_kernel)ILi\d+ELi1E")  # second template argument = MCCL_AVG
 # exp, erf, divisions and the polynomials they expand to fuse by design; the order of their sums is set in the source
-_MODEL_KERNEL = re.compile(r"(embedding\w*_kernel|sort_\w+_kernel|router\w*_kernel|layer_\w+_kernel)")
+_EXP_KERNEL = re.compile(r"(router(_grad)?|layer_in|layer_dense)_kernel")
 _SCRATCH = re.compile(r"^scratch_")
 
 
@@ -89,7 +90,7 @@ def scan(asm_path):
             op = t.split()[0]
             if _PACKED.match(op):
                 flagged.append((ln, t, "packed fp32 arithmetic", fn))
-            if _FMA.match(op) and not _AVG_KERNEL.search(fn or "") and not _MODEL_KERNEL.search(fn or ""):
+            if _FMA.match(op) and not _AVG_KERNEL.search(fn or "") and not _EXP_KERNEL.search(fn or ""):
                 flagged.append((ln, t, "fused multiply-add outside the AVG kernels", fn))
             if _SCRATCH.match(op):
                 flagged.append((ln, t, "scratch access (register spill)", fn))
