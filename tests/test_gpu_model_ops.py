@@ -954,3 +954,65 @@ def test_moe_layer_on_a_rank_without_experts_is_zero(mccl):
         mccl.moe_layer(x, w_in, w_out[:0], ids, weights)
     with pytest.raises(RuntimeError, match="at most 256"):  # as on the ranks that hold some
         mccl.moe_layer(x[:1].repeat(257, 1), *none, ids[:1].repeat(257, 1), weights[:1].repeat(257, 1))
+
+
+# ---------------------------------------------------------------------------------------------
+# sizes at which a call takes another way
+# ---------------------------------------------------------------------------------------------
+def unevenly(g, T, k, E, hot):
+    """ids [T, k]: the first `hot` tokens have expert 1 among their choices, no other token has; choices differ."""
+    ids = torch.argsort(torch.rand(T, E, generator=g), dim=1)[:, :k]
+    for t in range(T):
+        row = [int(e) for e in ids[t] if e != 1]
+        row += [e for e in range(2, E) if e not in row]
+        ids[t] = torch.tensor(([1] if t < hot else []) + row)[:k] if E > 1 else 0
+    return ids.to(torch.int32).contiguous()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("T,k,E,hot,H,I", [
+    # through LDS: one tile and two of an expert's tokens, over 3 and 4 (and 5) chunks of 128 columns of either product,
+    # turns of 128 and of 64 columns, one or more parts of inter
+    (256, 1, 1, 256, 392, 520), (129, 1, 1, 129, 520, 392), (128, 1, 1, 128, 264, 640), (65, 1, 1, 65, 640, 264), (64, 1, 1, 64, 520, 520),
+    (256, 2, 3, 200, 136, 264), (150, 2, 6, 67, 400, 136), (13, 1, 1, 13, 264, 1160),
+    # from memory: an expert with more pairs than one list holds, more than 32, 16, 8 and 4 of them
+    (256, 8, 200, 256, 72, 40), (130, 4, 60, 130, 136, 72), (100, 4, 64, 65, 72, 136), (40, 4, 30, 33, 136, 72), (40, 4, 30, 17, 72, 72),
+    (20, 4, 30, 9, 136, 200), (20, 4, 30, 5, 264, 72)])
+def test_moe_layer_of_uneven_experts(mccl, dtype, T, k, E, hot, H, I):
+    g = gen(95, T, k, E, hot, H, I)
+    x, w_in, w_out, _, weights = layer_inputs(g, T, k, E, E, H, I, dtype)
+    ids = unevenly(g, T, k, E, hot)
+    assert int((ids == min(1, E - 1)).sum()) == hot
+    out = torch.full((T, H), float("nan"), dtype=dtype, device=DEV)
+    mccl.moe_layer(x.to(DEV), w_in.to(DEV), w_out.to(DEV), ids.to(DEV), weights.to(DEV), out=out)
+    want, tol = layer_reference_unrounded(x, w_in, w_out, ids, weights, 0, "silu", dtype)
+    within(out, want, tol, "layer")
+
+
+@pytest.mark.parametrize("T,k,E,local,first", [(1, 8, 64, 8, 16), (8, 8, 64, 8, 0), (60, 8, 64, 8, 24), (70, 8, 64, 8, 56), (256, 8, 64, 8, 8), (256, 8, 64, 1, 63)])
+def test_moe_layer_on_a_shard_at_every_batch(mccl, T, k, E, local, first):
+    """Most pairs are other ranks' experts; the workspace holds NaN where nothing of this rank is written."""
+    from torch_ccl_amd import capi
+    H, I, dtype = 136, 264, torch.bfloat16
+    x, w_in, w_out, ids, weights = layer_inputs(gen(96, T, local, first), T, k, E, local, H, I, dtype)
+    ws = torch.full((capi.lib().mccl_moe_layer_workspace(T, k, local, H, I),), 255, dtype=torch.uint8, device=DEV)
+    out = mccl.moe_layer(x.to(DEV), w_in.to(DEV), w_out.to(DEV), ids.to(DEV), weights.to(DEV), first_expert=first, workspace=ws)
+    want, tol = layer_reference_unrounded(x, w_in, w_out, ids, weights, first, "silu", dtype)
+    within(out, want, tol, "layer")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_embedding_grad_gives_a_columns_bits_whatever_is_beside_it(mccl, dtype):
+    """The columns of a wide row, which one wavefront takes two chunks of, alone: one chunk, spread over workgroups, or
+    shorter than a vector.  The order of a column's sum depends on the offsets alone."""
+    g = gen(97)
+    n, rows, hidden = 3000, 6000, 4 * 512 + 8 * 64 + 24
+    ids = torch.randint(0, rows, (n,), generator=g)
+    ids[torch.rand(n, generator=g) < 0.3] = 1234
+    ids[torch.rand(n, generator=g) < 0.1] = 7
+    up = torch.randn(n, hidden, generator=g).to(dtype).to(DEV)
+    plan = mccl.sort_ids(ids.to(DEV), rows)
+    wide = mccl.embedding_grad(up, plan, scale=0.75)
+    for first, count in ((0, 512), (0, 2048), (512, 1032), (hidden - 24, 24), (hidden - 3, 3), (77, 1), (100, 513)):
+        part = mccl.embedding_grad(up[:, first:first + count].contiguous(), plan, scale=0.75)
+        assert torch.equal(part, wide[:, first:first + count]), (first, count)
