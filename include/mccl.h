@@ -646,8 +646,9 @@ int mccl_moe_route_grad(const float* grad_weights, const void* logits, const int
  * into the second product over fp32's range and within 2^-16 of itself, so the output's rounding is the
  * only one to the type.
  * Every rank that holds `experts` experts from first_expert on calls it with all tokens, and an
- * all_reduce (SUM) adds the ranks' outputs.  At most 256 tokens, topk <= 64 and 4096 pairs: each
- * expert's weights are read once for all of its tokens.  The same bits every time.
+ * all_reduce (SUM) adds the ranks' outputs.  At most 256 tokens, topk <= 64 and 4096 pairs: an
+ * expert's weights are read once for up to 16 of its tokens, w_in for up to 32, and both for up to 128 where
+ * there are more than 12 pairs per expert.  The same bits every time.
  * workspace: mccl_moe_layer_workspace(...) bytes.
  */
 typedef enum {

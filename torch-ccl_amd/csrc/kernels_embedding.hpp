@@ -99,7 +99,7 @@ constexpr int kLookupWaves = 4;
 // that is no whole number of them begins early enough to be whole (its first elements are written twice,
 // with the same values).  Rows shorter than a vector, and a table without rows, take the SHORT form.
 // Bound by memory, the output's share by far the larger (a word's row is in the caches after its first use):
-// 32768 rows of 7168 bf16 115 us, 5.2 TB/s of what has to move; 8 rows of 4096 take 2.6 us, which is a launch and two
+// 32768 rows of 7168 bf16 115 us (118 alone), 5.2 TB/s of what has to move; 8 rows of 4096 take 2.6 us, which is a launch and two
 // loads that depend on each other.  Stores past the caches: rows of the table stay in them.
 template <int DT, typename ID, bool SHORT>
 __global__ __launch_bounds__(kLookupWaves * kWave) void embedding_kernel(const EmbeddingArgs a) {

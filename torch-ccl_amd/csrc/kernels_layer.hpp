@@ -1,5 +1,6 @@
-// A whole mixture-of-experts layer for a few tokens (no kernel of the reference): every expert that a
-// token of the batch was routed to is read once, for all of its tokens.
+// A whole mixture-of-experts layer for a few tokens (no kernel of the reference): every expert that a token of
+// the batch was routed to is read once for up to 32 of its tokens (its second product: 16), or for up to 128 where
+// tokens go through LDS.
 #pragma once
 
 #include "kernels_common.hpp"
@@ -138,7 +139,7 @@ __device__ __forceinline__ f32x2 add_halves(f32x4 v) { return (f32x2){v[0] + fro
 constexpr uint32_t kOutside = 0x80000000u;
 constexpr size_t kLayerMaxColumns = 1u << 17;          // hidden and inter: 4096 pairs of a part of h are 1 GiB
 constexpr size_t kLayerMaxExpert = kOutside - 65536u;  // bytes of an expert's w_in
-constexpr int kStreamed = 2;  // non-temporal: weights are read once
+constexpr int kStreamed = 2;  // non-temporal: weights are not read again soon
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t matrix_at(const char* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, (int)bytes, 0x00020000);
@@ -423,8 +424,8 @@ __global__ __launch_bounds__(WAVES * kWave) void layer_out_kernel(const LayerArg
 // product: 64 gate rows and their up rows) or one part of inter (second product: 128 rows).  Its tokens go
 // through LDS, a chunk of columns of 128 of them at a time.  While a chunk is multiplied, the rows and tokens of the
 // next one are on their way into registers.
-// 160 tokens on 8 experts of 4096 x 7168 f16, 40 each: 194 us for the first product (4.9 TB/s, 194 TFLOP/s) and 147 for
-// the second (3.2 TB/s); 96 tokens on each of 2 experts of 4096 x 8192 bf16 122 us in all.  Two workgroups fit on a
+// 160 tokens on 8 experts of 4096 x 7168 f16, 40 each: 192 us for the first product (4.9 TB/s, 196 TFLOP/s) and 143 for
+// the second (3.3 TB/s); 96 tokens on each of 2 experts of 4096 x 8192 bf16 122 us in all.  Two workgroups fit on a
 // compute unit by registers (128) and LDS (80 KiB); with the products of few tokens, half of whose sums are not used,
 // it was one and the layer took a tenth longer.
 // What is lost is a workgroup's start and end, the join, and in the second product the turns, whose tokens are twice

@@ -118,7 +118,8 @@ __device__ __forceinline__ void load_logits(const typename Elem<DT>::store_t* ro
 // the largest, and in it the first.  The weights need no more than fp32 of the logits: one exp per choice (and
 // per expert where they are not normalised), fp32 sums.
 // Bound by the vector instructions of the selection, not by memory: 32768 tokens x 256 experts bf16, 8 choices,
-// 11.3 us, where reading them takes 2.8 (1.7 TB/s); 16 tokens 3.5 us, one wavefront's time.
+// 11.4 us back to back and 13.1 alone, where reading them takes 2.8; fp32, with a ballot and a removal for every choice,
+// 18.2 back to back; 16 tokens 3.5 us, one wavefront's time.
 template <int DT, int LANES, int PER>
 __global__ __launch_bounds__(kRouterWaves * kWave) void router_kernel(const RouterArgs a) {
   using S = typename Elem<DT>::store_t;
@@ -214,8 +215,8 @@ __global__ __launch_bounds__(kRouterWaves * kWave) void router_kernel(const Rout
 //   normalised (w = softmax of the chosen): d_e = [e chosen] w_e (g_e - s)
 // LANES lanes per token as in router_kernel; what the chosen experts get goes through LDS to the lanes that
 // write it.  p is made again from the logits, which costs less than keeping it: 32768 tokens x 256 experts bf16
-// 11.2 us for 36 MB (3.2 TB/s), not normalised fp32 14.1 us for 69 MB (4.9 TB/s).  Normalised, all logits are read for a NaN
-// alone, which makes the weights NaN wherever it stands (10.2 us if only the chosen ones are).
+// 11.2 us back to back for 36 MB (3.2 TB/s) and 9.8 alone, not normalised fp32 14.1 us for 69 MB (4.9 TB/s).  Normalised,
+// all logits are read for a NaN alone, which makes the weights NaN wherever it stands (10.2 us if only the chosen are).
 template <int DT, int LANES, int PER>
 __global__ __launch_bounds__(kRouterWaves * kWave) void router_grad_kernel(const RouterArgs a) {
   using S = typename Elem<DT>::store_t;

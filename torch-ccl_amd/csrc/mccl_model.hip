@@ -158,13 +158,13 @@ void launch_route(const RouterArgs& a, hipStream_t s) {
                      dim3(std::min(kMaxGroups, (a.tokens + per_group - 1) / per_group)), dim3(kRouterWaves * kWave), 0, s, a);
 }
 
-// A batch takes 16 lanes per token, of 16 experts at most: 32768 tokens x 256 experts bf16 11.6 us and 10.1 for the
-// gradient, against 18.7 and 11.9 with a wavefront per token; x 64 experts 6.3 and 5.3 against 13.7 and 8.4.  Few
+// A batch takes 16 lanes per token, of 16 experts at most: 32768 tokens x 256 experts bf16 11.4 us and 11.2 for the
+// gradient, against 18.4 and 13.0 with a wavefront per token; x 64 experts 6.2 and 5.3 against 13.6 and 9.2.  Few
 // tokens are bound by one wavefront's time, which is shorter where it has one token and less per lane: 256 tokens x
-// 256 experts 3.3 us against 3.9.  They meet at 4096 tokens (4.2 against 4.6, the gradient 4.0 against 3.7; 2048
-// tokens 4.0 against 3.7; x 128 experts 3.3 against 3.5).  16 experts of fp32 are a cache line's half per lane, which
-// the gradient, reading and writing them, does slower than a wavefront per token: 32768 x 256 18.7 us against 14.5
-// (x 128 9.1 against 11.5).
+// 256 experts 3.2 and 2.7 us against 3.9 and 3.7.  They meet at 4096 tokens (4.1 against 4.5, the gradient 4.1 against
+// 3.5; 2048 tokens 4.0 against 3.6 and 3.9 against 2.9; 4096 x 128 experts 3.3 against 4.1).  16 experts of fp32 are a
+// cache line's half per lane, which the gradient, reading and writing them, does slower than a wavefront per token (not
+// normalised, 32768 x 256 18.7 us against 14.1), unlike 8 of them (x 128 10.1 against 11.7).
 constexpr uint32_t kRouterBatch = 4096;
 
 template <int DT, bool GRAD>
