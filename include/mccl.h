@@ -643,8 +643,8 @@ int mccl_moe_route_grad(const float* grad_weights, const void* logits, const int
  * rounding; a token without any gets zeros.  x, out: [tokens][hidden]; w_in: [experts][2 * inter][hidden];
  * w_out: [experts][hidden][inter]; bf16 or f16, hidden and inter multiples of 8 up to 2^17, 16-byte
  * aligned, an expert's w_in at most 2 GiB - 64 KiB.  Sums and the activation are fp32; act(..) * (..) goes
- * into the second product over fp32's range and within 2^-16 of itself, so the output's rounding is the
- * only one to the type.
+ * into the second product over fp32's range and within 2^-16 of itself (from 2^-110 on), so the output's
+ * rounding is the only one to the type.
  * Every rank that holds `experts` experts from first_expert on calls it with all tokens, and an
  * all_reduce (SUM) adds the ranks' outputs.  At most 256 tokens, topk <= 64 and 4096 pairs: an
  * expert's weights are read once for up to 16 of its tokens, w_in for up to 32, and both for up to 128 where

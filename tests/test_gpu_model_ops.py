@@ -1016,3 +1016,20 @@ def test_embedding_grad_gives_a_columns_bits_whatever_is_beside_it(mccl, dtype):
     for first, count in ((0, 512), (0, 2048), (512, 1032), (hidden - 24, 24), (hidden - 3, 3), (77, 1), (100, 513)):
         part = mccl.embedding_grad(up[:, first:first + count].contiguous(), plan, scale=0.75)
         assert torch.equal(part, wide[:, first:first + count]), (first, count)
+
+
+@pytest.mark.parametrize("T", [1, 6, 20])
+@pytest.mark.parametrize("power", [40, 54, 55, 56, 58, 60, 61, 62])
+def test_moe_layer_of_very_small_values(mccl, T, power):
+    """gate = up = 2^-power: silu's half of that times up is 2^-(2 power + 1), exactly (exp(-gate) is 1), down to the
+    smallest normal numbers of bf16; so is the output."""
+    H, I = 8, 8
+    x = torch.zeros(T, H, dtype=torch.bfloat16)
+    x[:, 3] = 2.0 ** -power
+    w_in, w_out = torch.zeros(1, 2 * I, H, dtype=torch.bfloat16), torch.zeros(1, H, I, dtype=torch.bfloat16)
+    w_in[0, :, 3], w_out[0, 5, 6] = 1.0, 1.0
+    ids, weights = torch.zeros(T, 1, dtype=torch.int32), torch.ones(T, 1)
+    out = mccl.moe_layer(*[t.to(DEV) for t in (x, w_in, w_out, ids, weights)]).cpu().double()
+    want = torch.zeros(T, H, dtype=torch.float64)
+    want[:, 5] = 2.0 ** -(2 * power + 1)
+    assert torch.equal(out, want)

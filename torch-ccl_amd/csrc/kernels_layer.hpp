@@ -63,8 +63,9 @@ __device__ __forceinline__ float activate(float v, int activation) {
 // layer's type, it made the result's error 1.4 times that of its own last rounding (0.0024 against 0.0017 in bf16), and
 // in f16 infinite above 65504.  So h is kept as the sum of two bf16: its upper 8 significant bits as they are, and what they leave,
 // rounded: 2^-16 of h at the most, over fp32's range.  The second product adds the products of both parts.
-// Where nothing is left (h has 8 bits, or is infinite) the low part is the smallest normal number of h's sign, so that
-// an infinite weight meets no zero that h does not have; what it adds elsewhere is below 2^-100 of any weight's.
+// Where nothing is left (h has 8 bits, or is infinite) the low part is the smallest normal number of h's sign, 2^-126, so
+// that an infinite weight meets no zero that h does not have; from 2^-110 on that is below 2^-16 of h as well, and
+// smaller ones are left as they are.
 // That costs nothing for up to 4 pairs of an expert (1 token 36.4 us for the layer with and without, 32 tokens on an
 // expert-parallel shard 213 and 212) and up to a tenth for more in bf16 (64 tokens on 128 experts 322 and 302, 160 on 8
 // wide ones 307 and 287); the f16 weights' split a few percent more.
@@ -74,7 +75,7 @@ struct Parts {
 __device__ __forceinline__ Parts split(float h) {
   const uint32_t bits = f32_to_bits(h), high = bits >> 16;
   const float rest = h - bits_to_f32(high << 16);
-  const uint32_t least = (high & 0x8000u) | ((high & 0x7fffu) ? 0x0080u : 0u);
+  const uint32_t least = (high & 0x8000u) | ((high & 0x7fffu) >= (127u - 110u) << 7 ? 0x0080u : 0u);
   return {(uint16_t)high, rest < 0.0f || rest > 0.0f ? Elem<MCCL_BF16>::store(rest) : (uint16_t)least};
 }
 
